@@ -117,6 +117,8 @@ def build_kernels(force: bool = False, verbose: bool = False, jobs: int | None =
         "-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-D__HIP_PLATFORM_AMD__=1",
         "-DUSE_ROCM=1", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi, "-DTORCH_API_INCLUDE_EXTENSION_H",
         "-Wno-unused-result", "-Wno-deprecated-declarations", "-Wno-unused-command-line-argument",
+        # no packed fp32 arithmetic (v_pk_{add,mul,fma}_f32): some of its forms have returned wrong values
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-I" + os.path.join(CSRC, "kernels"), *["-I" + p for p in tinc],
     ]
     if os.environ.get("MIHVD_SAVE_TEMPS"):
