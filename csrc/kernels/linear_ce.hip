@@ -1,0 +1,338 @@
+// Softmax cross entropy of a vocabulary projection, without keeping the logits.
+//
+//   z = h W^T + b;   L_r = lse_r - z[r][y_r],  lse_r = log sum_v exp(z[r][v])
+//   dz = g_r (exp(z - lse) - onehot);  dh = dz W;  dW = dz^T h;  db = sum_r dz
+//
+// Forward: the logits exist only as MFMA accumulators; every wave reduces its columns of a row to a
+// running (max, sum of exp) pair in fp32 and writes that pair, and the row's own label logit where
+// it holds it. A second kernel joins the pairs of a row. Backward recomputes the logits piece by
+// piece of the vocabulary, writes dz of the piece in 16 bits (the operand format of the two products
+// that follow), and multiplies it into dW (that piece's rows, final) and dh (fp32 slabs, summed over
+// pieces and k splits in a fixed order). No atomics: results repeat bit for bit.
+//
+// Rows whose label is `ignore_index` are dropped before anything is multiplied: the labelled rows
+// are compacted (their count stays on the device), so a masked-LM head over all positions costs what
+// its masked positions cost.
+//
+// dz is held as (exp(z - lse) - onehot) * (g_r / G) * 2^shift with G = max |g_r|; G and 2^-shift come
+// back in the epilogues. bf16 needs no shift; fp16 takes 2^14, so that probabilities down to 4e-9
+// stay normal numbers (fp16's smallest is 6e-5) and 1.0 stays far from 65504.
+#include "gemm16.h"
+
+#include "transformer.h"
+
+MIHVD_OPNS_BEGIN
+
+namespace {
+#ifdef MIHVD_F16
+constexpr float DZ_SCALE = 16384.f;
+#else
+constexpr float DZ_SCALE = 1.f;
+#endif
+
+// Row r of the compact hidden matrix; one wave per row, 16 bytes a lane where the row allows it.
+__global__ void __launch_bounds__(256) lce_gather(const u16* __restrict__ h, int64_t s0, int64_t s1,
+                                                  const int* __restrict__ idx, const int* __restrict__ cnt, int K, int K8,
+                                                  u16* __restrict__ out) {
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= *cnt) return;
+  const u16* src = h + (int64_t)idx[r] * s0;
+  u16* dst = out + (int64_t)r * K8;
+  if (s1 == 1 && (s0 & 7) == 0 && ((uintptr_t)h & 15) == 0 && K == K8) {
+    for (int k = lane * 8; k < K; k += 512) *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
+  } else {
+    for (int k = lane; k < K8; k += 64) dst[k] = k < K ? src[(int64_t)k * s1] : (u16)0;
+  }
+}
+
+__device__ __forceinline__ float bias_at(const void* b, int kind, int n) {
+  return kind == 0 ? 0.f : kind == 1 ? static_cast<const float*>(b)[n] : bf2f(static_cast<const u16*>(b)[n]);
+}
+
+// Statistics of one wave's columns: part[row][2 * pieces] = (max, sum of exp(z - max)).
+struct EpiStats {
+  const void* bias;
+  int bias_kind;
+  const int* label;   // compact labels
+  float2* part;       // [rows][npart]
+  int npart;
+  float* zlab;        // [rows]
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+    const int g4 = 4 * (c.lane >> 4);
+    if (bias_kind) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float b = bias_at(bias, bias_kind, min(c.n0 + i * 16 + g4 + k, c.N - 1));
+#pragma unroll
+          for (int j = 0; j < MI; ++j) acc[i][j][k] += b;
+        }
+    }
+    const int wn_per_tile = 2;
+    const int slot = c.nt * wn_per_tile + c.wn;
+#pragma unroll
+    for (int j = 0; j < MI; ++j) {
+      const int m = c.m0 + j * 16 + (c.lane & 15);
+      const int lab = m < c.M ? label[m] : -1;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = c.n0 + i * 16 + g4 + k;
+          if (n < c.N) mx = fmaxf(mx, acc[i][j][k]);
+          if (n == lab) zlab[m] = acc[i][j][k];
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float ref = mx == -INFINITY ? 0.f : mx;  // a row of -inf adds nothing, without inf - inf
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = c.n0 + i * 16 + g4 + k;
+          if (n < c.N) s += __expf(acc[i][j][k] - ref);
+        }
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      if (c.lane < 16 && m < c.M) part[(int64_t)m * npart + slot] = make_float2(mx, s);
+    }
+  }
+};
+
+// Joins the pairs of every row: 16 lanes a row. Writes lse (compact) and the row's loss (all rows).
+__global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ part, int npart,
+                                                  const float* __restrict__ zlab, const int* __restrict__ label,
+                                                  const int* __restrict__ inv, int N, int V, float* __restrict__ lse,
+                                                  float* __restrict__ rows) {
+  const int l = threadIdx.x & 15;
+  const int r = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int c = r < N ? inv[r] : -1;
+  if (c < 0) {
+    if (r < N && l == 0) rows[r] = 0.f;
+    return;
+  }
+  float mx = -INFINITY, s = 0.f;
+  for (int p = l; p < npart; p += 16) {
+    const float2 q = part[(int64_t)c * npart + p];
+    const float m2 = fmaxf(mx, q.x);
+    const float ref = m2 == -INFINITY ? 0.f : m2;
+    s = s * __expf(mx - ref) + q.y * __expf(q.x - ref);
+    mx = m2;
+  }
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) {
+    const float om = __shfl_xor(mx, x), os = __shfl_xor(s, x);
+    const float m2 = fmaxf(mx, om);
+    const float ref = m2 == -INFINITY ? 0.f : m2;
+    s = s * __expf(mx - ref) + os * __expf(om - ref);
+    mx = m2;
+  }
+  if (l == 0) {
+    const int y = label[c];
+    // a label outside the vocabulary has no loss: NaN, and NaN gradients through lse
+    const float v = (y >= 0 && y < V) ? logf(s) + mx : NAN;
+    lse[c] = v;
+    rows[r] = v - (y >= 0 && y < V ? zlab[c] : 0.f);
+  }
+}
+
+// mean / sum over the rows, by one block in a fixed order
+__global__ void __launch_bounds__(1024) lce_reduce(const float* __restrict__ rows, int N, const int* __restrict__ cnt,
+                                                   int mean, float* __restrict__ out) {
+  __shared__ float sh[16];
+  float s = 0.f;
+  for (int r = threadIdx.x; r < N; r += 1024) s += rows[r];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float tot = 0.f;
+    for (int i = 0; i < 16; ++i) tot += sh[i];
+    *out = mean ? tot / (float)*cnt : tot;
+  }
+}
+
+// dz of one piece of the vocabulary, and its sums over the wave's rows (the bias gradient's terms).
+struct EpiDz {
+  const void* bias;
+  int bias_kind;
+  const int* label;
+  const float* lse;
+  const float* rowscale;  // g_r / G per compact row, or null (1)
+  int v0;                 // first vocabulary entry of the piece
+  u16* dz;                // [rows][ld]
+  int64_t ld;
+  float* dbp;             // [m waves][ld] or null
+  int wm_per_tile;
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+    const int g4 = 4 * (c.lane >> 4);
+    f32x4 sum[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < MI; ++j) {
+      const int m = c.m0 + j * 16 + (c.lane & 15);
+      const bool on = m < c.M;
+      const int mm = min(m, c.M - 1);
+      const float ls = lse[mm], rs = rowscale ? rowscale[mm] : 1.f;
+      const int lab = label[mm] - v0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int n = c.n0 + i * 16 + g4;
+        float d[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float z = acc[i][j][k] + bias_at(bias, bias_kind, min(v0 + n + k, v0 + c.N - 1));
+          const float p = __expf(z - ls) - (n + k == lab ? 1.f : 0.f);
+          d[k] = n + k < c.N ? p * rs : 0.f;
+          if (on) sum[i][k] += d[k];
+        }
+        if (on && n < ld)  // columns N..ld are the zeros that the next products read
+          *reinterpret_cast<uint2*>(dz + (int64_t)m * ld + n) =
+              pack4bf(d[0] * DZ_SCALE, d[1] * DZ_SCALE, d[2] * DZ_SCALE, d[3] * DZ_SCALE);
+      }
+    }
+    if (!dbp) return;
+    float* o = dbp + (int64_t)(c.mt * wm_per_tile + c.wm) * ld;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int n = c.n0 + i * 16 + g4;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[i][k] = row_sum16(sum[i][k]);
+      if ((c.lane & 15) == 0 && n < ld) *reinterpret_cast<f32x4*>(o + n) = sum[i];
+    }
+  }
+};
+
+__global__ void __launch_bounds__(256) lce_db(const float* __restrict__ dbp, int64_t ld, const int* __restrict__ cnt,
+                                              int tm, int wm_per_tile, int V, const float* __restrict__ gs,
+                                              void* __restrict__ db, int kind) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  const int n = (*cnt + tm - 1) / tm * wm_per_tile;
+  float s = 0.f;
+  for (int i = 0; i < n; ++i) s += dbp[(int64_t)i * ld + v];
+  s *= *gs;
+  if (kind == 1) static_cast<float*>(db)[v] = s;
+  else static_cast<u16*>(db)[v] = f2bf(s);
+}
+
+// dh of every row: the sum of its slabs, or zeros where the label was ignored.
+__global__ void __launch_bounds__(256) lce_dh(const float* __restrict__ slab, int nslab, int64_t stride, int64_t ld,
+                                              const int* __restrict__ inv, int N, int K, const float* __restrict__ gs,
+                                              u16* __restrict__ dh) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int k4 = (K + 3) / 4;
+  const int64_t r = i / k4;
+  const int k = (int)(i - r * k4) * 4;
+  if (r >= N) return;
+  const int c = inv[r];
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (c >= 0) {
+    for (int q = 0; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(slab + q * stride + (int64_t)c * ld + k);
+    s *= *gs * (1.f / DZ_SCALE);
+  }
+  g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
+}
+
+}  // namespace
+
+#ifndef MIHVD_F16
+int lce_splits(int64_t rows, int64_t hidden, int64_t piece) {
+  return g16::pick_splits((int64_t)g16::cdiv(rows, 128) * g16::cdiv(hidden, 128), g16::cdiv(piece, g16::BK));
+}
+#endif
+
+void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t hs0, int64_t hs1, const u16* w, int64_t ldw,
+                    const void* bias, int bias_kind, u16* hc, float2* part, float* zlab, float* lse, float* rows,
+                    float* loss, int mean, hipStream_t st) {
+  const int npart = lce_npart(s.V);
+  lce_gather<<<g16::cdiv(s.N, 4), 256, 0, st>>>(h, hs0, hs1, rw.idx, rw.cnt, s.K, s.K8, hc);
+  g16::Args a;
+  a.m.p[0] = hc;
+  a.m.ld = s.K8;
+  a.m.ext = s.N;
+  a.n.p[0] = w;
+  a.n.ld = ldw;
+  a.n.ext = s.V;
+  a.M = s.N;
+  a.N = s.V;
+  a.K = s.K;
+  a.dyn_m = rw.cnt;
+  EpiStats e{bias, bias_kind, rw.label, part, npart, zlab};
+  g16::launch<g16::KC, g16::KC, 128, 128, 2, 2>(a, e, st);
+  lce_finish<<<g16::cdiv(s.N, 16), 256, 0, st>>>(part, npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
+  if (loss) lce_reduce<<<1, 1024, 0, st>>>(rows, s.N, rw.cnt, mean, loss);
+}
+
+void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, const u16* hc, const u16* w, int64_t ldw,
+                     const void* bias, int bias_kind, const float* lse, const LceScratch& x, u16* dh, u16* dw, void* db,
+                     hipStream_t st) {
+  for (int v0 = 0, first = 1; v0 < s.V; v0 += x.piece, first = 0) {
+    const int nv = std::min(x.piece, s.V - v0);
+    const u16* wp = w + (int64_t)v0 * ldw;
+    {
+      g16::Args a;
+      a.m.p[0] = hc;
+      a.m.ld = s.K8;
+      a.m.ext = s.N;
+      a.n.p[0] = wp;
+      a.n.ld = ldw;
+      a.n.ext = nv;
+      a.M = s.N;
+      a.N = nv;
+      a.K = s.K;
+      a.dyn_m = rw.cnt;
+      EpiDz e{bias, bias_kind, rw.label, lse, g.rowscale, v0, x.dz, x.ldz, db ? x.dbp : nullptr, 2};
+      g16::launch<g16::KC, g16::KC, 128, 128, 2, 2>(a, e, st);
+    }
+    if (db) {
+      const int esz = bias_kind == 1 ? 4 : 2;
+      lce_db<<<g16::cdiv(nv, 256), 256, 0, st>>>(x.dbp, x.ldz, rw.cnt, 128, 2, nv, g.scale,
+                                                 static_cast<char*>(db) + (int64_t)v0 * esz, bias_kind);
+    }
+    if (dw) {
+      g16::Args a;
+      a.m.p[0] = x.dz;
+      a.m.ld = x.ldz;
+      a.m.ext = (int)g16::up8(nv);
+      a.n.p[0] = hc;
+      a.n.ld = s.K8;
+      a.n.ext = s.K8;
+      a.M = nv;
+      a.N = s.K;
+      a.K = s.N;
+      a.dyn_k = rw.cnt;
+      g16::EpiStore e{{dw + (int64_t)v0 * s.K, nullptr}, s.K, 1.f / DZ_SCALE, g.scale};
+      g16::launch<g16::KS, g16::KS, 128, 128, 2, 2>(a, e, st);
+    }
+    if (dh) {
+      g16::Args a;
+      a.m.p[0] = x.dz;
+      a.m.ld = x.ldz;
+      a.m.ext = s.N;
+      a.n.p[0] = wp;
+      a.n.ld = ldw;
+      a.n.ext = s.K8;
+      a.M = s.N;
+      a.N = s.K;
+      a.K = nv;
+      a.splits = x.splits;
+      a.dyn_m = rw.cnt;
+      g16::EpiSlab e{x.slab, s.K8, (int64_t)s.N * s.K8, x.splits, first ? 0 : 1};
+      g16::launch<g16::KC, g16::KS, 128, 128, 2, 2>(a, e, st);
+    }
+  }
+  if (dh) {
+    const int64_t work = (int64_t)s.N * ((s.K + 3) / 4);
+    lce_dh<<<g16::cdiv(work, 256), 256, 0, st>>>(x.slab, x.splits, (int64_t)s.N * s.K8, s.K8, rw.inv, s.N, s.K, g.scale, dh);
+  }
+}
+
+MIHVD_OPNS_END

@@ -1,0 +1,295 @@
+// Orthogonalising a matrix by Newton-Schulz steps, and the weight update made of it.
+//
+//   X = u / (|u|_F + eps);   per step  A = X X^T,  B = b A + c A A,  X <- a X + B X
+// (for more rows than columns the same on the other side: A = X^T X, X <- a X + X B).
+//
+// X, A and B are bounded (singular values stay below ~1.3), so they are held in fp16 scaled by 2^12:
+// the MFMA rate of bf16 with three more bits. fp32 values are held as two fp16 planes hi + lo (22
+// bits) and multiplied as hi hi + hi lo + lo hi, three k segments of one product; the dropped lo lo
+// is below 2^-22. A and B are symmetric: only tiles on and above the diagonal are computed, and
+// stored twice.
+//
+// Elements below 2^-26 of the norm lose relative precision in the scaled planes (fp16's smallest
+// step is 2^-24); their absolute error is 2^-37, below the fp32 rounding of the sums they enter.
+#define MIHVD_F16 1
+#include "gemm16.h"
+
+#include "transformer.h"
+
+namespace mihvd {
+
+using namespace f16;
+
+namespace {
+
+constexpr float S = 4096.f, INV_S = 1.f / 4096.f;
+
+struct NsTable {
+  const void* src[NS_MAX];
+  float* mom[NS_MAX];
+};
+struct NsOut {
+  void* dst[NS_MAX];
+};
+
+__device__ __forceinline__ float load_src(const void* p, int kind, int64_t i) {
+  if (kind == 0) return static_cast<const float*>(p)[i];
+  const u16 h = static_cast<const u16*>(p)[i];
+  return kind == 1 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+}
+
+// Sum of squares of each matrix, NS_PART partial sums; for Muon the momentum is updated on the way:
+// m = mu m + g, u = g + mu m (nesterov) or m.
+__global__ void __launch_bounds__(256) ns_norm(const NsTable t, int64_t n, int kind, int muon, float mu, int nesterov,
+                                               float* __restrict__ partial) {
+  __shared__ float sh[4];
+  const int b = blockIdx.y;
+  float s = 0.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float v = load_src(t.src[b], kind, i);
+    if (muon) {
+      const float m = fmaf(mu, t.mom[b][i], v);
+      t.mom[b][i] = m;
+      v = nesterov ? fmaf(mu, m, v) : m;
+    }
+    s = fmaf(v, v, s);
+  }
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[b * NS_PART + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// planes of S * v: hi, and lo = the rest
+__device__ __forceinline__ void put_planes(u16* p, int64_t plane, int planes, float v) {
+  const u16 hi = f2bf(v);
+  p[0] = hi;
+  if (planes == 2) p[plane] = f2bf(v - bf2f(hi));
+}
+
+__global__ void __launch_bounds__(256) ns_scale(const NsTable t, int rows, int cols, int c8, int planes, int kind,
+                                                int muon, float mu, int nesterov, float eps,
+                                                const float* __restrict__ partial, u16* __restrict__ x) {
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const float norm = sqrtf(wave_sum(partial[b * NS_PART + lane]));
+  const float inv = S / (norm + eps);
+  const int64_t plane = (int64_t)rows * c8;
+  u16* o = x + (int64_t)b * planes * plane;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / c8;
+    const int c = (int)(i - r * c8);
+    float v = 0.f;
+    if (c < cols) {
+      const int64_t k = r * cols + c;
+      v = load_src(t.src[b], kind, k);
+      if (muon) {
+        const float m = t.mom[b][k];
+        v = nesterov ? fmaf(mu, m, v) : m;
+      }
+      v *= inv;
+    }
+    put_planes(o + i, plane, planes, v);
+  }
+}
+
+// out planes [batch][planes][rows][ld] = alpha * acc + beta * in; symmetric: mirrored as well.
+struct EpiPlanes {
+  u16* out;
+  const u16* in;  // planes of the same layout, or null
+  int64_t ld, plane;
+  int planes, sym;
+  float alpha, beta;
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+    u16* o = out + (int64_t)c.batch * planes * plane;
+    const u16* q = in ? in + (int64_t)c.batch * planes * plane : nullptr;
+#pragma unroll
+    for (int j = 0; j < MI; ++j) {
+      const int m = c.m0 + j * 16 + (c.lane & 15);
+      if (m >= c.M) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
+        if (n >= ld) continue;
+        const int64_t at = (int64_t)m * ld + n;
+        float v[4] = {alpha * acc[i][j][0], alpha * acc[i][j][1], alpha * acc[i][j][2], alpha * acc[i][j][3]};
+        if (q) {
+          for (int p = 0; p < planes; ++p) {
+            const uint2 w = *reinterpret_cast<const uint2*>(q + p * plane + at);
+            v[0] = fmaf(beta, bf2f((u16)w.x), v[0]);
+            v[1] = fmaf(beta, bf2f((u16)(w.x >> 16)), v[1]);
+            v[2] = fmaf(beta, bf2f((u16)w.y), v[2]);
+            v[3] = fmaf(beta, bf2f((u16)(w.y >> 16)), v[3]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = n + k < c.N ? v[k] : 0.f;  // the padding stays zero
+        const uint2 hi = pack4bf(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<uint2*>(o + at) = hi;
+        const float lo[4] = {v[0] - bf2f((u16)hi.x), v[1] - bf2f((u16)(hi.x >> 16)), v[2] - bf2f((u16)hi.y),
+                             v[3] - bf2f((u16)(hi.y >> 16))};
+        uint2 lw = make_uint2(0, 0);
+        if (planes == 2) {
+          lw = pack4bf(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint2*>(o + plane + at) = lw;
+        }
+        if (sym && c.nt != c.mt) {
+          const u16 h4[4] = {(u16)hi.x, (u16)(hi.x >> 16), (u16)hi.y, (u16)(hi.y >> 16)};
+          const u16 l4[4] = {(u16)lw.x, (u16)(lw.x >> 16), (u16)lw.y, (u16)(lw.y >> 16)};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n + k < c.N) {
+              o[(int64_t)(n + k) * ld + m] = h4[k];
+              if (planes == 2) o[plane + (int64_t)(n + k) * ld + m] = l4[k];
+            }
+        }
+      }
+    }
+  }
+};
+
+// the last step: v = alpha * acc + beta * X, unscaled, into the result or the weight
+struct EpiFinal {
+  NsOut out;
+  const u16* in;
+  int64_t ld, plane;
+  int planes, cols, kind, muon;
+  float alpha, beta, decay, step;
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+    const u16* q = in + (int64_t)c.batch * planes * plane;
+    void* o = out.dst[c.batch];
+#pragma unroll
+    for (int j = 0; j < MI; ++j) {
+      const int m = c.m0 + j * 16 + (c.lane & 15);
+      if (m >= c.M) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (n + k >= c.N) continue;
+          float v = alpha * acc[i][j][k];
+          for (int p = 0; p < planes; ++p) v = fmaf(beta, bf2f(q[p * plane + (int64_t)m * ld + n + k]), v);
+          const int64_t at = (int64_t)m * cols + n + k;
+          if (muon) {
+            float* w = static_cast<float*>(o) + at;
+            *w = fmaf(-step, v, *w * decay);
+          } else if (kind == 0) {
+            static_cast<float*>(o)[at] = v;
+          } else if (kind == 1) {
+            static_cast<u16*>(o)[at] = __builtin_bit_cast(u16, (__bf16)v);
+          } else {
+            static_cast<u16*>(o)[at] = f2bf(v);
+          }
+        }
+      }
+    }
+  }
+};
+
+// steps == 0: the normalised matrix itself
+__global__ void __launch_bounds__(256) ns_copy_out(const u16* __restrict__ x, const NsOut out, int rows, int cols, int c8,
+                                                   int planes, int kind, int muon, float decay, float step) {
+  const int b = blockIdx.y;
+  const int64_t plane = (int64_t)rows * c8, n = (int64_t)rows * cols;
+  const u16* q = x + (int64_t)b * planes * plane;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / cols, at = r * c8 + (i - r * cols);
+    float v = bf2f(q[at]);
+    if (planes == 2) v += bf2f(q[plane + at]);
+    v *= INV_S;
+    if (muon) {
+      float* w = static_cast<float*>(out.dst[b]) + i;
+      *w = fmaf(-step, v, *w * decay);
+    } else if (kind == 0) {
+      static_cast<float*>(out.dst[b])[i] = v;
+    } else if (kind == 1) {
+      static_cast<u16*>(out.dst[b])[i] = __builtin_bit_cast(u16, (__bf16)v);
+    } else {
+      static_cast<u16*>(out.dst[b])[i] = f2bf(v);
+    }
+  }
+}
+
+g16::Side plane_side(const u16* x, int64_t ld, int ext, int64_t plane, int planes, bool second) {
+  // segments hi hi, hi lo, lo hi
+  g16::Side s;
+  s.p[0] = x;
+  s.p[1] = second ? x + plane : x;
+  s.p[2] = second ? x : x + plane;
+  s.ld = ld;
+  s.bs = planes * plane;
+  s.ext = ext;
+  return s;
+}
+
+}  // namespace
+
+void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_t st) {
+  using namespace g16;
+  NsTable tab;
+  NsOut out;
+  for (int i = 0; i < NS_MAX; ++i) {
+    tab.src[i] = g.src[i];
+    tab.mom[i] = g.mom[i];
+    out.dst[i] = g.dst[i];
+  }
+  const int64_t n = (int64_t)g.rows * g.cols, px = (int64_t)g.rows * g.c8, pa = (int64_t)g.side * g.s8;
+  const int grid = (int)std::min<int64_t>(512, (px + 255) / 256);
+  ns_norm<<<dim3(NS_PART, g.count), 256, 0, st>>>(tab, n, p.src_kind, p.muon, p.momentum, p.nesterov, sc.partial);
+  ns_scale<<<dim3(grid, g.count), 256, 0, st>>>(tab, g.rows, g.cols, g.c8, g.planes, p.src_kind, p.muon, p.momentum,
+                                               p.nesterov, p.eps, sc.partial, sc.x0);
+  const float step = p.lr * p.scale;
+  if (p.steps == 0) {
+    ns_copy_out<<<dim3(grid, g.count), 256, 0, st>>>(sc.x0, out, g.rows, g.cols, g.c8, g.planes, p.src_kind, p.muon,
+                                                     p.decay, step);
+    return;
+  }
+  const bool tall = g.rows > g.cols;
+  const int nseg = g.planes == 2 ? 3 : 1;
+  u16 *x = sc.x0, *y = sc.x1;
+  for (int it = 0; it < p.steps; ++it) {
+    Args a;
+    a.batch = g.count;
+    a.nseg = nseg;
+    a.sym = 1;
+    a.M = a.N = g.side;
+    EpiPlanes gram{sc.gram, nullptr, g.s8, pa, g.planes, 1, INV_S, 0.f};
+    if (tall) {
+      a.K = g.rows;
+      a.m = plane_side(x, g.c8, g.c8, px, g.planes, false);
+      a.n = plane_side(x, g.c8, g.c8, px, g.planes, true);
+      launch<KS, KS, 128, 128, 2, 2>(a, gram, st);
+    } else {
+      a.K = g.cols;
+      a.m = plane_side(x, g.c8, g.rows, px, g.planes, false);
+      a.n = plane_side(x, g.c8, g.rows, px, g.planes, true);
+      launch<KC, KC, 128, 128, 2, 2>(a, gram, st);
+    }
+    a.K = g.side;
+    a.m = plane_side(sc.gram, g.s8, g.side, pa, g.planes, false);
+    a.n = plane_side(sc.gram, g.s8, g.side, pa, g.planes, true);
+    launch<KC, KC, 128, 128, 2, 2>(a, EpiPlanes{sc.poly, sc.gram, g.s8, pa, g.planes, 1, p.c * INV_S, p.b}, st);
+    a.sym = 0;
+    a.M = g.rows;
+    a.N = g.cols;
+    const bool last = it + 1 == p.steps;
+    EpiPlanes upd{y, x, g.c8, px, g.planes, 0, INV_S, p.a};
+    EpiFinal fin{out, x, g.c8, px, g.planes, g.cols, p.src_kind, p.muon, INV_S * INV_S, p.a * INV_S, p.decay, step};
+    if (tall) {  // X B: rows of X against rows of the symmetric B
+      a.m = plane_side(x, g.c8, g.rows, px, g.planes, false);
+      a.n = plane_side(sc.poly, g.s8, g.side, pa, g.planes, true);
+      if (last) launch<KC, KC, 128, 128, 2, 2>(a, fin, st);
+      else launch<KC, KC, 128, 128, 2, 2>(a, upd, st);
+    } else {
+      a.m = plane_side(sc.poly, g.s8, g.side, pa, g.planes, false);
+      a.n = plane_side(x, g.c8, g.c8, px, g.planes, true);
+      if (last) launch<KC, KS, 128, 128, 2, 2>(a, fin, st);
+      else launch<KC, KS, 128, 128, 2, 2>(a, upd, st);
+    }
+    std::swap(x, y);
+  }
+}
+
+}  // namespace mihvd

@@ -1,0 +1,451 @@
+// torch.ops.mihvd registration of the transformer-step operators: argument checks, packing of
+// operands the matrix core cannot read in place, workspaces, and the choice of the operand format.
+#include <ATen/ATen.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/library.h>
+
+#include <map>
+#include <tuple>
+
+#include "common.h"
+#include "transformer.h"
+
+namespace mihvd {
+namespace {
+
+constexpr int64_t MAX_ROWS = int64_t(1) << 30, MAX_LD = int64_t(1) << 22;
+constexpr int64_t DZ_BYTES = int64_t(512) << 20;  // bound on the gradient piece that backward holds
+
+inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline hipStream_t cur_stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+const u16* p16(const at::Tensor& t) { return static_cast<const u16*>(t.data_ptr()); }
+u16* m16(at::Tensor& t) { return t.defined() ? static_cast<u16*>(t.data_ptr()) : nullptr; }
+
+// [R][C] with any strides -> [R][C8], the padding zero
+__global__ void __launch_bounds__(256) pack_kernel(const u16* __restrict__ src, int64_t s0, int64_t s1, int64_t R, int C,
+                                                   int C8, u16* __restrict__ dst) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < R * C8; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / C8;
+    const int c = (int)(i - r * C8);
+    dst[i] = c < C ? src[r * s0 + c * s1] : (u16)0;
+  }
+}
+
+// A matrix the core reads: rows of unit stride, 16-byte aligned, columns a multiple of 8; anything
+// else is copied into that form once.
+struct Mat {
+  at::Tensor hold;
+  const u16* p;
+  int64_t ld;
+};
+bool direct(const at::Tensor& t) {
+  return t.stride(1) == 1 && t.size(1) % 8 == 0 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) &&
+         t.stride(0) <= MAX_LD && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+Mat mat(const at::Tensor& t, bool force = false) {
+  if (!force && direct(t)) return {t, p16(t), t.stride(0)};
+  const int64_t R = t.size(0), C = t.size(1), C8 = up8(C);
+  at::Tensor d = at::empty({R, C8}, t.options());
+  const int64_t blocks = std::min<int64_t>(cdiv(R * C8, 256), 8192);
+  if (blocks > 0)
+    pack_kernel<<<dim3((unsigned)blocks), 256, 0, cur_stream()>>>(p16(t), t.stride(0), t.stride(1), R, (int)C, (int)C8,
+                                                                  m16(d));
+  return {d, p16(d), C8};
+}
+
+void check16(const at::Tensor& t, const char* op, const char* name, const at::Tensor& like, int64_t dim) {
+  TORCH_CHECK_VALUE(t.dim() == dim, op, ": ", name, " must have ", dim, " dimensions (got ", t.dim(), ")");
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": ", name,
+                   " must be bfloat16 or float16 (got ", t.scalar_type(), ")");
+  TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), op, ": ", name, " must have the type of the first argument");
+  TORCH_CHECK_VALUE(t.device() == like.device() && t.is_cuda(), op, ": ", name, " must be on the same GPU");
+}
+
+// ------------------------------------------------------------------------------------------ //
+// linear_cross_entropy
+
+// One block: the labelled rows in order, their labels in 32 bits (-1: outside the vocabulary), and
+// for every row its place among them.
+__global__ void __launch_bounds__(1024) lce_compact(const int64_t* __restrict__ labels, int N, int V, int64_t ignore,
+                                                    int* __restrict__ idx, int* __restrict__ inv,
+                                                    int* __restrict__ label, int* __restrict__ cnt) {
+  __shared__ int wsum[16];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  int base = 0;
+  for (int r0 = 0; r0 < N; r0 += 1024) {
+    const int r = r0 + t;
+    const int64_t y = r < N ? labels[r] : ignore;
+    const bool on = y != ignore;
+    const unsigned long long b = __ballot(on);
+    const int before = __popcll(b & ((1ull << lane) - 1));
+    if (lane == 0) wsum[w] = __popcll(b);
+    __syncthreads();
+    int off = base, tot = 0;
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) off += wsum[i];
+      tot += wsum[i];
+    }
+    if (r < N) inv[r] = on ? off + before : -1;
+    if (on) {
+      idx[off + before] = r;
+      label[off + before] = y >= 0 && y < V ? (int)y : -1;
+    }
+    base += tot;
+    __syncthreads();
+  }
+  if (t == 0) *cnt = base;
+}
+
+// G (over count for the mean) and the rows' shares of it. reduction: 0 none, 1 mean, 2 sum.
+__global__ void __launch_bounds__(1024) lce_scale(const float* __restrict__ gout, int64_t gstride, int reduction,
+                                                  const int* __restrict__ idx, const int* __restrict__ cnt,
+                                                  float* __restrict__ scale, float* __restrict__ rowscale) {
+  const int n = *cnt;
+  if (reduction != 0) {
+    if (threadIdx.x == 0) *scale = reduction == 2 ? *gout : n > 0 ? *gout / (float)n : 0.f;
+    return;
+  }
+  __shared__ float sh[16];
+  float m = 0.f;  // over the finite ones: an infinite share stays infinite in its own row
+  for (int c = threadIdx.x; c < n; c += 1024) {
+    const float g = fabsf(gout[idx[c] * gstride]);
+    if (g < INFINITY) m = fmaxf(m, g);
+  }
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = sh[0];
+  for (int i = 1; i < 16; ++i) m = fmaxf(m, sh[i]);
+  const float G = m > 0.f ? m : 1.f;
+  for (int c = threadIdx.x; c < n; c += 1024) rowscale[c] = gout[idx[c] * gstride] / G;
+  if (threadIdx.x == 0) *scale = G;
+}
+
+LceRows rows_of(const at::Tensor& meta, int64_t N) {
+  const int* p = meta.data_ptr<int>();
+  return {p, p + N, p + 2 * N, p + 3 * N};
+}
+int bias_kind(const c10::optional<at::Tensor>& b) { return !b ? 0 : b->scalar_type() == at::kFloat ? 1 : 2; }
+
+void lce_check(const at::Tensor& h, const at::Tensor& w, const c10::optional<at::Tensor>& bias) {
+  const char* op = "linear_cross_entropy";
+  check16(h, op, "hidden", h, 2);
+  check16(w, op, "weight", h, 2);
+  const int64_t N = h.size(0), K = h.size(1), V = w.size(0);
+  TORCH_CHECK_VALUE(w.size(1) == K, op, ": weight has ", w.size(1), " columns, hidden has ", K);
+  TORCH_CHECK_VALUE(K >= 1 && V >= 1 && N <= MAX_ROWS && V <= MAX_ROWS && K <= MAX_LD, op, ": sizes out of range (",
+                    N, " rows, ", K, " hidden, ", V, " vocabulary)");
+  if (bias) {
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == V && bias->device() == h.device(), op,
+                      ": bias must be a vector of ", V, " on the same GPU");
+    TORCH_CHECK_TYPE(bias->scalar_type() == at::kFloat || bias->scalar_type() == h.scalar_type(), op,
+                     ": bias must be float32 or of hidden's type");
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at::Tensor& h, const at::Tensor& w,
+                                                                       const at::Tensor& labels,
+                                                                       const c10::optional<at::Tensor>& bias_in,
+                                                                       int64_t ignore_index, int64_t reduction) {
+  lce_check(h, w, bias_in);
+  const int64_t N = h.size(0), K = h.size(1), V = w.size(0), K8 = up8(K);
+  TORCH_CHECK_TYPE(labels.scalar_type() == at::kLong, "linear_cross_entropy: labels must be int64");
+  TORCH_CHECK_VALUE(labels.dim() == 1 && labels.size(0) == N && labels.device() == h.device(),
+                    "linear_cross_entropy: labels must be a vector of ", N, " on the same GPU");
+  TORCH_CHECK_VALUE(reduction >= 0 && reduction <= 2, "linear_cross_entropy: reduction");
+  c10::DeviceGuard guard(h.device());
+  hipStream_t st = cur_stream();
+  const auto f32 = h.options().dtype(at::kFloat);
+  c10::optional<at::Tensor> bias;
+  if (bias_in) bias = bias_in->contiguous();
+  at::Tensor rows = at::empty({N}, f32), loss = reduction ? at::empty({}, f32) : rows;
+  at::Tensor hc = at::empty({N, K8}, h.options()), lse = at::empty({N}, f32);
+  at::Tensor meta = at::empty({3 * N + 1}, h.options().dtype(at::kInt));
+  if (N == 0) {
+    if (reduction) loss.fill_(reduction == 1 ? NAN : 0.f);
+    meta.zero_();
+    return {loss, hc, meta, lse};
+  }
+  at::Tensor lab = labels.contiguous();
+  int* m = meta.data_ptr<int>();
+  lce_compact<<<1, 1024, 0, st>>>(lab.data_ptr<int64_t>(), (int)N, (int)V, ignore_index, m, m + N, m + 2 * N, m + 3 * N);
+  const Mat wm = mat(w);
+  at::Tensor part = at::empty({N, lce_npart((int)V), 2}, f32), zlab = at::empty({N}, f32);
+  const LceShape s{(int)N, (int)K, (int)K8, (int)V};
+  auto run = h.scalar_type() == at::kHalf ? &f16::lce_forward_16 : &lce_forward_16;
+  run(s, rows_of(meta, N), p16(h), h.stride(0), h.stride(1), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr,
+      bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part.data_ptr<float>()), zlab.data_ptr<float>(),
+      lse.data_ptr<float>(), rows.data_ptr<float>(), reduction ? loss.data_ptr<float>() : nullptr, reduction == 1, st);
+  return {loss, hc, meta, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& gout, const at::Tensor& hc,
+                                                            const at::Tensor& w, const c10::optional<at::Tensor>& bias_in,
+                                                            const at::Tensor& meta, const at::Tensor& lse,
+                                                            int64_t reduction, bool need_h, bool need_w, bool need_b) {
+  const int64_t N = lse.size(0), V = w.size(0), K = w.size(1), K8 = up8(K);
+  TORCH_CHECK_VALUE(hc.dim() == 2 && hc.size(0) == N && hc.size(1) == K8 && hc.is_contiguous() &&
+                        meta.numel() == 3 * N + 1 && hc.scalar_type() == w.scalar_type(),
+                    "lce_backward: not the tensors that lce_forward returned");
+  check16(w, "lce_backward", "weight", hc, 2);
+  TORCH_CHECK_VALUE(gout.scalar_type() == at::kFloat && gout.device() == w.device() &&
+                        (reduction ? gout.numel() == 1 : (gout.dim() == 1 && gout.size(0) == N)),
+                    "lce_backward: the loss gradient does not fit the loss");
+  c10::DeviceGuard guard(w.device());
+  hipStream_t st = cur_stream();
+  const auto f32 = w.options().dtype(at::kFloat);
+  c10::optional<at::Tensor> bias;
+  if (bias_in) bias = bias_in->contiguous();
+  need_b = need_b && bias.has_value();
+  at::Tensor dh, dw, db;
+  if (need_h) dh = at::empty({N, K}, w.options());
+  if (need_w) dw = at::empty({V, K}, w.options());
+  if (need_b) db = at::empty({V}, bias->options());
+  if (N == 0) {
+    if (need_w) dw.zero_();
+    if (need_b) db.zero_();
+    return {dh, dw, db};
+  }
+  const LceRows rw = rows_of(meta, N);
+  at::Tensor scale = at::empty({1}, f32), rowscale;
+  if (reduction == 0) rowscale = at::empty({N}, f32);
+  lce_scale<<<1, 1024, 0, st>>>(gout.data_ptr<float>(), reduction ? 0 : gout.stride(0), (int)reduction, rw.idx, rw.cnt,
+                                scale.data_ptr<float>(), reduction ? nullptr : rowscale.data_ptr<float>());
+  const Mat wm = mat(w);
+  LceScratch x{};
+  x.piece = (int)std::min<int64_t>(up8(V), std::max<int64_t>(256, DZ_BYTES / (2 * N) / 256 * 256));
+  x.ldz = up8(x.piece);
+  at::Tensor dz = at::empty({N, x.ldz}, w.options()), dbp, slab;
+  x.dz = m16(dz);
+  if (need_b) {
+    dbp = at::empty({2 * cdiv(N, 128), x.ldz}, f32);
+    x.dbp = dbp.data_ptr<float>();
+  }
+  if (need_h) {
+    x.splits = lce_splits(N, K, x.piece);
+    slab = at::empty({x.splits, N, K8}, f32);
+    x.slab = slab.data_ptr<float>();
+  }
+  const LceShape s{(int)N, (int)K, (int)K8, (int)V};
+  const LceGrad g{scale.data_ptr<float>(), reduction ? nullptr : rowscale.data_ptr<float>()};
+  auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
+  run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias), lse.data_ptr<float>(), x, m16(dh),
+      m16(dw), need_b ? db.data_ptr() : nullptr, st);
+  return {dh, dw, db};
+}
+
+// ------------------------------------------------------------------------------------------ //
+// gated_ffn
+
+struct FfnMats {
+  Mat gate, up, down;
+  FfnWeights w;
+};
+FfnMats ffn_weights(const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd) {
+  // one leading dimension serves both input projections
+  const bool same = direct(wg) && direct(wu) && wg.stride(0) == wu.stride(0);
+  FfnMats m{mat(wg, !same), mat(wu, !same), mat(wd), {}};
+  m.w = {m.gate.p, m.up.p, m.down.p, m.gate.ld, m.down.ld};
+  return m;
+}
+void ffn_check(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t act) {
+  const char* op = "gated_ffn";
+  check16(x, op, "x", x, 2);
+  check16(wg, op, "w_gate", x, 2);
+  check16(wu, op, "w_up", x, 2);
+  check16(wd, op, "w_down", x, 2);
+  const int64_t N = x.size(0), K = x.size(1), F = wg.size(0);
+  TORCH_CHECK_VALUE(wg.size(1) == K && wu.size(0) == F && wu.size(1) == K && wd.size(0) == K && wd.size(1) == F, op,
+                    ": w_gate and w_up must be [inner, ", K, "] and w_down [", K, ", inner]");
+  TORCH_CHECK_VALUE(N <= MAX_ROWS && K >= 1 && F >= 1 && K <= MAX_LD && F <= MAX_LD / 2, op, ": sizes out of range (", N,
+                    " rows, ", K, " hidden, ", F, " inner)");
+  TORCH_CHECK_VALUE(act >= 0 && act < ACT_COUNT, op, ": unknown activation");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_forward(const at::Tensor& x, const at::Tensor& wg,
+                                                                       const at::Tensor& wu, const at::Tensor& wd,
+                                                                       int64_t act, bool save) {
+  ffn_check(x, wg, wu, wd, act);
+  c10::DeviceGuard guard(x.device());
+  const int64_t N = x.size(0), K = x.size(1), F = wg.size(0), F8 = up8(F);
+  at::Tensor y = at::empty({N, K}, x.options()), h = at::empty({N, F8}, x.options());
+  at::Tensor g, u;
+  if (save) {
+    g = at::empty({N, F8}, x.options());
+    u = at::empty({N, F8}, x.options());
+  }
+  if (N > 0) {
+    const Mat xm = mat(x);
+    const FfnMats wm = ffn_weights(wg, wu, wd);
+    const FfnShape s{(int)N, (int)K, (int)up8(K), (int)F, (int)F8};
+    auto run = x.scalar_type() == at::kHalf ? &f16::ffn_forward_16 : &ffn_forward_16;
+    run(s, xm.p, xm.ld, wm.w, (int)act, m16(g), m16(u), m16(h), m16(y), x.device(), cur_stream());
+  }
+  if (!save) h = at::Tensor();
+  return {y, g, u, h};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
+    const at::Tensor& dy, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
+    const at::Tensor& g, const at::Tensor& u, const at::Tensor& h, int64_t act, bool need_x, bool need_g, bool need_u,
+    bool need_d) {
+  ffn_check(x, wg, wu, wd, act);
+  const int64_t N = x.size(0), K = x.size(1), F = wg.size(0), F8 = up8(F);
+  check16(dy, "gated_ffn", "the output gradient", x, 2);
+  TORCH_CHECK_VALUE(dy.size(0) == N && dy.size(1) == K, "gated_ffn: the output gradient's shape");
+  for (const at::Tensor* t : {&g, &u, &h})
+    TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == N && t->size(1) == F8 && t->is_contiguous() &&
+                          t->scalar_type() == x.scalar_type() && t->device() == x.device(),
+                      "gated_ffn: not the tensors that the forward pass kept");
+  c10::DeviceGuard guard(x.device());
+  at::Tensor dx, dwg, dwu, dwd;
+  if (need_x) dx = at::empty({N, K}, x.options());
+  if (need_g) dwg = at::empty({F, K}, x.options());
+  if (need_u) dwu = at::empty({F, K}, x.options());
+  if (need_d) dwd = at::empty({K, F}, x.options());
+  if (N == 0) {
+    for (at::Tensor* t : {&dwg, &dwu, &dwd})
+      if (t->defined()) t->zero_();
+    return {dx, dwg, dwu, dwd};
+  }
+  at::Tensor dgu;
+  if (need_x || need_g || need_u) dgu = at::empty({N, 2 * F8}, x.options());
+  const Mat xm = mat(x), dym = mat(dy);
+  const FfnMats wm = ffn_weights(wg, wu, wd);
+  const FfnShape s{(int)N, (int)K, (int)up8(K), (int)F, (int)F8};
+  auto run = x.scalar_type() == at::kHalf ? &f16::ffn_backward_16 : &ffn_backward_16;
+  run(s, dym.p, dym.ld, xm.p, xm.ld, wm.w, (int)act, p16(g), p16(u), p16(h), m16(dgu), m16(dx), m16(dwg), m16(dwu),
+      m16(dwd), x.device(), cur_stream());
+  return {dx, dwg, dwu, dwd};
+}
+
+// ------------------------------------------------------------------------------------------ //
+// Newton-Schulz
+
+constexpr int64_t NS_ELEMS = int64_t(1) << 28;  // elements of X per launch group (bounds the workspace)
+
+void ns_group(NsGroup& g, NsParams& p, const at::TensorOptions& opt) {
+  const int64_t px = (int64_t)g.rows * g.c8, pa = (int64_t)g.side * g.s8, k = (int64_t)g.count * g.planes;
+  const auto h = opt.dtype(at::kHalf);
+  at::Tensor x0 = at::empty({k * px}, h), x1, gram, poly;
+  if (p.steps > 0) {
+    gram = at::empty({k * pa}, h);
+    poly = at::empty({k * pa}, h);
+  }
+  if (p.steps > 1) x1 = at::empty({k * px}, h);
+  at::Tensor part = at::empty({g.count * NS_PART}, opt.dtype(at::kFloat));
+  ns_run(g, p, NsScratch{m16(x0), m16(x1), m16(gram), m16(poly), part.data_ptr<float>()}, cur_stream());
+}
+
+void ns_shape(NsGroup& g, int64_t rows, int64_t cols, bool split) {
+  TORCH_CHECK_VALUE(rows <= MAX_LD && cols <= MAX_LD, "orthogonalize: sides above ", MAX_LD, " are not supported");
+  g.rows = (int)rows;
+  g.cols = (int)cols;
+  g.c8 = (int)up8(cols);
+  g.side = (int)std::min(rows, cols);
+  g.s8 = (int)up8(g.side);
+  g.planes = split ? 2 : 1;
+}
+
+at::Tensor newton_schulz(const at::Tensor& x_in, int64_t steps, double a, double b, double c, double eps, bool split) {
+  TORCH_CHECK_VALUE(x_in.dim() == 3 && x_in.is_cuda(), "newton_schulz: a [batch, rows, cols] GPU tensor is expected");
+  const auto ty = x_in.scalar_type();
+  TORCH_CHECK_TYPE(ty == at::kFloat || ty == at::kBFloat16 || ty == at::kHalf,
+                   "newton_schulz: float32, bfloat16 or float16 expected (got ", ty, ")");
+  TORCH_CHECK_VALUE(steps >= 0 && steps <= 100, "newton_schulz: steps must be within 0..100");
+  c10::DeviceGuard guard(x_in.device());
+  at::Tensor x = x_in.contiguous(), out = at::empty_like(x);
+  if (x.numel() == 0) return out;
+  NsParams p{};
+  p.steps = (int)steps;
+  p.a = (float)a, p.b = (float)b, p.c = (float)c, p.eps = (float)eps;
+  p.src_kind = ty == at::kFloat ? 0 : ty == at::kBFloat16 ? 1 : 2;
+  const int64_t B = x.size(0), n = x.size(1) * x.size(2), bytes = n * x.element_size();
+  const int64_t per = std::max<int64_t>(1, std::min<int64_t>(NS_MAX, NS_ELEMS / n));
+  for (int64_t i0 = 0; i0 < B; i0 += per) {
+    NsGroup g{};
+    g.count = (int)std::min(per, B - i0);
+    ns_shape(g, x.size(1), x.size(2), split);
+    for (int i = 0; i < g.count; ++i) {
+      g.src[i] = static_cast<const char*>(x.data_ptr()) + (i0 + i) * bytes;
+      g.dst[i] = static_cast<char*>(out.data_ptr()) + (i0 + i) * bytes;
+    }
+    ns_group(g, p, x.options());
+  }
+  return out;
+}
+
+// scale_mode: 0 sqrt(max(1, rows / cols)), 1 0.2 sqrt(max(rows, cols))
+void muon_step(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vector<at::Tensor> ms, double lr,
+               double momentum, bool nesterov, double weight_decay, int64_t steps, double a, double b, double c, double eps,
+               int64_t scale_mode, bool split) {
+  TORCH_CHECK_VALUE(ps.size() == gs.size() && ps.size() == ms.size(), "muon_step: list lengths");
+  TORCH_CHECK_VALUE(steps >= 0 && steps <= 100, "muon_step: steps must be within 0..100");
+  // matrices of one shape run together
+  std::map<std::tuple<int, int64_t, int64_t>, std::vector<size_t>> groups;
+  for (size_t i = 0; i < ps.size(); ++i) {
+    TORCH_CHECK_VALUE(ps[i].dim() >= 2, "muon_step: parameters must be matrices");
+    for (const at::Tensor* t : {&ps[i], &gs[i], &ms[i]})
+      TORCH_CHECK_VALUE(t->is_cuda() && t->scalar_type() == at::kFloat && t->is_contiguous() &&
+                            t->sizes() == ps[i].sizes() && t->device() == ps[i].device(),
+                        "muon_step: contiguous fp32 GPU tensors of equal shapes expected");
+    if (ps[i].numel() == 0) continue;
+    const int64_t rows = ps[i].size(0);
+    groups[{(int)ps[i].get_device(), rows, ps[i].numel() / rows}].push_back(i);
+  }
+  for (const auto& kv : groups) {
+    const int64_t rows = std::get<1>(kv.first), cols = std::get<2>(kv.first);
+    const auto& list = kv.second;
+    c10::DeviceGuard guard(ps[list[0]].device());
+    NsParams p{};
+    p.steps = (int)steps;
+    p.a = (float)a, p.b = (float)b, p.c = (float)c, p.eps = (float)eps;
+    p.muon = 1;
+    p.lr = (float)lr, p.momentum = (float)momentum, p.decay = (float)(1.0 - lr * weight_decay);
+    p.scale = scale_mode == 0 ? (float)std::sqrt(std::max(1.0, (double)rows / (double)cols))
+                              : (float)(0.2 * std::sqrt((double)std::max(rows, cols)));
+    p.nesterov = nesterov;
+    const size_t per = (size_t)std::max<int64_t>(1, std::min<int64_t>(NS_MAX, NS_ELEMS / (rows * cols)));
+    for (size_t i0 = 0; i0 < list.size(); i0 += per) {
+      NsGroup g{};
+      g.count = (int)std::min(per, list.size() - i0);
+      ns_shape(g, rows, cols, split);
+      for (int i = 0; i < g.count; ++i) {
+        const size_t k = list[i0 + i];
+        g.src[i] = gs[k].data_ptr<float>();
+        g.dst[i] = ps[k].data_ptr<float>();
+        g.mom[i] = ms[k].data_ptr<float>();
+      }
+      ns_group(g, p, ps[list[0]].options());
+    }
+  }
+}
+
+}  // namespace
+}  // namespace mihvd
+
+TORCH_LIBRARY_FRAGMENT(mihvd, m) {
+  m.def("lce_forward(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, int ignore_index, int reduction) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("lce_backward(Tensor gout, Tensor hc, Tensor weight, Tensor? bias, Tensor meta, Tensor lse, int reduction, "
+        "bool need_h, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)");
+  m.def("ffn_forward(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act, bool save) -> (Tensor, Tensor, Tensor, "
+        "Tensor)");
+  m.def("ffn_backward(Tensor dy, Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, Tensor g, Tensor u, Tensor h, "
+        "int act, bool need_x, bool need_g, bool need_u, bool need_d) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("newton_schulz(Tensor x, int steps, float a, float b, float c, float eps, bool split) -> Tensor");
+  m.def("muon_step(Tensor(a!)[] p, Tensor[] g, Tensor(b!)[] m, float lr, float momentum, bool nesterov, "
+        "float weight_decay, int steps, float a, float b, float c, float eps, int scale_mode, bool split) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(mihvd, CUDA, m) {
+  m.impl("lce_forward", &mihvd::lce_forward);
+  m.impl("lce_backward", &mihvd::lce_backward);
+  m.impl("ffn_forward", &mihvd::ffn_forward);
+  m.impl("ffn_backward", &mihvd::ffn_backward);
+  m.impl("newton_schulz", &mihvd::newton_schulz);
+  m.impl("muon_step", &mihvd::muon_step);
+}

@@ -91,7 +91,7 @@ def _hipcc() -> str:
 
 
 # MFMA kernel sources compiled a second time with fp16 operands (-DMIHVD_F16).
-F16_SOURCES = ("conv_fwd.hip", "conv_bwd.hip", "fc.hip")
+F16_SOURCES = ("conv_fwd.hip", "conv_bwd.hip", "fc.hip", "linear_ce.hip", "gated_ffn.hip")
 
 
 def build_kernels(force: bool = False, verbose: bool = False, jobs: int | None = None) -> str:

@@ -1,0 +1,130 @@
+"""Autograd-facing wrappers of the transformer-step kernels (``torch.ops.mihvd.lce_* / ffn_*``).
+
+* ``linear_cross_entropy(hidden, weight, labels, bias)`` — the vocabulary projection and its softmax
+  cross entropy without materialised logits (csrc/kernels/linear_ce.hip).
+* ``gated_ffn(x, w_gate, w_up, w_down)`` — ``(act(x Wg^T) * (x Wu^T)) Wd^T`` with its backward pass
+  (csrc/kernels/gated_ffn.hip).
+
+Both run on bf16 or fp16 MFMA operands with fp32 accumulation. Under ``torch.autocast`` floating
+inputs are cast to the autocast type first, as ``torch.nn.functional.linear`` does; otherwise the
+inputs must be 16-bit themselves. There is no CPU or fp32 form: other inputs raise.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _native
+
+ACTIVATIONS = ("silu", "gelu", "gelu_tanh", "relu", "sigmoid")
+_REDUCTIONS = ("none", "mean", "sum")
+
+
+def _prepare(op, *tensors):
+    """Check the device and apply autocast's cast to the floating matrices of a call."""
+    first = tensors[0]
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise ValueError("%s: every tensor must be on the GPU (got one on %s)" % (op, t.device))
+    _native.require_kernels()
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        return [t if t is None or t.dtype == dt or not t.is_floating_point() else t.to(dt) for t in tensors]
+    if first.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("%s: bfloat16 or float16 inputs are needed outside autocast (got %s)" % (op, first.dtype))
+    return list(tensors)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, labels, ignore_index, reduction):
+        loss, hc, meta, lse = torch.ops.mihvd.lce_forward(hidden, weight, labels, bias, ignore_index, reduction)
+        ctx.save_for_backward(hc, weight, bias, meta, lse)
+        ctx.reduction = reduction
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        hc, weight, bias, meta, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dh, dw, db = torch.ops.mihvd.lce_backward(gout, hc, weight, bias, meta, lse, ctx.reduction, need[0], need[1],
+                                                  need[2])
+        return dh, dw, db, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                         bias: torch.Tensor | None = None, *, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(hidden @ weight.T + bias, labels, ...)`` without keeping the logits.
+
+    ``hidden`` [..., K] and ``weight`` [V, K] in bf16 or fp16 (any strides), ``bias`` [V] in fp32 or
+    the same type, ``labels`` [...] int64. The loss is fp32: a scalar for ``reduction="mean"`` (over
+    the labelled rows; NaN if there is none) and ``"sum"``, of ``labels``' shape for ``"none"`` (0 where
+    the label is ``ignore_index``). Gradients come in the types of their inputs; rows that are ignored
+    get exact zeros. A label outside [0, V) that is not ``ignore_index`` makes its row's loss NaN, and
+    with it the gradients.
+
+    Ignored rows are dropped before the products, so a head over all positions of a masked-LM batch
+    costs what its labelled positions cost. The call never synchronises with the host and can be
+    captured in a HIP graph; results repeat bit for bit.
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError("linear_cross_entropy: reduction must be one of %s (got %r)" % (_REDUCTIONS, reduction))
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError("linear_cross_entropy: hidden [..., K] and weight [V, K] are needed (got %s and %s)"
+                         % (tuple(hidden.shape), tuple(weight.shape)))
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError("linear_cross_entropy: labels must have the shape %s (got %s)"
+                         % (tuple(hidden.shape[:-1]), tuple(labels.shape)))
+    if labels.dtype != torch.int64:
+        raise TypeError("linear_cross_entropy: labels must be int64 (got %s)" % labels.dtype)
+    if bias is not None and bias.dtype == torch.float32:
+        h, w, y = _prepare("linear_cross_entropy", hidden, weight, labels)
+        b = bias
+        if not b.is_cuda:
+            raise ValueError("linear_cross_entropy: every tensor must be on the GPU (got one on %s)" % b.device)
+    else:
+        h, w, y, b = _prepare("linear_cross_entropy", hidden, weight, labels, bias)
+    loss = _LinearCrossEntropy.apply(h.reshape(-1, h.shape[-1]), w, b, y.reshape(-1), int(ignore_index),
+                                     _REDUCTIONS.index(reduction))
+    return loss.view(labels.shape) if reduction == "none" else loss
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, act):
+        save = any(ctx.needs_input_grad)
+        y, g, u, h = torch.ops.mihvd.ffn_forward(x, w_gate, w_up, w_down, act, save)
+        if save:
+            ctx.save_for_backward(x, w_gate, w_up, w_down, g, u, h)
+            ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, w_down, g, u, h = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*torch.ops.mihvd.ffn_backward(dy, x, w_gate, w_up, w_down, g, u, h, ctx.act, need[0], need[1], need[2],
+                                              need[3]), None)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
+              activation: str = "silu") -> torch.Tensor:
+    """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T``: ``x`` [..., K], ``w_gate`` and ``w_up`` [F, K],
+    ``w_down`` [K, F], all bf16 or all fp16, any strides; the result has ``x``'s shape and type.
+
+    ``activation``: "silu" (SwiGLU), "gelu" (GeGLU, the erf form), "gelu_tanh", "relu" or "sigmoid". For
+    the backward pass the two projections and their product are kept in 16 bits ([rows, F] each);
+    without gradients only the product is written. From one row up; results repeat bit for bit and
+    the call can be captured in a HIP graph.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError("gated_ffn: activation must be one of %s (got %r)" % (ACTIVATIONS, activation))
+    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[1] != x.shape[-1] or w_up.shape != w_gate.shape or \
+            w_down.shape != (w_gate.shape[1], w_gate.shape[0]):
+        raise ValueError("gated_ffn: x [..., K], w_gate and w_up [F, K] and w_down [K, F] are needed (got %s, %s, %s, %s)"
+                         % tuple(tuple(t.shape) for t in (x, w_gate, w_up, w_down)))
+    x, w_gate, w_up, w_down = _prepare("gated_ffn", x, w_gate, w_up, w_down)
+    y = _GatedFFN.apply(x.reshape(-1, x.shape[-1]), w_gate, w_up, w_down, ACTIVATIONS.index(activation))
+    return y.view(x.shape)

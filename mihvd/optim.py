@@ -253,3 +253,134 @@ class FusedSGD(torch.optim.Optimizer):
                     d = d.add(b, alpha=mom) if group["nesterov"] else b
                 p.add_(d, alpha=-group["lr"])
         return loss
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
+                  precision: str | None = None) -> torch.Tensor:
+    """The matrix (or each matrix of a batch, [..., rows, cols]) with its singular values driven towards
+    one by ``steps`` Newton-Schulz steps:
+
+        X = x / (|x|_F + eps);   A = X X^T;   X <- a X + (b A + c A A) X        (a, b, c = coefficients)
+
+    (on the smaller side; the default coefficients leave the singular values near 1 within about 0.3).
+    The result has ``x``'s type and shape. ``precision``: ``"fp16"`` — one fp16 product with fp32
+    accumulation per step, the default for 16-bit inputs — or ``"fp32"`` — three products over split
+    values (22 bits), the default for fp32. On the GPU it runs csrc/kernels/newton_schulz.hip; CPU
+    tensors take the formula in fp32 torch operations.
+    """
+    if x.dim() < 2:
+        raise ValueError("orthogonalize: a matrix or a batch of matrices is needed (got shape %s)" % (tuple(x.shape),))
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("orthogonalize: float32, bfloat16 or float16 is needed (got %s)" % x.dtype)
+    if precision not in (None, "fp32", "fp16"):
+        raise ValueError("orthogonalize: precision must be 'fp32' or 'fp16' (got %r)" % (precision,))
+    if len(coefficients) != 3:
+        raise ValueError("orthogonalize: three coefficients are needed")
+    if not 0 <= int(steps) <= 100:
+        raise ValueError("orthogonalize: steps must be within 0..100 (got %r)" % (steps,))
+    a, b, c = (float(v) for v in coefficients)
+    if x.is_cuda:
+        from . import _native
+
+        _native.require_kernels()
+        split = precision == "fp32" or (precision is None and x.dtype == torch.float32)
+        out = torch.ops.mihvd.newton_schulz(x.detach().reshape(-1, *x.shape[-2:]), int(steps), a, b, c, float(eps), split)
+        return out.view(x.shape)
+    z = x.detach().float()
+    z = z / (torch.linalg.vector_norm(z, dim=(-2, -1), keepdim=True) + eps)
+    tall = z.shape[-2] > z.shape[-1]
+    if tall:
+        z = z.transpose(-2, -1)
+    for _ in range(int(steps)):
+        gram = z @ z.transpose(-2, -1)
+        z = a * z + (b * gram + c * (gram @ gram)) @ z
+    return (z.transpose(-2, -1) if tall else z).to(x.dtype).contiguous()
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update is orthogonalised (:func:`orthogonalize`), for the matrices of a model:
+
+        m = momentum * m + g;   u = g + momentum * m  (``nesterov``)  or  m
+        p = p (1 - lr * weight_decay) - lr * s * orthogonalize(u)
+
+    ``scale="spectral"``: s = sqrt(max(1, rows / cols)); ``"rms"``: s = 0.2 sqrt(max(rows, cols)), which
+    gives updates of AdamW's size, so that its learning rate and decay carry over. Parameters of more
+    than two dimensions count as [first, rest]. Vectors, embeddings and heads belong to another
+    optimizer (``FusedAdam``); parameters of fewer than two dimensions are refused.
+
+    fp32 contiguous GPU parameters take one fused path (``torch.ops.mihvd.muon_step``: matrices of one
+    shape run together, momentum, products and weight update in the kernels, no host
+    synchronisation, capturable); others use torch operations around :func:`orthogonalize`.
+    ``precision`` is that of the products (see there).
+    """
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5,
+                 ns_coefficients=NS_COEFFICIENTS, eps=1e-7, scale="spectral", precision="fp32"):
+        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
+            raise ValueError("Muon: lr and weight_decay must not be negative, momentum must be within [0, 1)")
+        if not 0 <= int(ns_steps) <= 100:
+            raise ValueError("Muon: ns_steps must be within 0..100")
+        if scale not in ("spectral", "rms"):
+            raise ValueError("Muon: scale must be 'spectral' or 'rms'")
+        if precision not in ("fp32", "fp16"):
+            raise ValueError("Muon: precision must be 'fp32' or 'fp16'")
+        if len(ns_coefficients) != 3:
+            raise ValueError("Muon: three ns_coefficients are needed")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      ns_steps=int(ns_steps), ns_coefficients=tuple(ns_coefficients), eps=eps,
+                                      scale=scale, precision=precision))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError("Muon: parameters must have at least two dimensions (got shape %s); give vectors to "
+                                 "another optimizer" % (tuple(p.shape),))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            fused = ([], [], [])
+            for p in params:
+                st = self.state[p]
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                m = st["momentum_buffer"]
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon: sparse gradients are not supported")
+                if all(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() for t in (p, p.grad, m)):
+                    for lst, t in zip(fused, (p, p.grad, m)):
+                        lst.append(t)
+                else:
+                    self._plain(group, p, m)
+            if fused[0]:
+                from . import _native
+
+                _native.require_kernels()
+                a, b, c = group["ns_coefficients"]
+                torch.ops.mihvd.muon_step(*fused, float(group["lr"]), group["momentum"], bool(group["nesterov"]),
+                                          group["weight_decay"], group["ns_steps"], a, b, c, group["eps"],
+                                          0 if group["scale"] == "spectral" else 1, group["precision"] == "fp32")
+        return loss
+
+    @staticmethod
+    def _plain(group, p, m):
+        g, mu, lr = p.grad, group["momentum"], group["lr"]
+        m.mul_(mu).add_(g)
+        u = g.add(m, alpha=mu) if group["nesterov"] else m
+        rows, cols = p.shape[0], p.numel() // max(1, p.shape[0])
+        if not p.numel():
+            return
+        s = math.sqrt(max(1.0, rows / cols)) if group["scale"] == "spectral" else 0.2 * math.sqrt(max(rows, cols))
+        o = orthogonalize(u.reshape(rows, cols), group["ns_steps"], group["ns_coefficients"], group["eps"],
+                          group["precision"])
+        p.mul_(1.0 - lr * group["weight_decay"]).add_(o.view(p.shape), alpha=-lr * s)
