@@ -133,7 +133,7 @@ void up_gate(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, 
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch<g16::KC, g16::KC, 128, 128, 2, 2, true>(a, EpiGate<ACT>{g, u, h, s.F8}, st);
+  g16::launch<g16::KC, g16::KC, true>(g16::plan(s.N, 2 * (int64_t)s.F, s.K, 1, 1, false, false).tile, a, EpiGate<ACT>{g, u, h, s.F8}, st);
 }
 
 template <int ACT>
@@ -145,7 +145,7 @@ void grad_gate(const FfnShape& s, const u16* dy, int64_t lddy, const FfnWeights&
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch<g16::KC, g16::KS, 128, 128, 2, 2>(a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
+  g16::launch<g16::KC, g16::KS>(g16::plan(s.N, s.F, s.K, 1, 1, false, false).tile, a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
 }
 
 }  // namespace

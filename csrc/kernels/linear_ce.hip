@@ -71,8 +71,7 @@ struct EpiStats {
           for (int j = 0; j < MI; ++j) acc[i][j][k] += b;
         }
     }
-    const int wn_per_tile = 2;
-    const int slot = c.nt * wn_per_tile + c.wn;
+    const int slot = c.nt * 2 + c.wn;  // two waves along a tile's columns
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
       const int m = c.m0 + j * 16 + (c.lane & 15);
@@ -244,15 +243,22 @@ __global__ void __launch_bounds__(256) lce_dh(const float* __restrict__ slab, in
 }  // namespace
 
 #ifndef MIHVD_F16
-int lce_splits(int64_t rows, int64_t hidden, int64_t piece) {
-  return g16::pick_splits((int64_t)g16::cdiv(rows, 128) * g16::cdiv(hidden, 128), g16::cdiv(piece, g16::BK));
+void lce_plan(LceShape& s) {
+  s.tile = g16::plan(s.N, s.V, s.K, 1, 1, false, false).tile;
+  s.npart = g16::cdiv(s.V, s.tile) * 2;
+}
+void lce_plan_backward(LceShape& s, LceScratch& x) {
+  lce_plan(s);
+  const g16::Plan p = g16::plan(s.N, s.K, x.piece, 1, 1, false, true);
+  x.dh_tile = p.tile;
+  x.splits = p.splits;
+  x.dw_tile = g16::plan(std::min(x.piece, s.V), s.K, s.N, 1, 1, false, false).tile;
 }
 #endif
 
 void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t hs0, int64_t hs1, const u16* w, int64_t ldw,
                     const void* bias, int bias_kind, u16* hc, float2* part, float* zlab, float* lse, float* rows,
                     float* loss, int mean, hipStream_t st) {
-  const int npart = lce_npart(s.V);
   lce_gather<<<g16::cdiv(s.N, 4), 256, 0, st>>>(h, hs0, hs1, rw.idx, rw.cnt, s.K, s.K8, hc);
   g16::Args a;
   a.m.p[0] = hc;
@@ -265,9 +271,9 @@ void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t 
   a.N = s.V;
   a.K = s.K;
   a.dyn_m = rw.cnt;
-  EpiStats e{bias, bias_kind, rw.label, part, npart, zlab};
-  g16::launch<g16::KC, g16::KC, 128, 128, 2, 2>(a, e, st);
-  lce_finish<<<g16::cdiv(s.N, 16), 256, 0, st>>>(part, npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
+  EpiStats e{bias, bias_kind, rw.label, part, s.npart, zlab};
+  g16::launch<g16::KC, g16::KC>(s.tile, a, e, st);
+  lce_finish<<<g16::cdiv(s.N, 16), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
   if (loss) lce_reduce<<<1, 1024, 0, st>>>(rows, s.N, rw.cnt, mean, loss);
 }
 
@@ -290,11 +296,11 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       a.K = s.K;
       a.dyn_m = rw.cnt;
       EpiDz e{bias, bias_kind, rw.label, lse, g.rowscale, v0, x.dz, x.ldz, db ? x.dbp : nullptr, 2};
-      g16::launch<g16::KC, g16::KC, 128, 128, 2, 2>(a, e, st);
+      g16::launch<g16::KC, g16::KC>(s.tile, a, e, st);
     }
     if (db) {
       const int esz = bias_kind == 1 ? 4 : 2;
-      lce_db<<<g16::cdiv(nv, 256), 256, 0, st>>>(x.dbp, x.ldz, rw.cnt, 128, 2, nv, g.scale,
+      lce_db<<<g16::cdiv(nv, 256), 256, 0, st>>>(x.dbp, x.ldz, rw.cnt, s.tile, 2, nv, g.scale,
                                                  static_cast<char*>(db) + (int64_t)v0 * esz, bias_kind);
     }
     if (dw) {
@@ -310,7 +316,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       a.K = s.N;
       a.dyn_k = rw.cnt;
       g16::EpiStore e{{dw + (int64_t)v0 * s.K, nullptr}, s.K, 1.f / DZ_SCALE, g.scale};
-      g16::launch<g16::KS, g16::KS, 128, 128, 2, 2>(a, e, st);
+      g16::launch<g16::KS, g16::KS>(x.dw_tile, a, e, st);
     }
     if (dh) {
       g16::Args a;
@@ -326,7 +332,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       a.splits = x.splits;
       a.dyn_m = rw.cnt;
       g16::EpiSlab e{x.slab, s.K8, (int64_t)s.N * s.K8, x.splits, first ? 0 : 1};
-      g16::launch<g16::KC, g16::KS, 128, 128, 2, 2>(a, e, st);
+      g16::launch<g16::KC, g16::KS>(x.dh_tile, a, e, st);
     }
   }
   if (dh) {

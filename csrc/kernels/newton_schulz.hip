@@ -67,19 +67,19 @@ __device__ __forceinline__ void put_planes(u16* p, int64_t plane, int planes, fl
   if (planes == 2) p[plane] = f2bf(v - bf2f(hi));
 }
 
-__global__ void __launch_bounds__(256) ns_scale(const NsTable t, int rows, int cols, int c8, int planes, int kind,
+__global__ void __launch_bounds__(256) ns_scale(const NsTable t, int rows, int cols, int rp, int cp, int planes, int kind,
                                                 int muon, float mu, int nesterov, float eps,
                                                 const float* __restrict__ partial, u16* __restrict__ x) {
   const int b = blockIdx.y, lane = threadIdx.x & 63;
   const float norm = sqrtf(wave_sum(partial[b * NS_PART + lane]));
   const float inv = S / (norm + eps);
-  const int64_t plane = (int64_t)rows * c8;
+  const int64_t plane = (int64_t)rp * cp;
   u16* o = x + (int64_t)b * planes * plane;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / c8;
-    const int c = (int)(i - r * c8);
+    const int64_t r = i / cp;
+    const int c = (int)(i - r * cp);
     float v = 0.f;
-    if (c < cols) {
+    if (r < rows && c < cols) {
       const int64_t k = r * cols + c;
       v = load_src(t.src[b], kind, k);
       if (muon) {
@@ -110,7 +110,7 @@ struct EpiPlanes {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        if (n >= ld) continue;
+        if (n >= c.N) continue;  // N is a multiple of 64
         const int64_t at = (int64_t)m * ld + n;
         float v[4] = {alpha * acc[i][j][0], alpha * acc[i][j][1], alpha * acc[i][j][2], alpha * acc[i][j][3]};
         if (q) {
@@ -122,8 +122,6 @@ struct EpiPlanes {
             v[3] = fmaf(beta, bf2f((u16)(w.y >> 16)), v[3]);
           }
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = n + k < c.N ? v[k] : 0.f;  // the padding stays zero
         const uint2 hi = pack4bf(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<uint2*>(o + at) = hi;
         const float lo[4] = {v[0] - bf2f((u16)hi.x), v[1] - bf2f((u16)(hi.x >> 16)), v[2] - bf2f((u16)hi.y),
@@ -137,11 +135,10 @@ struct EpiPlanes {
           const u16 h4[4] = {(u16)hi.x, (u16)(hi.x >> 16), (u16)hi.y, (u16)(hi.y >> 16)};
           const u16 l4[4] = {(u16)lw.x, (u16)(lw.x >> 16), (u16)lw.y, (u16)(lw.y >> 16)};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n + k < c.N) {
-              o[(int64_t)(n + k) * ld + m] = h4[k];
-              if (planes == 2) o[plane + (int64_t)(n + k) * ld + m] = l4[k];
-            }
+          for (int k = 0; k < 4; ++k) {
+            o[(int64_t)(n + k) * ld + m] = h4[k];
+            if (planes == 2) o[plane + (int64_t)(n + k) * ld + m] = l4[k];
+          }
         }
       }
     }
@@ -153,7 +150,7 @@ struct EpiFinal {
   NsOut out;
   const u16* in;
   int64_t ld, plane;
-  int planes, cols, kind, muon;
+  int planes, rows, cols, kind, muon;
   float alpha, beta, decay, step;
   template <int NI, int MI>
   __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
@@ -162,13 +159,13 @@ struct EpiFinal {
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= c.M) continue;
+      if (m >= rows) continue;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (n + k >= c.N) continue;
+          if (n + k >= cols) continue;
           float v = alpha * acc[i][j][k];
           for (int p = 0; p < planes; ++p) v = fmaf(beta, bf2f(q[p * plane + (int64_t)m * ld + n + k]), v);
           const int64_t at = (int64_t)m * cols + n + k;
@@ -189,13 +186,13 @@ struct EpiFinal {
 };
 
 // steps == 0: the normalised matrix itself
-__global__ void __launch_bounds__(256) ns_copy_out(const u16* __restrict__ x, const NsOut out, int rows, int cols, int c8,
-                                                   int planes, int kind, int muon, float decay, float step) {
+__global__ void __launch_bounds__(256) ns_copy_out(const u16* __restrict__ x, const NsOut out, int rows, int cols, int rp,
+                                                   int cp, int planes, int kind, int muon, float decay, float step) {
   const int b = blockIdx.y;
-  const int64_t plane = (int64_t)rows * c8, n = (int64_t)rows * cols;
+  const int64_t plane = (int64_t)rp * cp, n = (int64_t)rows * cols;
   const u16* q = x + (int64_t)b * planes * plane;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols, at = r * c8 + (i - r * cols);
+    const int64_t r = i / cols, at = r * cp + (i - r * cols);
     float v = bf2f(q[at]);
     if (planes == 2) v += bf2f(q[plane + at]);
     v *= INV_S;
@@ -235,58 +232,61 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     tab.mom[i] = g.mom[i];
     out.dst[i] = g.dst[i];
   }
-  const int64_t n = (int64_t)g.rows * g.cols, px = (int64_t)g.rows * g.c8, pa = (int64_t)g.side * g.s8;
+  const int64_t n = (int64_t)g.rows * g.cols, px = (int64_t)g.rp * g.cp, pa = (int64_t)g.sp * g.sp;
   const int grid = (int)std::min<int64_t>(512, (px + 255) / 256);
   ns_norm<<<dim3(NS_PART, g.count), 256, 0, st>>>(tab, n, p.src_kind, p.muon, p.momentum, p.nesterov, sc.partial);
-  ns_scale<<<dim3(grid, g.count), 256, 0, st>>>(tab, g.rows, g.cols, g.c8, g.planes, p.src_kind, p.muon, p.momentum,
+  ns_scale<<<dim3(grid, g.count), 256, 0, st>>>(tab, g.rows, g.cols, g.rp, g.cp, g.planes, p.src_kind, p.muon, p.momentum,
                                                p.nesterov, p.eps, sc.partial, sc.x0);
   const float step = p.lr * p.scale;
   if (p.steps == 0) {
-    ns_copy_out<<<dim3(grid, g.count), 256, 0, st>>>(sc.x0, out, g.rows, g.cols, g.c8, g.planes, p.src_kind, p.muon,
+    ns_copy_out<<<dim3(grid, g.count), 256, 0, st>>>(sc.x0, out, g.rows, g.cols, g.rp, g.cp, g.planes, p.src_kind, p.muon,
                                                      p.decay, step);
     return;
   }
-  const bool tall = g.rows > g.cols;
+  // All sides are padded to 64 with zeros, which the products keep: a zero row or column of X gives zero
+  // rows and columns of A, B and the next X.
+  const bool tall = g.rp > g.cp;
   const int nseg = g.planes == 2 ? 3 : 1;
+  const int big = std::max(g.rp, g.cp);
+  const int t_gram = plan(g.sp, g.sp, big, nseg, g.count, true, false).tile;
+  const int t_poly = plan(g.sp, g.sp, g.sp, nseg, g.count, true, false).tile;
+  const int t_upd = plan(g.rp, g.cp, g.sp, nseg, g.count, false, false).tile;
   u16 *x = sc.x0, *y = sc.x1;
   for (int it = 0; it < p.steps; ++it) {
     Args a;
     a.batch = g.count;
     a.nseg = nseg;
     a.sym = 1;
-    a.M = a.N = g.side;
-    EpiPlanes gram{sc.gram, nullptr, g.s8, pa, g.planes, 1, INV_S, 0.f};
-    if (tall) {
-      a.K = g.rows;
-      a.m = plane_side(x, g.c8, g.c8, px, g.planes, false);
-      a.n = plane_side(x, g.c8, g.c8, px, g.planes, true);
-      launch<KS, KS, 128, 128, 2, 2>(a, gram, st);
-    } else {
-      a.K = g.cols;
-      a.m = plane_side(x, g.c8, g.rows, px, g.planes, false);
-      a.n = plane_side(x, g.c8, g.rows, px, g.planes, true);
-      launch<KC, KC, 128, 128, 2, 2>(a, gram, st);
-    }
-    a.K = g.side;
-    a.m = plane_side(sc.gram, g.s8, g.side, pa, g.planes, false);
-    a.n = plane_side(sc.gram, g.s8, g.side, pa, g.planes, true);
-    launch<KC, KC, 128, 128, 2, 2>(a, EpiPlanes{sc.poly, sc.gram, g.s8, pa, g.planes, 1, p.c * INV_S, p.b}, st);
+    a.M = a.N = g.sp;
+    a.K = big;
+    const Side xk = plane_side(x, g.cp, g.rp, px, g.planes, false);       // rows of X
+    const Side xk2 = plane_side(x, g.cp, g.rp, px, g.planes, true);
+    const Side xs = plane_side(x, g.cp, g.cp, px, g.planes, false);       // columns of X
+    const Side xs2 = plane_side(x, g.cp, g.cp, px, g.planes, true);
+    const EpiPlanes gram{sc.gram, nullptr, g.sp, pa, g.planes, 1, INV_S, 0.f};
+    a.m = tall ? xs : xk;
+    a.n = tall ? xs2 : xk2;
+    if (tall) launch<KS, KS>(t_gram, a, gram, st);
+    else launch<KC, KC>(t_gram, a, gram, st);
+    a.K = g.sp;
+    a.m = plane_side(sc.gram, g.sp, g.sp, pa, g.planes, false);
+    a.n = plane_side(sc.gram, g.sp, g.sp, pa, g.planes, true);
+    launch<KC, KC>(t_poly, a, EpiPlanes{sc.poly, sc.gram, g.sp, pa, g.planes, 1, p.c * INV_S, p.b}, st);
     a.sym = 0;
-    a.M = g.rows;
-    a.N = g.cols;
-    const bool last = it + 1 == p.steps;
-    EpiPlanes upd{y, x, g.c8, px, g.planes, 0, INV_S, p.a};
-    EpiFinal fin{out, x, g.c8, px, g.planes, g.cols, p.src_kind, p.muon, INV_S * INV_S, p.a * INV_S, p.decay, step};
-    if (tall) {  // X B: rows of X against rows of the symmetric B
-      a.m = plane_side(x, g.c8, g.rows, px, g.planes, false);
-      a.n = plane_side(sc.poly, g.s8, g.side, pa, g.planes, true);
-      if (last) launch<KC, KC, 128, 128, 2, 2>(a, fin, st);
-      else launch<KC, KC, 128, 128, 2, 2>(a, upd, st);
+    a.M = g.rp;
+    a.N = g.cp;
+    // tall: X B, rows of X against rows of the symmetric B; else B X
+    a.m = tall ? xk : plane_side(sc.poly, g.sp, g.sp, pa, g.planes, false);
+    a.n = tall ? plane_side(sc.poly, g.sp, g.sp, pa, g.planes, true) : xs2;
+    if (it + 1 < p.steps) {
+      const EpiPlanes upd{y, x, g.cp, px, g.planes, 0, INV_S, p.a};
+      if (tall) launch<KC, KC>(t_upd, a, upd, st);
+      else launch<KC, KS>(t_upd, a, upd, st);
     } else {
-      a.m = plane_side(sc.poly, g.s8, g.side, pa, g.planes, false);
-      a.n = plane_side(x, g.c8, g.c8, px, g.planes, true);
-      if (last) launch<KC, KS, 128, 128, 2, 2>(a, fin, st);
-      else launch<KC, KS, 128, 128, 2, 2>(a, upd, st);
+      const EpiFinal fin{out, x, g.cp, px, g.planes, g.rows, g.cols, p.src_kind, p.muon, INV_S * INV_S, p.a * INV_S,
+                         p.decay, step};
+      if (tall) launch<KC, KC>(t_upd, a, fin, st);
+      else launch<KC, KS>(t_upd, a, fin, st);
     }
     std::swap(x, y);
   }

@@ -14,6 +14,7 @@ typedef unsigned short u16;
 
 struct LceShape {
   int N, K, K8, V;  // rows, hidden size, hidden size padded to 8, vocabulary
+  int tile, npart;  // of the logits: output tile, (max, sum) pairs per row (two waves along a tile)
 };
 // The labelled rows: compact position -> row, row -> compact position or -1, their labels and count.
 struct LceRows {
@@ -31,14 +32,13 @@ struct LceScratch {
   int64_t ldz;   // row stride of dz, a multiple of 8
   u16* dz;       // [N][ldz]
   float* dbp;    // [2 * tiles of rows][ldz]
-  int splits;
+  int splits, dh_tile, dw_tile;
   float* slab;   // [splits][N][K8]
 };
 
-// (max, sum) pairs per row: two waves along each 128-wide vocabulary tile
-inline int lce_npart(int V) { return (V + 127) / 128 * 2; }
-// k splits of the hidden gradient's product over a piece of the vocabulary
-int lce_splits(int64_t rows, int64_t hidden, int64_t piece);
+// How the products of a shape run (tiles, k splits of the hidden gradient); x.piece is set.
+void lce_plan(LceShape& s);
+void lce_plan_backward(LceShape& s, LceScratch& x);
 
 #define MIHVD_TRANSFORMER_DECLS                                                                                        \
   void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t hs0, int64_t hs1, const u16* w,      \
@@ -71,7 +71,8 @@ MIHVD_TRANSFORMER_DECLS
 // Newton-Schulz (newton_schulz.hip): one group of equally shaped matrices.
 constexpr int NS_MAX = 32;
 struct NsGroup {
-  int count, rows, cols, c8, side, s8;  // side = min(rows, cols); *8: padded to 8
+  int count, rows, cols;
+  int rp, cp, sp;  // rows, cols and the smaller of them, padded to the products' k tile of 64
   int planes;                           // 1: fp16; 2: fp16 hi + lo
   const void* src[NS_MAX];              // u (orthogonalize) / gradient (Muon)
   void* dst[NS_MAX];                    // result / weight

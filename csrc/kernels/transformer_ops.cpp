@@ -173,8 +173,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   int* m = meta.data_ptr<int>();
   lce_compact<<<1, 1024, 0, st>>>(lab.data_ptr<int64_t>(), (int)N, (int)V, ignore_index, m, m + N, m + 2 * N, m + 3 * N);
   const Mat wm = mat(w);
-  at::Tensor part = at::empty({N, lce_npart((int)V), 2}, f32), zlab = at::empty({N}, f32);
-  const LceShape s{(int)N, (int)K, (int)K8, (int)V};
+  LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0};
+  lce_plan(s);
+  at::Tensor part = at::empty({N, s.npart, 2}, f32), zlab = at::empty({N}, f32);
   auto run = h.scalar_type() == at::kHalf ? &f16::lce_forward_16 : &lce_forward_16;
   run(s, rows_of(meta, N), p16(h), h.stride(0), h.stride(1), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr,
       bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part.data_ptr<float>()), zlab.data_ptr<float>(),
@@ -218,18 +219,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   LceScratch x{};
   x.piece = (int)std::min<int64_t>(up8(V), std::max<int64_t>(256, DZ_BYTES / (2 * N) / 256 * 256));
   x.ldz = up8(x.piece);
+  LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0};
+  lce_plan_backward(s, x);
   at::Tensor dz = at::empty({N, x.ldz}, w.options()), dbp, slab;
   x.dz = m16(dz);
   if (need_b) {
-    dbp = at::empty({2 * cdiv(N, 128), x.ldz}, f32);
+    dbp = at::empty({2 * cdiv(N, s.tile), x.ldz}, f32);
     x.dbp = dbp.data_ptr<float>();
   }
   if (need_h) {
-    x.splits = lce_splits(N, K, x.piece);
     slab = at::empty({x.splits, N, K8}, f32);
     x.slab = slab.data_ptr<float>();
   }
-  const LceShape s{(int)N, (int)K, (int)K8, (int)V};
   const LceGrad g{scale.data_ptr<float>(), reduction ? nullptr : rowscale.data_ptr<float>()};
   auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
   run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias), lse.data_ptr<float>(), x, m16(dh),
@@ -328,7 +329,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
 constexpr int64_t NS_ELEMS = int64_t(1) << 28;  // elements of X per launch group (bounds the workspace)
 
 void ns_group(NsGroup& g, NsParams& p, const at::TensorOptions& opt) {
-  const int64_t px = (int64_t)g.rows * g.c8, pa = (int64_t)g.side * g.s8, k = (int64_t)g.count * g.planes;
+  const int64_t px = (int64_t)g.rp * g.cp, pa = (int64_t)g.sp * g.sp, k = (int64_t)g.count * g.planes;
   const auto h = opt.dtype(at::kHalf);
   at::Tensor x0 = at::empty({k * px}, h), x1, gram, poly;
   if (p.steps > 0) {
@@ -344,9 +345,9 @@ void ns_shape(NsGroup& g, int64_t rows, int64_t cols, bool split) {
   TORCH_CHECK_VALUE(rows <= MAX_LD && cols <= MAX_LD, "orthogonalize: sides above ", MAX_LD, " are not supported");
   g.rows = (int)rows;
   g.cols = (int)cols;
-  g.c8 = (int)up8(cols);
-  g.side = (int)std::min(rows, cols);
-  g.s8 = (int)up8(g.side);
+  g.rp = (int)cdiv(rows, 64) * 64;
+  g.cp = (int)cdiv(cols, 64) * 64;
+  g.sp = std::min(g.rp, g.cp);
   g.planes = split ? 2 : 1;
 }
 
