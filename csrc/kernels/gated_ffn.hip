@@ -28,9 +28,15 @@ __device__ __forceinline__ void act_both(float x, float& a, float& d) {
     a = x * s;
     d = s * (1.f + x * (1.f - s));
   } else if constexpr (ACT == ACT_GELU) {
-    const float c = 0.5f * (1.f + erff(x * 0.70710678f));
+    // Phi(x) by Abramowitz & Stegun 7.1.26: for z = |x| / sqrt(2), erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2)
+    // with t = 1 / (1 + p z), |error| <= 1.5e-7; its exponential is the one that the density needs
+    const float z = fabsf(x) * 0.70710678f;
+    const float e = __expf(-z * z), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.f));
+    const float q = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t,
+                         0.254829592f) * t * e * 0.5f;
+    const float c = x < 0.f ? q : 1.f - q;
     a = x * c;
-    d = c + x * 0.39894228f * __expf(-0.5f * x * x);
+    d = fmaf(x * 0.39894228f, e, c);
   } else if constexpr (ACT == ACT_GELU_TANH) {
     // 0.5 (1 + tanh(q)) = sigmoid(2 q)
     const float q = 0.79788456f * (x + 0.044715f * x * x * x);
@@ -52,16 +58,29 @@ struct EpiGate {
   u16 *g, *u, *h;  // [N][F8]; g and u null without gradients
   int64_t ld;
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+  struct Pre {};
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
     constexpr int H = NI / 2;
+    const g16::RowStage<H * 16> st{c.stage, c.lane};
+    g16::unroll<MI>([&](auto J) {
+      constexpr int j = J.value;
+      g16::pin(acc, j);
+      auto out = [&](u16* o) {
+        st.turn();
 #pragma unroll
-    for (int j = 0; j < MI; ++j) {
-      const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= c.M) continue;
+        for (int q = 0; q < st.GETS; ++q) {
+          const int m = c.m0 + j * 16 + st.row(q), n = c.n0 + st.col();
+          const uint4 v = st.get(q);
+          if (m < c.M && n < ld) *reinterpret_cast<uint4*>(o + (int64_t)m * ld + n) = v;
+        }
+        st.turn();
+      };
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        if (n >= ld) continue;
         float v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -69,50 +88,103 @@ struct EpiGate {
           act_both<ACT>(acc[i][j][k], a, d);
           v[k] = n + k < c.N ? a * acc[i + H][j][k] : 0.f;  // columns F..F8: zeros for the next product
         }
-        const int64_t o = (int64_t)m * ld + n;
-        *reinterpret_cast<uint2*>(h + o) = pack4bf(v[0], v[1], v[2], v[3]);
-        if (g) {
-          *reinterpret_cast<uint2*>(g + o) = pack4bf(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-          *reinterpret_cast<uint2*>(u + o) = pack4bf(acc[i + H][j][0], acc[i + H][j][1], acc[i + H][j][2], acc[i + H][j][3]);
-        }
+        st.put(i, pack4bf(v[0], v[1], v[2], v[3]));
       }
-    }
+      out(h);
+      if (g) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) st.put(i, pack4bf(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]));
+        out(g);
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+          st.put(i, pack4bf(acc[i + H][j][0], acc[i + H][j][1], acc[i + H][j][2], acc[i + H][j][3]));
+        out(u);
+      }
+    });
   }
 };
 
+__device__ __forceinline__ void unpack4(uint2 q, float (&v)[4]) {
+  v[0] = bf2f((u16)q.x);
+  v[1] = bf2f((u16)(q.x >> 16));
+  v[2] = bf2f((u16)q.y);
+  v[3] = bf2f((u16)(q.y >> 16));
+}
+
+// g and u come from memory as they went there: whole rows of 16 bytes a lane, turned into the
+// accumulators' layout in LDS, and dg and du back.
 template <int ACT>
 struct EpiGateGrad {
   const u16 *g, *u;  // [N][ld]
   u16* dgu;          // [N][2 ld]: dg, then du
   int64_t ld;
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+  struct Pre {};
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
+    const g16::RowStage<NI * 16> st{c.stage, c.lane};
+    constexpr int G = st.GETS;
+    uint4 gq[G], uq[G];
+    auto fetch = [&](int j) {
 #pragma unroll
-    for (int j = 0; j < MI; ++j) {
-      const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= c.M) continue;
+      for (int q = 0; q < G; ++q) {
+        const int m = min(c.m0 + j * 16 + st.row(q), c.M - 1);
+        const int64_t o = (int64_t)m * ld + min(c.n0 + st.col(), (int)ld - 8);
+        gq[q] = *reinterpret_cast<const uint4*>(g + o);
+        uq[q] = *reinterpret_cast<const uint4*>(u + o);
+      }
+    };
+    fetch(0);
+    g16::unroll<MI>([&](auto J) {
+      constexpr int j = J.value;
+      g16::pin(acc, j);
+      auto turned = [&](const uint4 (&q)[G], uint2 (&r)[NI]) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) st.set(k, q[k]);
+        st.turn();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) r[i] = st.take(i);
+        st.turn();
+      };
+      uint2 gr[NI], ur[NI];
+      turned(gq, gr);
+      turned(uq, ur);
+      if (j + 1 < MI) fetch(j + 1);
+      uint2 du[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        if (n >= ld) continue;
-        const int64_t o = (int64_t)m * ld + n;
-        const uint2 gq = *reinterpret_cast<const uint2*>(g + o), uq = *reinterpret_cast<const uint2*>(u + o);
-        const float gv[4] = {bf2f((u16)gq.x), bf2f((u16)(gq.x >> 16)), bf2f((u16)gq.y), bf2f((u16)(gq.y >> 16))};
-        const float uv[4] = {bf2f((u16)uq.x), bf2f((u16)(uq.x >> 16)), bf2f((u16)uq.y), bf2f((u16)(uq.y >> 16))};
-        float dg[4], du[4];
+        float gv[4], uv[4], x[4], y[4];
+        unpack4(gr[i], gv);
+        unpack4(ur[i], uv);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float a, d;
           act_both<ACT>(gv[k], a, d);
           const bool in = n + k < c.N;
-          dg[k] = in ? acc[i][j][k] * uv[k] * d : 0.f;
-          du[k] = in ? acc[i][j][k] * a : 0.f;
+          x[k] = in ? acc[i][j][k] * uv[k] * d : 0.f;
+          y[k] = in ? acc[i][j][k] * a : 0.f;
         }
-        u16* q = dgu + (int64_t)m * 2 * ld + n;
-        *reinterpret_cast<uint2*>(q) = pack4bf(dg[0], dg[1], dg[2], dg[3]);
-        *reinterpret_cast<uint2*>(q + ld) = pack4bf(du[0], du[1], du[2], du[3]);
+        st.put(i, pack4bf(x[0], x[1], x[2], x[3]));
+        du[i] = pack4bf(y[0], y[1], y[2], y[3]);
       }
-    }
+      auto out = [&](u16* o) {
+        st.turn();
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+          const int m = c.m0 + j * 16 + st.row(q), n = c.n0 + st.col();
+          const uint4 v = st.get(q);
+          if (m < c.M && n < ld) *reinterpret_cast<uint4*>(o + (int64_t)m * 2 * ld + n) = v;
+        }
+        st.turn();
+      };
+      out(dgu);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) st.put(i, du[i]);
+      out(dgu + ld);
+    });
   }
 };
 
@@ -145,7 +217,7 @@ void grad_gate(const FfnShape& s, const u16* dy, int64_t lddy, const FfnWeights&
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch<g16::KC, g16::KS>(g16::plan(s.N, s.F, s.K, 1, 1, false, false).tile, a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
+  g16::launch_tile<g16::KC, g16::KS, 128, 128, 2, 2>(a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
 }
 
 }  // namespace

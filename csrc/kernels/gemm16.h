@@ -46,9 +46,9 @@ struct Side {
 struct Args {
   Side m, n;
   int M = 0, N = 0, K = 0;  // K: per segment
-  int nseg = 1, batch = 1, splits = 1;  // three segments need K % 64 == 0
+  int nseg = 1, batch = 1, splits = 1;
   int sym = 0;                  // out is symmetric (M == N): only tiles with nt >= mt run
-  const int* dyn_m = nullptr;   // device count that replaces M (tiles past it exit)
+  const int* dyn_m = nullptr;   // device count that replaces M (tiles past it do not run)
   const int* dyn_k = nullptr;   // device count that replaces K
   int tiles_m = 0, tiles_n = 0; // filled by launch()
 };
@@ -60,6 +60,31 @@ struct Ctx {
   int mt, nt;      // tile indices
   int wm, wn;      // wave position in the tile
   int batch, split, lane;
+  u16* stage;      // this wave's LDS for RowStage
+};
+
+// 16 rows of 16-bit results on their way out, in LDS that only this wave uses: a lane's four
+// consecutive values go in where the accumulators hold them (16 rows, 32 bytes of each), and come back
+// as 16 bytes of a row, so that a store instruction writes whole rows of the wave's tile. Rows are
+// padded by 16 bytes: both directions are free of bank conflicts.
+template <int COLS>
+struct RowStage {
+  static constexpr int RS = COLS + 8, CH = COLS / 8, GETS = 16 * CH / 64;
+  u16* p;
+  int lane;
+  __device__ __forceinline__ void put(int i, uint2 v) const {
+    *reinterpret_cast<uint2*>(p + (lane & 15) * RS + i * 16 + 4 * (lane >> 4)) = v;
+  }
+  __device__ __forceinline__ uint2 take(int i) const {
+    return *reinterpret_cast<const uint2*>(p + (lane & 15) * RS + i * 16 + 4 * (lane >> 4));
+  }
+  __device__ __forceinline__ void set(int g, uint4 v) const { *reinterpret_cast<uint4*>(p + row(g) * RS + col()) = v; }
+  __device__ __forceinline__ static void turn() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+  __device__ __forceinline__ int row(int g) const { return lane / CH + g * (64 / CH); }
+  __device__ __forceinline__ int col() const { return (lane % CH) * 8; }
+  __device__ __forceinline__ uint4 get(int g) const {
+    return *reinterpret_cast<const uint4*>(p + row(g) * RS + col());
+  }
 };
 
 // Row permutation of a KS image: 16-byte chunks of k row `k` are XORed with 2*h(k), so that the
@@ -70,30 +95,124 @@ __device__ __forceinline__ int ks_h(int k) {
   else return ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
 }
 
+// A wave-uniform value into a scalar register. In asm because the compiler drops its own readfirstlane
+// where it knows the value to be uniform, and may then keep it, and what follows from it, in vector
+// registers. The waits: one state between a vector instruction that writes x and the lane read (gfx940
+// and later need it), five before a memory access that takes the result as its base.
+__device__ __forceinline__ int uni(int x) {
+  int r;
+  asm("s_nop 1\n\tv_readfirstlane_b32 %0, %1\n\ts_nop 4" : "=s"(r) : "v"(x));
+  return r;
+}
+
 // Direct global -> LDS copies of 16 bytes a lane (lane l's land at lds + 16 l; lds is wave-uniform).
 // Written in asm because the compiler, which cannot tell the two LDS buffers apart, waits for every
 // copy in flight before any LDS read; the kernel's own s_waitcnt before the barrier is the wait these
 // need. They have no destination registers, and later waits of the compiler's only get stricter.
 __device__ __forceinline__ void dma16(const char* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(lds), "v"(off), "s"(base) );
-}
-// the same with the lanes of `live`: all or none, so that a loop body needs no branch around its copies
-// (called where every lane of the wave is active)
-__device__ __forceinline__ void dma16_if(const char* base, uint32_t off, uint32_t lds, uint32_t live) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\t"
-               "global_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
-               :: "s"(lds), "v"(off), "s"(base), "s"(live) );
 }
 __device__ __forceinline__ void dma16_at(const char* addr, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(addr) );
+}
+// f(0), f(1), ... f(N - 1) with constants, whatever the unroller thinks of the size
+template <int N, class F, int I = 0>
+__device__ __forceinline__ void unroll(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unroll<N, F, I + 1>(static_cast<F&&>(f));
+  }
+}
+
+// Four MFMAs that accumulate in place. In asm so that the accumulators stay where they are (the compiler
+// moves them between registers when they fill the accumulation file) and the order of MFMAs, copies
+// and LDS reads stays as written; s_nop 1 covers operands that a vector instruction wrote just before.
+// BIG: 256 accumulators, in the accumulation registers; else any vector registers.
+#ifdef MIHVD_F16
+#define MIHVD_G16_MFMA "v_mfma_f32_16x16x32_f16"
+#else
+#define MIHVD_G16_MFMA "v_mfma_f32_16x16x32_bf16"
+#endif
+template <bool BIG>
+__device__ __forceinline__ void mfma4(f32x4& c0, f32x4& c1, f32x4& c2, f32x4& c3, const bf16x8& a, const bf16x8& b0,
+                                      const bf16x8& b1, const bf16x8& b2, const bf16x8& b3) {
+#define MIHVD_G16_ASM                                                                                           \
+  "s_nop 1\n\t" MIHVD_G16_MFMA " %0, %4, %5, %0\n\t" MIHVD_G16_MFMA " %1, %4, %6, %1\n\t" MIHVD_G16_MFMA       \
+  " %2, %4, %7, %2\n\t" MIHVD_G16_MFMA " %3, %4, %8, %3"
+  if constexpr (BIG)
+    asm volatile(MIHVD_G16_ASM : "+a"(c0), "+a"(c1), "+a"(c2), "+a"(c3) : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+  else
+    asm volatile(MIHVD_G16_ASM : "+v"(c0), "+v"(c1), "+v"(c2), "+v"(c3) : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+#undef MIHVD_G16_ASM
+}
+// The same with one or two of the tile's copies between them, each no longer than an MFMA: from base +
+// off to LDS l + at, by all lanes or none (`live`: a loop body then needs no branch around its copies;
+// every lane of the wave is active here).
+#define MIHVD_G16_COPY(OFF, BASE)                                                                       \
+  "s_mov_b64 exec, %10\n\tglobal_load_lds_dwordx4 " OFF ", " BASE "\n\ts_mov_b64 exec, -1\n\t"
+template <bool BIG>
+__device__ __forceinline__ void mfma4_copy(f32x4& c0, f32x4& c1, f32x4& c2, f32x4& c3, const bf16x8& a, const bf16x8& b0,
+                                           const bf16x8& b1, const bf16x8& b2, const bf16x8& b3, uint32_t l, uint64_t live,
+                                           int at, uint32_t off, const char* base) {
+#define MIHVD_G16_ASM                                                                                              \
+  "s_nop 1\n\t" MIHVD_G16_MFMA " %0, %4, %5, %0\n\ts_add_u32 m0, %9, %11\n\t" MIHVD_G16_MFMA                     \
+  " %1, %4, %6, %1\n\t" MIHVD_G16_COPY("%12", "%13") MIHVD_G16_MFMA " %2, %4, %7, %2\n\t" MIHVD_G16_MFMA     \
+  " %3, %4, %8, %3"
+  if constexpr (BIG)
+    asm volatile(MIHVD_G16_ASM : "+a"(c0), "+a"(c1), "+a"(c2), "+a"(c3)
+                 : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3), "s"(l), "s"(live), "n"(at), "v"(off), "s"(base) : "scc");
+  else
+    asm volatile(MIHVD_G16_ASM : "+v"(c0), "+v"(c1), "+v"(c2), "+v"(c3)
+                 : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3), "s"(l), "s"(live), "n"(at), "v"(off), "s"(base) : "scc");
+#undef MIHVD_G16_ASM
+}
+template <bool BIG>
+__device__ __forceinline__ void mfma4_copy2(f32x4& c0, f32x4& c1, f32x4& c2, f32x4& c3, const bf16x8& a, const bf16x8& b0,
+                                            const bf16x8& b1, const bf16x8& b2, const bf16x8& b3, uint32_t l,
+                                            uint64_t live, int at, uint32_t off, const char* base, int at2, uint32_t off2,
+                                            const char* base2) {
+#define MIHVD_G16_ASM                                                                                              \
+  "s_nop 1\n\t" MIHVD_G16_MFMA " %0, %4, %5, %0\n\ts_add_u32 m0, %9, %11\n\t" MIHVD_G16_MFMA                     \
+  " %1, %4, %6, %1\n\t" MIHVD_G16_COPY("%12", "%13") MIHVD_G16_MFMA                                         \
+  " %2, %4, %7, %2\n\ts_add_u32 m0, %9, %14\n\t" MIHVD_G16_COPY("%15", "%16") MIHVD_G16_MFMA " %3, %4, %8, %3"
+  if constexpr (BIG)
+    asm volatile(MIHVD_G16_ASM : "+a"(c0), "+a"(c1), "+a"(c2), "+a"(c3)
+                 : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3), "s"(l), "s"(live), "n"(at), "v"(off), "s"(base), "n"(at2),
+                   "v"(off2), "s"(base2) : "scc");
+  else
+    asm volatile(MIHVD_G16_ASM : "+v"(c0), "+v"(c1), "+v"(c2), "+v"(c3)
+                 : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3), "s"(l), "s"(live), "n"(at), "v"(off), "s"(base), "n"(at2),
+                   "v"(off2), "s"(base2) : "scc");
+#undef MIHVD_G16_ASM
+}
+// The matrix pipe's results may be read after this (16 wait states; the longest needed is 11).
+template <bool BIG>
+__device__ __forceinline__ void mfma_done(f32x4& c0, f32x4& c1, f32x4& c2, f32x4& c3) {
+  if constexpr (BIG) asm volatile("s_nop 15" : "+a"(c0), "+a"(c1), "+a"(c2), "+a"(c3));
+  else asm volatile("s_nop 15" : "+v"(c0), "+v"(c1), "+v"(c2), "+v"(c3));
+}
+// Keeps the accumulators of row block j where they are until an epilogue comes to them (left alone, the
+// compiler copies all of them to vector registers at once, which do not suffice).
+template <int NI, int MI>
+__device__ __forceinline__ void pin(f32x4 (&acc)[NI][MI], int j) {
+#pragma unroll
+  for (int i = 0; i < NI; i += 4) {
+    if constexpr (NI * MI > 16) asm volatile("" : "+a"(acc[i][j]), "+a"(acc[i + 1][j]), "+a"(acc[i + 2][j]), "+a"(acc[i + 3][j]));
+    else asm volatile("" : "+v"(acc[i][j]), "+v"(acc[i + 1][j]), "+v"(acc[i + 2][j]), "+v"(acc[i + 3][j]));
+  }
 }
 // Every copy of this wave has landed and its LDS reads are back; then all waves meet. Memory accesses
 // stay on their side.
 __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
+
+__device__ __forceinline__ void tile_barrier_landed() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // One side's staging of an [R x 64] (KC) or [64 x R] (KS) tile by NT threads.
 template <int LAYOUT, int R, int NT, bool DUAL>
@@ -125,10 +244,6 @@ struct Stage {
   }
   __device__ __forceinline__ static bool is_alt(int j) { return DUAL && (((j * NT) >> 3) & 64); }
 
-  // j-th load of a whole k tile
-  __device__ __forceinline__ void one(int j, const char* base, const char* alt, uint32_t lds_wave, uint32_t live) const {
-    dma16_if(is_alt(j) ? alt : base, off[j], lds_wave + j * NT * 16, live);
-  }
   __device__ __forceinline__ void all(const char* base, const char* alt, uint32_t lds_wave) const {
 #pragma unroll
     for (int j = 0; j < J; ++j) dma16(is_alt(j) ? alt : base, off[j], lds_wave + j * NT * 16);
@@ -193,33 +308,48 @@ struct Frags {
   }
 };
 
-// Tile order: the blocks that one XCD runs (every eighth) take a contiguous run of tiles, walked in
-// groups of eight m tiles, so that the 32 tiles an XCD has in flight share rows of both operands in
-// its L2.
-__device__ __forceinline__ void tile_of(const Args& a, int& batch, int& split, int& mt, int& nt) {
-  const int nb = gridDim.x, id = blockIdx.x;
-  const int q = nb >> 3, r = nb & 7, x = id & 7;
-  int pos = x * q + min(x, r) + (id >> 3);
-  const int tiles = a.sym ? a.tiles_m * (a.tiles_m + 1) / 2 : a.tiles_m * a.tiles_n;
-  batch = pos / (tiles * a.splits);
-  pos -= batch * tiles * a.splits;
-  split = pos / tiles;
-  pos -= split * tiles;
+// One output tile of one k split: where it is and its k tiles [it, end).
+struct Tile {
+  int batch, split, mt, nt, it, end;
+};
+
+// Tile order. Blocks are persistent: the blocks of one XCD (every eighth block) walk a contiguous
+// run of tiles together, in groups of eight m tiles, so that the tiles an XCD has in flight share rows
+// of both operands in its L2. `l` counts within the XCD's run; false past its end.
+__device__ __forceinline__ bool tile_at(const Args& a, int tiles_m, int kts, int l, Tile& t) {
+  const int tiles = a.sym ? tiles_m * (tiles_m + 1) / 2 : tiles_m * a.tiles_n;
+  const int nb = tiles * a.splits * a.batch, x = blockIdx.x & 7;
+  const int q = nb >> 3, r = nb & 7;
+  if (l >= q + (x < r ? 1 : 0)) return false;
+  int pos = x * q + min(x, r) + l, mt, nt, batch = 0, split = 0;
+  if (a.batch > 1 || a.splits > 1) {
+    const int e = pos / tiles;
+    pos -= e * tiles;
+    batch = e / a.splits;
+    split = e - batch * a.splits;
+  }
   if (a.sym) {
     mt = 0;
-    while (pos >= a.tiles_m - mt) {
-      pos -= a.tiles_m - mt;
+    while (pos >= tiles_m - mt) {
+      pos -= tiles_m - mt;
       ++mt;
     }
     nt = mt + pos;
-    return;
+  } else {
+    constexpr int G = 8;
+    const int g = pos / (G * a.tiles_n), first = g * G;
+    const int gs = min(G, tiles_m - first);
+    pos -= g * G * a.tiles_n;
+    nt = pos / gs;
+    mt = first + pos - nt * gs;
   }
-  constexpr int G = 8;
-  const int g = pos / (G * a.tiles_n), first = g * G;
-  const int gs = min(G, a.tiles_m - first);
-  pos -= g * G * a.tiles_n;
-  mt = first + pos % gs;
-  nt = pos / gs;
+  t.batch = uni(batch);
+  t.split = uni(split);
+  t.mt = uni(mt);
+  t.nt = uni(nt);
+  t.it = a.splits == 1 ? 0 : uni((int)((int64_t)kts * t.split / a.splits));
+  t.end = a.splits == 1 ? kts : uni((int)((int64_t)kts * (t.split + 1) / a.splits));
+  return true;
 }
 
 // k tiles are double buffered. While tile t is multiplied, tile t + 1 is on its way or has landed;
@@ -227,65 +357,87 @@ __device__ __forceinline__ void tile_of(const Args& a, int& batch, int& split, i
 // second half are in registers), so the copies of tile t + 2 go out there, between the MFMAs, and the
 // first fragments of tile t + 1 are read: one barrier a tile, a whole tile's time for the copies,
 // and no MFMA waits on an LDS read that was not issued half a tile earlier.
+//
+// The stream of k tiles runs on from one output tile to the next: while the epilogue works, the next
+// output tile's first two k tiles are already in LDS and its first fragments in registers, and the
+// epilogue's stores drain under the next products.
 template <int LM, int LN, int TM, int TN, int WM, int WN, bool DUAL, class Epi>
 __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gemm16_kernel(const Args a, const Epi epi) {
   constexpr int NT = 64 * WM * WN, WTM = TM / WM, WTN = TN / WN, MI = WTM / 16, NI = WTN / 16;
   constexpr int BUF = (TM + TN) * BK;  // elements of one buffer
-  __shared__ __attribute__((aligned(128))) u16 lds[2 * BUF];
-  int batch, split, mt, nt;
-  tile_of(a, batch, split, mt, nt);
-  batch = __builtin_amdgcn_readfirstlane(batch);  // (divisions leave uniform values in vector registers)
-  split = __builtin_amdgcn_readfirstlane(split);
-  mt = __builtin_amdgcn_readfirstlane(mt);
-  nt = __builtin_amdgcn_readfirstlane(nt);
-  const int M = __builtin_amdgcn_readfirstlane(a.dyn_m ? *a.dyn_m : a.M);
-  const int K = __builtin_amdgcn_readfirstlane(a.dyn_k ? *a.dyn_k : a.K);
-  const int x0m = mt * TM, x0n = nt * (DUAL ? TN / 2 : TN);
-  if (x0m >= M) return;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  constexpr bool BIG = TM * TN > 128 * 128;
+  constexpr int STAGE = 16 * (WTN + 8);  // a wave's RowStage
+  __shared__ __attribute__((aligned(128))) u16 lds[2 * BUF + WM * WN * STAGE];
+  const int M = uni(a.dyn_m ? *a.dyn_m : a.M);
+  const int K = uni(a.dyn_k ? *a.dyn_k : a.K);
+  const int tiles_m = a.dyn_m ? (M + TM - 1) / TM : a.tiles_m;
+  const int kt = (K + BK - 1) / BK, kts = kt * a.nseg;
+  const int hops = (int)(gridDim.x >> 3) + ((blockIdx.x & 7) < (gridDim.x & 7) ? 1 : 0);
+  int l_mul = blockIdx.x >> 3, l_cpy = l_mul;  // the tile being multiplied, the tile being copied
+  Tile cur, nxt;
+  if (!tile_at(a, tiles_m, kts, l_mul, cur)) return;
+  const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
   Stage<LM, TM, NT, false> sm;
   Stage<LN, TN, NT, DUAL> sn;
-  sm.init(a.m, x0m, t);
-  sn.init(a.n, x0n, t);
-  const int64_t tm0 = a.m.bs * batch + (LM == KC ? (int64_t)x0m * a.m.ld : x0m);
-  const int64_t tn0 = a.n.bs * batch + (LN == KC ? (int64_t)x0n * a.n.ld : x0n);
   const int64_t stepm = LM == KC ? BK : BK * a.m.ld, stepn = LN == KC ? BK : BK * a.n.ld;
 
-  // k tiles in order: the segments' last, partial tiles first (at most two: they go out ahead of the
-  // loop, which then copies whole tiles only), then the whole tiles of every segment
-  const int full = K / BK, parts = K % BK ? a.nseg : 0, total = full * a.nseg + parts;
-  const int per = (total + a.splits - 1) / a.splits;
-  const int it0 = __builtin_amdgcn_readfirstlane(split * per);
-  const int it1 = __builtin_amdgcn_readfirstlane(min(total, it0 + per));
-
-  f32x4 acc[NI][MI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i)
-#pragma unroll
-    for (int j = 0; j < MI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const char *pm = nullptr, *pn = nullptr, *pa = nullptr;  // the next tile to copy
-  int seg, kp;
-  auto locate = [&](int it) {
-    seg = __builtin_amdgcn_readfirstlane(it < parts ? it : full > 0 ? (it - parts) / full : 0);
-    kp = it < parts ? full : it - parts - seg * full;
+  // The next k tile to copy: `run` whole ones lie ahead at (pm, pn), one step apart; then, with run == 0,
+  // what `next_run` finds: a partial tile (krem > 0 of its k positions, none for a split without any k),
+  // the next segment, the next output tile, or the end.
+  const char *pm = nullptr, *pn = nullptr, *pa = nullptr;
+  int run = 0, seg = 0, krem = 0;
+  bool partial = false, more = true;
+  auto locate = [&](int kp) {
+    const int x0m = nxt.mt * TM, x0n = nxt.nt * (DUAL ? TN / 2 : TN);
+    const int64_t tm0 = a.m.bs * nxt.batch + (LM == KC ? (int64_t)x0m * a.m.ld : x0m);
+    const int64_t tn0 = a.n.bs * nxt.batch + (LN == KC ? (int64_t)x0n * a.n.ld : x0n);
     const u16* bm = seg == 0 ? a.m.p[0] : seg == 1 ? a.m.p[1] : a.m.p[2];
     const u16* bn = seg == 0 ? a.n.p[0] : seg == 1 ? a.n.p[1] : a.n.p[2];
     pm = (const char*)(bm + tm0 + kp * stepm);
     pn = (const char*)(bn + tn0 + kp * stepn);
     if (DUAL) pa = (const char*)(a.n.alt + tn0 + kp * stepn);
+    const int whole = K / BK - kp;  // whole tiles of this segment from here on
+    run = min(whole, nxt.end - nxt.it);
+    partial = run == 0;
+    krem = nxt.it < nxt.end ? K - kp * BK : 0;
+    nxt.it += max(run, 1);
+  };
+  auto enter = [&]() {  // the copies reach output tile nxt
+    sm.init(a.m, nxt.mt * TM, t);
+    sn.init(a.n, nxt.nt * (DUAL ? TN / 2 : TN), t);
+    seg = a.nseg == 1 ? 0 : uni(kt > 0 ? nxt.it / kt : 0);
+    locate(nxt.it - seg * kt);
+  };
+  auto next_run = [&]() {
+    if (!more) return;
+    if (nxt.it < nxt.end) {
+      const int kp = nxt.it - seg * kt;
+      if (kp == kt) ++seg;
+      locate(kp == kt ? 0 : kp);
+    } else {
+      l_cpy += hops;
+      more = tile_at(a, tiles_m, kts, l_cpy, nxt);
+      if (more) enter();
+    }
   };
   const uint32_t ldsb = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u16*)lds;
   const uint32_t lds0 = ldsb + (uint32_t)wave * 1024u;
+  // the next k tile as a whole, ahead of the loop or where the run ends
   auto issue = [&](uint32_t l) {
-    if (kp < full) {
+    if (run == 0 && !partial) next_run();
+    if (run > 0) {
       sm.all(pm, nullptr, l);
       sn.all(pn, pa, l + TM * BK * 2);
-    } else {
-      sm.tail(pm, nullptr, l, t, K - full * BK);
-      sn.tail(pn, pa, l + TM * BK * 2, t, K - full * BK);
+      pm += stepm * 2;
+      pn += stepn * 2;
+      if (DUAL) pa += stepn * 2;
+      --run;
+    } else if (partial) {
+      sm.tail(pm, nullptr, l, t, krem);
+      sn.tail(pn, pa, l + TM * BK * 2, t, krem);
+      partial = false;
     }
   };
   Frags<LM, TM, MI, false> gm;
@@ -293,76 +445,123 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
   gm.init(ldsb, wm, lane);
   gn.init(ldsb + TM * BK * 2, wn, lane);
 
-  if (it0 < it1) {
-    constexpr int NF = MI + NI, NQ = sm.J + sn.J, NX = NI * MI;
-    bf16x8 fm[2][MI], fn[2][NI];
-    locate(it0);
-    issue(lds0);
-    if (it0 + 1 < it1) {
-      locate(it0 + 1);
-      tile_barrier();
-      issue(lds0 + BUF * 2);
-    } else {
-      tile_barrier();
-    }
+  f32x4 acc[NI][MI];
+  auto clear = [&]() {
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
-      else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
-    }
-    locate(it0 + 2);
-    uint32_t lq = lds0, hop = BUF * 2;  // where the next copies go; to the other buffer
-    for (int it = it0; it < it1; ++it) {
-      const uint32_t live = (uint32_t)__builtin_amdgcn_readfirstlane(it + 2 < it1 ? -1 : 0);
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
+      for (int j = 0; j < MI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  clear();
+
+  constexpr int NF = MI + NI, NQ = sm.J + sn.J, NX = NI * MI;
+  // fragments read before MFMA x of a half tile: all within its first three quarters, so that none is
+  // waited for at the barrier
+  auto ahead = [](int x) constexpr { return x * NF * 4 / (3 * NX) < NF ? x * NF * 4 / (3 * NX) : NF; };
+  bf16x8 fm[2][MI], fn[2][NI];
+  nxt = cur;
+  enter();
+  issue(lds0);
+  tile_barrier();
+  issue(lds0 + BUF * 2);
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
+    else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
+  }
+  uint32_t lq = lds0, hop = BUF * 2;  // where the next copies go; to the other buffer
+  bool landed = false;                // the copies in flight were waited for ahead of an epilogue
+
+  auto first_half = [&]() {
+#pragma unroll
+    for (int x = 0; x < NX; x += 4) {
+#pragma unroll
+      for (int f = ahead(x); f < ahead(x + 4); ++f) {
         if (f < MI) fm[1][f < MI ? f : 0] = gm.get(f, 1);
         else fn[1][f < MI ? 0 : f - MI] = gn.get(f - MI, 1);
-#pragma unroll
-        for (int x = f * NX / NF; x < (f + 1) * NX / NF; ++x)
-          acc[x / MI][x % MI] = mfma16(fn[0][x / MI], fm[0][x % MI], acc[x / MI][x % MI]);
       }
-      tile_barrier();
-      gm.move(hop);
-      gn.move(hop);
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-#pragma unroll
-        for (int q = f * NQ / NF; q < (f + 1) * NQ / NF; ++q) {
-          if (q < sm.J) sm.one(q < sm.J ? q : 0, pm, nullptr, lq, live);
-          else sn.one(q < sm.J ? 0 : q - sm.J, pn, pa, lq + TM * BK * 2, live);
-        }
-        // (of the last tile: not used)
-        if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
-        else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
-#pragma unroll
-        for (int x = f * NX / NF; x < (f + 1) * NX / NF; ++x)
-          acc[x / MI][x % MI] = mfma16(fn[1][x / MI], fm[1][x % MI], acc[x / MI][x % MI]);
-      }
-      lq += hop;
-      hop = 0u - hop;
-      if (++kp == full) {
-        locate(it + 3);
-      } else {
-        pm += stepm * 2;
-        pn += stepn * 2;
-        if (DUAL) pa += stepn * 2;
+      const int i = x / MI, j = x % MI;
+      mfma4<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[0][i], fm[0][j], fm[0][j + 1], fm[0][j + 2],
+                 fm[0][j + 3]);
+      if (x + 8 == NX) {
+        gm.move(hop);
+        gn.move(hop);
       }
     }
+  };
+  // the next k tile's copies between the MFMAs
+  auto second_half = [&](uint64_t live) {
+    unroll<NX / 4>([&](auto B) {
+      constexpr int x = B.value * 4, i = x / MI, j = x % MI;
+      // the next tile's first fragments (after the last tile: not used)
+#pragma unroll
+      for (int f = ahead(x); f < ahead(x + 4); ++f) {
+        if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
+        else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
+      }
+      constexpr int PER = NQ * 4 / NX;  // copies among four MFMAs
+      static_assert(PER == 1 || PER == 2, "copies per four MFMAs");
+      constexpr int JM = decltype(sm)::J, q = x * NQ / NX, q2 = q + PER - 1;
+      constexpr int at1 = q < JM ? q * NT * 16 : TM * BK * 2 + (q - JM) * NT * 16;
+      constexpr int at2 = q2 < JM ? q2 * NT * 16 : TM * BK * 2 + (q2 - JM) * NT * 16;
+      const uint32_t o1 = q < JM ? sm.off[q < JM ? q : 0] : sn.off[q < JM ? 0 : q - JM];
+      const uint32_t o2 = q2 < JM ? sm.off[q2 < JM ? q2 : 0] : sn.off[q2 < JM ? 0 : q2 - JM];
+      const char* b1 = q < JM ? pm : sn.is_alt(q < JM ? 0 : q - JM) ? pa : pn;
+      const char* b2 = q2 < JM ? pm : sn.is_alt(q2 < JM ? 0 : q2 - JM) ? pa : pn;
+      if constexpr (PER == 1)
+        mfma4_copy<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
+                        fm[1][j + 2], fm[1][j + 3], lq, live, at1, o1, b1);
+      else
+        mfma4_copy2<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
+                         fm[1][j + 2], fm[1][j + 3], lq, live, at1, o1, b1, at2, o2, b2);
+    });
+    lq += hop;
+    hop = 0u - hop;
+  };
+  for (;;) {
+    for (int n = max(1, cur.end - cur.it); n > 0; --n) {
+      first_half();
+      if (__builtin_expect(landed, 0)) tile_barrier_landed();
+      else tile_barrier();
+      landed = false;
+      const int go = run > 0 ? -1 : 0;
+      if (__builtin_expect(!go, 0)) issue(lq);  // a run's end: this k tile in one go, or nothing
+      uint64_t live;  // all lanes or none, in scalar registers
+      asm volatile("v_cmp_ne_u32 %0, 0, %1" : "=s"(live) : "v"(go));
+      second_half(live);
+      run += go;
+      pm += (stepm * 2) & (int64_t)go;
+      pn += (stepn * 2) & (int64_t)go;
+      if (DUAL) pa += (stepn * 2) & (int64_t)go;
+    }
+    Ctx c;
+    c.m0 = cur.mt * TM + wm * WTM;
+    c.n0 = cur.nt * (DUAL ? TN / 2 : TN) + wn * (DUAL ? WTN / 2 : WTN);
+    c.M = M;
+    c.N = a.N;
+    c.mt = cur.mt;
+    c.nt = cur.nt;
+    c.wm = wm;
+    c.wn = wn;
+    c.batch = cur.batch;
+    c.split = cur.split;
+    c.lane = lane;
+    c.stage = lds + 2 * BUF + wave * STAGE;
+    typename Epi::template Pre<NI, MI> pre;
+    epi.load(c, pre);
+    // the copies in flight land before the epilogue stores anything, so that the next barrier need
+    // not wait for those stores
+    copies_landed();
+    landed = true;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MI; j += 4) mfma_done<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+    epi.template run<NI, MI>(c, pre, acc);
+    l_mul += hops;
+    if (!tile_at(a, tiles_m, kts, l_mul, cur)) break;
+    clear();
   }
-  Ctx c;
-  c.m0 = x0m + wm * WTM;
-  c.n0 = x0n + wn * (DUAL ? WTN / 2 : WTN);
-  c.M = M;
-  c.N = a.N;
-  c.mt = mt;
-  c.nt = nt;
-  c.wm = wm;
-  c.wn = wn;
-  c.batch = batch;
-  c.split = split;
-  c.lane = lane;
-  epi.template run<NI, MI>(c, acc);
 }
 
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -376,7 +575,8 @@ void launch_tile(Args a, const Epi& e, hipStream_t stream) {
   a.tiles_m = cdiv(a.M, TM);
   a.tiles_n = cdiv(a.N, DUAL ? TN / 2 : TN);
   const int64_t tiles = a.sym ? (int64_t)a.tiles_m * (a.tiles_m + 1) / 2 : (int64_t)a.tiles_m * a.tiles_n;
-  const int64_t blocks = tiles * a.splits * a.batch;
+  const int64_t slots = (int64_t)device_cu_count() * (TM * TN > 128 * 128 ? 1 : 2);  // resident blocks
+  const int64_t blocks = std::min<int64_t>(tiles * a.splits * a.batch, slots);
   if (blocks <= 0) return;
   gemm16_kernel<LM, LN, TM, TN, WM, WN, DUAL, Epi><<<dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream>>>(a, e);
 }
@@ -416,7 +616,11 @@ inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym,
   return best;
 }
 
-// ---- epilogue helpers ---------------------------------------------------------------------- //
+// ---- epilogues -----------------------------------------------------------------------------
+// An epilogue is a struct with `load` (what it reads from memory early, into a Pre: on its way while
+// the tile's copies land) and `run` (its work on the accumulators: acc[i][j][k] is column
+// n0 + 16 i + 4 (lane >> 4) + k of row m0 + 16 j + (lane & 15)).
+// ---- helpers ---------------------------------------------------------------------- //
 // Store four consecutive values of a row: one 8-byte store when `vec` (row starts 8-byte aligned).
 __device__ __forceinline__ void store4(u16* row, int n, int N, bool vec, float a, float b, float c, float d) {
   if (vec && n + 3 < N) {
@@ -429,6 +633,18 @@ __device__ __forceinline__ void store4(u16* row, int n, int N, bool vec, float a
   if (n + 3 < N) row[n + 3] = f2bf(d);
 }
 
+// Eight consecutive values of a row: one 16-byte store when `vec` (rows start 16-byte aligned).
+__device__ __forceinline__ void store8(u16* row, int n, int N, bool vec, uint4 v) {
+  if (vec && n + 7 < N) {
+    *reinterpret_cast<uint4*>(row + n) = v;
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (n + k < N) row[n + k] = (u16)(w[k >> 1] >> (16 * (k & 1)));
+}
+
 // out[batch][m][n] = alpha * acc, rounded once to the 16-bit format; alpha times an optional device
 // scalar. `out[]` holds one base per batch entry.
 struct EpiStore {
@@ -437,20 +653,29 @@ struct EpiStore {
   float alpha;
   const float* dev_alpha;
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const Ctx& c, f32x4 (&acc)[NI][MI]) const {
+  struct Pre {};
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const Ctx&, Pre<NI, MI>&) const {}
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
     const float al = dev_alpha ? alpha * *dev_alpha : alpha;
     u16* o = c.batch == 0 ? out[0] : out[1];
-    const bool vec = (ld & 3) == 0;
+    const bool vec = (ld & 7) == 0;
+    const RowStage<NI * 16> st{c.stage, c.lane};
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
-      const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= c.M) continue;
-      u16* row = o + (int64_t)m * ld;
+      pin(acc, j);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        store4(row, n, c.N, vec, acc[i][j][0] * al, acc[i][j][1] * al, acc[i][j][2] * al, acc[i][j][3] * al);
+      for (int i = 0; i < NI; ++i)
+        st.put(i, pack4bf(acc[i][j][0] * al, acc[i][j][1] * al, acc[i][j][2] * al, acc[i][j][3] * al));
+      st.turn();
+#pragma unroll
+      for (int g = 0; g < st.GETS; ++g) {
+        const int m = c.m0 + j * 16 + st.row(g);
+        const uint4 v = st.get(g);
+        if (m < c.M) store8(o + (int64_t)m * ld, c.n0 + st.col(), c.N, vec, v);
       }
+      st.turn();
     }
   }
 };
@@ -461,11 +686,16 @@ struct EpiSlab {
   int64_t ld, stride;
   int splits, add;
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const Ctx& c, f32x4 (&acc)[NI][MI]) const {
+  struct Pre {};
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const Ctx&, Pre<NI, MI>&) const {}
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
     float* o = slab + (int64_t)(c.batch * splits + c.split) * stride;
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
       const int m = c.m0 + j * 16 + (c.lane & 15);
+      pin(acc, j);
       if (m >= c.M) continue;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {

@@ -46,11 +46,55 @@ __global__ void __launch_bounds__(256) lce_gather(const u16* __restrict__ h, int
   }
 }
 
-__device__ __forceinline__ float bias_at(const void* b, int kind, int n) {
-  return kind == 0 ? 0.f : kind == 1 ? static_cast<const float*>(b)[n] : bf2f(static_cast<const u16*>(b)[n]);
+// A lane's bias values, as its accumulators hold the columns.
+template <bool BIAS, int NI>
+struct BiasRegs {
+  float v[BIAS ? NI : 1][4];
+  __device__ __forceinline__ void load(const void* b, int kind, int n0, int N, int lane) {
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = min(n0 + i * 16 + 4 * (lane >> 4) + k, N - 1);
+          v[i][k] = kind == 1 ? static_cast<const float*>(b)[n] : bf2f(static_cast<const u16*>(b)[n]);
+        }
+    }
+  }
+  __device__ __forceinline__ float add(float z, int i, int k) const {
+    if constexpr (BIAS) return z + v[i][k];
+    else return z;
+  }
+};
+
+// logits in place; columns past N (only a tile that ends inside has them) become -inf
+template <bool BIAS, int NI, int MI>
+__device__ __forceinline__ void logits(const g16::Ctx& c, const BiasRegs<BIAS, NI>& b, f32x4 (&acc)[NI][MI], int j,
+                                       f32x4 (&z)[NI]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z[i][k] = b.add(acc[i][j][k], i, k);
+  if (c.n0 + NI * 16 > c.N) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c.n0 + i * 16 + 4 * (c.lane >> 4) + k >= c.N) z[i][k] = -INFINITY;
+  }
 }
 
-// Statistics of one wave's columns: part[row][2 * pieces] = (max, sum of exp(z - max)).
+// Does column `lab` lie among the lane's? Then (lab - first) >> 4 and & 3 are its i and k.
+template <int NI>
+__device__ __forceinline__ bool mine(const g16::Ctx& c, int lab, int& d) {
+  d = lab - (c.n0 + 4 * (c.lane >> 4));
+  return d >= 0 && d < NI * 16 && (d & 15) < 4;
+}
+
+// Statistics of one wave's columns: part[row][piece] = (max, sum of exp(z - max)), and the label's logit.
+// About nine vector instructions a logit, the exponential four of their time: with one wave a SIMD
+// that is a third of the products' time at K = 768.
+template <bool BIAS>
 struct EpiStats {
   const void* bias;
   int bias_kind;
@@ -59,47 +103,51 @@ struct EpiStats {
   int npart;
   float* zlab;        // [rows]
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
-    const int g4 = 4 * (c.lane >> 4);
-    if (bias_kind) {
+  struct Pre {
+    BiasRegs<BIAS, NI> b;
+    int lab[MI];
+  };
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const g16::Ctx& c, Pre<NI, MI>& p) const {
+    p.b.load(bias, bias_kind, c.n0, c.N, c.lane);
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float b = bias_at(bias, bias_kind, min(c.n0 + i * 16 + g4 + k, c.N - 1));
-#pragma unroll
-          for (int j = 0; j < MI; ++j) acc[i][j][k] += b;
-        }
-    }
+    for (int j = 0; j < MI; ++j) p.lab[j] = label[min(c.m0 + j * 16 + (c.lane & 15), c.M - 1)];
+  }
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>& p, f32x4 (&acc)[NI][MI]) const {
     const int slot = c.nt * 2 + c.wn;  // two waves along a tile's columns
-#pragma unroll
-    for (int j = 0; j < MI; ++j) {
+    g16::unroll<MI>([&](auto J) {
+      constexpr int j = J.value;
+      g16::pin(acc, j);
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      const int lab = m < c.M ? label[m] : -1;
-      float mx = -INFINITY;
+      f32x4 z[NI];
+      logits(c, p.b, acc, j, z);
+      int d;
+      if (mine<NI>(c, p.lab[j], d) && m < c.M) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (d == i * 16 + k) zlab[m] = z[i][k];
+      }
+      float mx = z[0][0];
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = c.n0 + i * 16 + g4 + k;
-          if (n < c.N) mx = fmaxf(mx, acc[i][j][k]);
-          if (n == lab) zlab[m] = acc[i][j][k];
-        }
+        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, z[i][k]);
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float ref = mx == -INFINITY ? 0.f : mx;  // a row of -inf adds nothing, without inf - inf
-      float s = 0.f;
+      f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = c.n0 + i * 16 + g4 + k;
-          if (n < c.N) s += __expf(acc[i][j][k] - ref);
-        }
+        for (int k = 0; k < 4; ++k) s4[k] += __expf(z[i][k] - ref);
+      float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
       if (c.lane < 16 && m < c.M) part[(int64_t)m * npart + slot] = make_float2(mx, s);
-    }
+    });
   }
 };
 
@@ -156,55 +204,93 @@ __global__ void __launch_bounds__(1024) lce_reduce(const float* __restrict__ row
   }
 }
 
-// dz of one piece of the vocabulary, and its sums over the wave's rows (the bias gradient's terms).
+// dz of one piece of the vocabulary (its columns start at v0), times DZ_SCALE, and with BIAS its sums over
+// the wave's rows (the bias gradient's terms). ROWS: rows have weights of their own. The scale is
+// folded into the exponent; the label's column is put right afterwards, by the one lane that has it.
+template <bool BIAS, bool ROWS>
 struct EpiDz {
-  const void* bias;
+  const void* bias;  // from v0 on
   int bias_kind;
   const int* label;
   const float* lse;
-  const float* rowscale;  // g_r / G per compact row, or null (1)
-  int v0;                 // first vocabulary entry of the piece
+  const float* rowscale;  // g_r / G per compact row
+  int v0;
   u16* dz;                // [rows][ld]
   int64_t ld;
-  float* dbp;             // [m waves][ld] or null
-  int wm_per_tile;
+  float* dbp;             // [m waves][ld]
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
-    const int g4 = 4 * (c.lane >> 4);
-    f32x4 sum[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Pre {
+    BiasRegs<BIAS, NI> b;
+    int lab[MI];
+    float ls[MI], rs[ROWS ? MI : 1];
+  };
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const g16::Ctx& c, Pre<NI, MI>& p) const {
+    p.b.load(bias, bias_kind, c.n0, c.N, c.lane);
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
+      const int m = min(c.m0 + j * 16 + (c.lane & 15), c.M - 1);
+      p.lab[j] = label[m];
+      p.ls[j] = lse[m];
+      if constexpr (ROWS) p.rs[j] = rowscale[m];
+    }
+  }
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>& p, f32x4 (&acc)[NI][MI]) const {
+    f32x4 sum[BIAS ? NI : 1];
+#pragma unroll
+    for (int i = 0; i < (BIAS ? NI : 1); ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const g16::RowStage<NI * 16> st{c.stage, c.lane};
+    g16::unroll<MI>([&](auto J) {
+      constexpr int j = J.value;
+      g16::pin(acc, j);
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      const bool on = m < c.M;
-      const int mm = min(m, c.M - 1);
-      const float ls = lse[mm], rs = rowscale ? rowscale[mm] : 1.f;
-      const int lab = label[mm] - v0;
+      const float ls = DZ_SCALE == 1.f ? p.ls[j] : p.ls[j] - __logf(DZ_SCALE);
+      f32x4 z[NI];
+      logits(c, p.b, acc, j, z);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[i][k] = __expf(z[i][k] - ls);
+      int d;
+      if (mine<NI>(c, p.lab[j] - v0, d)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (d == i * 16 + k && c.n0 + i * 16 + 4 * (c.lane >> 4) + k < c.N) z[i][k] -= DZ_SCALE;
+      }
+      if constexpr (ROWS) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) z[i] *= p.rs[j];
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int n = c.n0 + i * 16 + g4;
-        float d[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float z = acc[i][j][k] + bias_at(bias, bias_kind, min(v0 + n + k, v0 + c.N - 1));
-          const float p = __expf(z - ls) - (n + k == lab ? 1.f : 0.f);
-          d[k] = n + k < c.N ? p * rs : 0.f;
-          if (on) sum[i][k] += d[k];
+        if constexpr (BIAS) {
+          if (m < c.M) sum[i] += z[i];
         }
-        if (on && n < ld)  // columns N..ld are the zeros that the next products read
-          *reinterpret_cast<uint2*>(dz + (int64_t)m * ld + n) =
-              pack4bf(d[0] * DZ_SCALE, d[1] * DZ_SCALE, d[2] * DZ_SCALE, d[3] * DZ_SCALE);
+        st.put(i, pack4bf(z[i][0], z[i][1], z[i][2], z[i][3]));
       }
-    }
-    if (!dbp) return;
-    float* o = dbp + (int64_t)(c.mt * wm_per_tile + c.wm) * ld;
+      st.turn();
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int n = c.n0 + i * 16 + g4;
+      for (int g = 0; g < st.GETS; ++g) {
+        const int r = c.m0 + j * 16 + st.row(g), n = c.n0 + st.col();
+        const uint4 v = st.get(g);
+        if (r < c.M && n < ld)  // columns N..ld are the zeros that the next products read
+          *reinterpret_cast<uint4*>(dz + (int64_t)r * ld + n) = v;
+      }
+      st.turn();
+    });
+    if constexpr (BIAS) {
+      float* o = dbp + (int64_t)(c.mt * 2 + c.wm) * ld;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[i][k] = row_sum16(sum[i][k]);
-      if ((c.lane & 15) == 0 && n < ld) *reinterpret_cast<f32x4*>(o + n) = sum[i];
+      for (int i = 0; i < NI; ++i) {
+        const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
+        f32x4 t = sum[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = row_sum16(t[k]);
+        if ((c.lane & 15) == 0 && n < ld) *reinterpret_cast<f32x4*>(o + n) = t;
+      }
     }
   }
 };
@@ -217,7 +303,7 @@ __global__ void __launch_bounds__(256) lce_db(const float* __restrict__ dbp, int
   const int n = (*cnt + tm - 1) / tm * wm_per_tile;
   float s = 0.f;
   for (int i = 0; i < n; ++i) s += dbp[(int64_t)i * ld + v];
-  s *= *gs;
+  s *= *gs * (1.f / DZ_SCALE);
   if (kind == 1) static_cast<float*>(db)[v] = s;
   else static_cast<u16*>(db)[v] = f2bf(s);
 }
@@ -271,8 +357,8 @@ void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t 
   a.N = s.V;
   a.K = s.K;
   a.dyn_m = rw.cnt;
-  EpiStats e{bias, bias_kind, rw.label, part, s.npart, zlab};
-  g16::launch<g16::KC, g16::KC>(s.tile, a, e, st);
+  if (bias) g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<true>{bias, bias_kind, rw.label, part, s.npart, zlab}, st);
+  else g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<false>{nullptr, 0, rw.label, part, s.npart, zlab}, st);
   lce_finish<<<g16::cdiv(s.N, 16), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
   if (loss) lce_reduce<<<1, 1024, 0, st>>>(rows, s.N, rw.cnt, mean, loss);
 }
@@ -295,8 +381,15 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       a.N = nv;
       a.K = s.K;
       a.dyn_m = rw.cnt;
-      EpiDz e{bias, bias_kind, rw.label, lse, g.rowscale, v0, x.dz, x.ldz, db ? x.dbp : nullptr, 2};
-      g16::launch<g16::KC, g16::KC>(s.tile, a, e, st);
+      const void* b = bias ? static_cast<const char*>(bias) + (int64_t)v0 * (bias_kind == 1 ? 4 : 2) : nullptr;
+      auto go = [&](auto B, auto R) {
+        EpiDz<B.value, R.value> e{b, bias_kind, rw.label, lse, g.rowscale, v0, x.dz, x.ldz, x.dbp};
+        g16::launch<g16::KC, g16::KC>(s.tile, a, e, st);
+      };
+      if (bias && g.rowscale) go(std::true_type{}, std::true_type{});
+      else if (bias) go(std::true_type{}, std::false_type{});
+      else if (g.rowscale) go(std::false_type{}, std::true_type{});
+      else go(std::false_type{}, std::false_type{});
     }
     if (db) {
       const int esz = bias_kind == 1 ? 4 : 2;

@@ -92,96 +92,168 @@ __global__ void __launch_bounds__(256) ns_scale(const NsTable t, int rows, int c
   }
 }
 
-// out planes [batch][planes][rows][ld] = alpha * acc + beta * in; symmetric: mirrored as well.
+// out planes [batch][planes][rows][ld] = alpha * acc + beta * in (planes of the same layout); symmetric
+// ones off the diagonal are stored a second time with rows and columns exchanged. N is a multiple of 64.
+template <bool IN>
 struct EpiPlanes {
   u16* out;
-  const u16* in;  // planes of the same layout, or null
+  const u16* in;
   int64_t ld, plane;
   int planes, sym;
   float alpha, beta;
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+  struct Pre {};
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
     u16* o = out + (int64_t)c.batch * planes * plane;
-    const u16* q = in ? in + (int64_t)c.batch * planes * plane : nullptr;
+    const u16* q = IN ? in + (int64_t)c.batch * planes * plane : nullptr;
+    const g16::RowStage<NI * 16> st{c.stage, c.lane};
+    constexpr int G = st.GETS;
+    uint4 iq[2][G];
+    auto fetch = [&](int j) {
 #pragma unroll
-    for (int j = 0; j < MI; ++j) {
-      const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= c.M) continue;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        if (n >= c.N) continue;  // N is a multiple of 64
-        const int64_t at = (int64_t)m * ld + n;
-        float v[4] = {alpha * acc[i][j][0], alpha * acc[i][j][1], alpha * acc[i][j][2], alpha * acc[i][j][3]};
-        if (q) {
-          for (int p = 0; p < planes; ++p) {
-            const uint2 w = *reinterpret_cast<const uint2*>(q + p * plane + at);
-            v[0] = fmaf(beta, bf2f((u16)w.x), v[0]);
-            v[1] = fmaf(beta, bf2f((u16)(w.x >> 16)), v[1]);
-            v[2] = fmaf(beta, bf2f((u16)w.y), v[2]);
-            v[3] = fmaf(beta, bf2f((u16)(w.y >> 16)), v[3]);
-          }
-        }
-        const uint2 hi = pack4bf(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<uint2*>(o + at) = hi;
-        const float lo[4] = {v[0] - bf2f((u16)hi.x), v[1] - bf2f((u16)(hi.x >> 16)), v[2] - bf2f((u16)hi.y),
-                             v[3] - bf2f((u16)(hi.y >> 16))};
-        uint2 lw = make_uint2(0, 0);
-        if (planes == 2) {
-          lw = pack4bf(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<uint2*>(o + plane + at) = lw;
-        }
-        if (sym && c.nt != c.mt) {
-          const u16 h4[4] = {(u16)hi.x, (u16)(hi.x >> 16), (u16)hi.y, (u16)(hi.y >> 16)};
-          const u16 l4[4] = {(u16)lw.x, (u16)(lw.x >> 16), (u16)lw.y, (u16)(lw.y >> 16)};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            o[(int64_t)(n + k) * ld + m] = h4[k];
-            if (planes == 2) o[plane + (int64_t)(n + k) * ld + m] = l4[k];
-          }
-        }
+      for (int r = 0; r < G; ++r) {
+        const int64_t at = (int64_t)min(c.m0 + j * 16 + st.row(r), c.M - 1) * ld + min(c.n0 + st.col(), c.N - 8);
+        iq[0][r] = *reinterpret_cast<const uint4*>(q + at);
+        if (planes == 2) iq[1][r] = *reinterpret_cast<const uint4*>(q + plane + at);
       }
-    }
+    };
+    if constexpr (IN) fetch(0);
+    g16::unroll<MI>([&](auto J) {
+      constexpr int j = J.value;
+      g16::pin(acc, j);
+      auto write = [&](u16* p) {
+        st.turn();
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          const int m = c.m0 + j * 16 + st.row(r), n = c.n0 + st.col();
+          const uint4 v = st.get(r);
+          if (m < c.M && n < c.N) *reinterpret_cast<uint4*>(p + (int64_t)m * ld + n) = v;
+        }
+        st.turn();
+      };
+#pragma unroll
+      for (int i = 0; i < NI; ++i) acc[i][j] *= alpha;
+      if constexpr (IN) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          if (p == 1 && planes == 1) break;
+#pragma unroll
+          for (int r = 0; r < G; ++r) st.set(r, iq[p][r]);
+          st.turn();
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const uint2 w = st.take(i);
+            acc[i][j][0] = fmaf(beta, bf2f((u16)w.x), acc[i][j][0]);
+            acc[i][j][1] = fmaf(beta, bf2f((u16)(w.x >> 16)), acc[i][j][1]);
+            acc[i][j][2] = fmaf(beta, bf2f((u16)w.y), acc[i][j][2]);
+            acc[i][j][3] = fmaf(beta, bf2f((u16)(w.y >> 16)), acc[i][j][3]);
+          }
+          st.turn();
+        }
+        if (j + 1 < MI) fetch(j + 1);
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) st.put(i, pack4bf(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]));
+      write(o);
+      if (planes == 2) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) st.put(i, pack4bf(rest(acc[i][j][0]), rest(acc[i][j][1]), rest(acc[i][j][2]), rest(acc[i][j][3])));
+        write(o + plane);
+      }
+      if constexpr (NI * MI > 16) g16::pin(acc, j);  // (kept for the mirror image)
+    });
+    if (!sym || c.nt == c.mt) return;
+    // the mirror image, by blocks of 16 of its rows (this tile's columns)
+    constexpr int RS = MI * 16 + 8, CH = MI * 2, GT = 16 * CH / 64;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        if (p == 1 && planes == 1) break;
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            c.stage[(4 * (c.lane >> 4) + k) * RS + j * 16 + (c.lane & 15)] = f2bf(p ? rest(acc[i][j][k]) : acc[i][j][k]);
+        st.turn();
+#pragma unroll
+        for (int r = 0; r < GT; ++r) {
+          const int row = c.lane / CH + r * (64 / CH), col = (c.lane % CH) * 8;
+          const int n = c.n0 + i * 16 + row, m = c.m0 + col;
+          const uint4 v = *reinterpret_cast<const uint4*>(c.stage + row * RS + col);
+          if (n < c.N && m < c.M) *reinterpret_cast<uint4*>(o + p * plane + (int64_t)n * ld + m) = v;
+        }
+        st.turn();
+      }
   }
+  __device__ __forceinline__ static float rest(float v) { return v - bf2f(f2bf(v)); }
 };
 
-// the last step: v = alpha * acc + beta * X, unscaled, into the result or the weight
+// The last step: v = alpha * acc + beta * X, unscaled, into the result (KIND 0 fp32, 1 bf16, 2 fp16) or the
+// weight (3: w = w * decay - step * v).
+template <int KIND>
 struct EpiFinal {
   NsOut out;
   const u16* in;
   int64_t ld, plane;
-  int planes, rows, cols, kind, muon;
+  int planes, rows, cols;
   float alpha, beta, decay, step;
   template <int NI, int MI>
-  __device__ __forceinline__ void run(const g16::Ctx& c, f32x4 (&acc)[NI][MI]) const {
+  struct Pre {};
+  template <int NI, int MI>
+  __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
+  template <int NI, int MI>
+  __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
     const u16* q = in + (int64_t)c.batch * planes * plane;
     void* o = out.dst[c.batch];
-#pragma unroll
-    for (int j = 0; j < MI; ++j) {
+    const bool vec = cols % 4 == 0;
+    g16::unroll<MI>([&](auto J) {
+      constexpr int j = J.value;
+      g16::pin(acc, j);
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= rows) continue;
+      if (m >= rows) return;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
+        if (n >= cols) continue;
+        const uint2 h = *reinterpret_cast<const uint2*>(q + (int64_t)m * ld + n);
+        uint2 l = make_uint2(0, 0);
+        if (planes == 2) l = *reinterpret_cast<const uint2*>(q + plane + (int64_t)m * ld + n);
+        const float x[4] = {bf2f((u16)h.x) + bf2f((u16)l.x), bf2f((u16)(h.x >> 16)) + bf2f((u16)(l.x >> 16)),
+                            bf2f((u16)h.y) + bf2f((u16)l.y), bf2f((u16)(h.y >> 16)) + bf2f((u16)(l.y >> 16))};
+        f32x4 v;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (n + k >= cols) continue;
-          float v = alpha * acc[i][j][k];
-          for (int p = 0; p < planes; ++p) v = fmaf(beta, bf2f(q[p * plane + (int64_t)m * ld + n + k]), v);
-          const int64_t at = (int64_t)m * cols + n + k;
-          if (muon) {
-            float* w = static_cast<float*>(o) + at;
-            *w = fmaf(-step, v, *w * decay);
-          } else if (kind == 0) {
-            static_cast<float*>(o)[at] = v;
-          } else if (kind == 1) {
-            static_cast<u16*>(o)[at] = __builtin_bit_cast(u16, (__bf16)v);
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(beta, x[k], alpha * acc[i][j][k]);
+        const int64_t at = (int64_t)m * cols + n;
+        if constexpr (KIND == 0 || KIND == 3) {
+          float* w = static_cast<float*>(o) + at;
+          if (vec && ((uintptr_t)o & 15) == 0) {
+            f32x4 r = v;
+            if constexpr (KIND == 3) r = *reinterpret_cast<f32x4*>(w) * decay - v * step;
+            *reinterpret_cast<f32x4*>(w) = r;
           } else {
-            static_cast<u16*>(o)[at] = f2bf(v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n + k < cols) w[k] = KIND == 3 ? fmaf(-step, v[k], w[k] * decay) : v[k];
+          }
+        } else {
+          u16* w = static_cast<u16*>(o) + at;
+          u16 r[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[k] = KIND == 1 ? __builtin_bit_cast(u16, (__bf16)v[k]) : f2bf(v[k]);
+          if (vec && ((uintptr_t)o & 7) == 0) {
+            *reinterpret_cast<uint2*>(w) = make_uint2((uint32_t)r[0] | ((uint32_t)r[1] << 16), (uint32_t)r[2] | ((uint32_t)r[3] << 16));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n + k < cols) w[k] = r[k];
           }
         }
       }
-    }
+    });
   }
 };
 
@@ -263,7 +335,7 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     const Side xk2 = plane_side(x, g.cp, g.rp, px, g.planes, true);
     const Side xs = plane_side(x, g.cp, g.cp, px, g.planes, false);       // columns of X
     const Side xs2 = plane_side(x, g.cp, g.cp, px, g.planes, true);
-    const EpiPlanes gram{sc.gram, nullptr, g.sp, pa, g.planes, 1, INV_S, 0.f};
+    const EpiPlanes<false> gram{sc.gram, nullptr, g.sp, pa, g.planes, 1, INV_S, 0.f};
     a.m = tall ? xs : xk;
     a.n = tall ? xs2 : xk2;
     if (tall) launch<KS, KS>(t_gram, a, gram, st);
@@ -271,7 +343,7 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     a.K = g.sp;
     a.m = plane_side(sc.gram, g.sp, g.sp, pa, g.planes, false);
     a.n = plane_side(sc.gram, g.sp, g.sp, pa, g.planes, true);
-    launch<KC, KC>(t_poly, a, EpiPlanes{sc.poly, sc.gram, g.sp, pa, g.planes, 1, p.c * INV_S, p.b}, st);
+    launch<KC, KC>(t_poly, a, EpiPlanes<true>{sc.poly, sc.gram, g.sp, pa, g.planes, 1, p.c * INV_S, p.b}, st);
     a.sym = 0;
     a.M = g.rp;
     a.N = g.cp;
@@ -279,14 +351,19 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     a.m = tall ? xk : plane_side(sc.poly, g.sp, g.sp, pa, g.planes, false);
     a.n = tall ? plane_side(sc.poly, g.sp, g.sp, pa, g.planes, true) : xs2;
     if (it + 1 < p.steps) {
-      const EpiPlanes upd{y, x, g.cp, px, g.planes, 0, INV_S, p.a};
+      const EpiPlanes<true> upd{y, x, g.cp, px, g.planes, 0, INV_S, p.a};
       if (tall) launch<KC, KC>(t_upd, a, upd, st);
       else launch<KC, KS>(t_upd, a, upd, st);
     } else {
-      const EpiFinal fin{out, x, g.cp, px, g.planes, g.rows, g.cols, p.src_kind, p.muon, INV_S * INV_S, p.a * INV_S,
-                         p.decay, step};
-      if (tall) launch<KC, KC>(t_upd, a, fin, st);
-      else launch<KC, KS>(t_upd, a, fin, st);
+      auto fin = [&](auto KIND) {
+        const EpiFinal<KIND.value> e{out, x, g.cp, px, g.planes, g.rows, g.cols, INV_S * INV_S, p.a * INV_S, p.decay, step};
+        if (tall) launch<KC, KC>(t_upd, a, e, st);
+        else launch<KC, KS>(t_upd, a, e, st);
+      };
+      if (p.muon) fin(std::integral_constant<int, 3>{});
+      else if (p.src_kind == 0) fin(std::integral_constant<int, 0>{});
+      else if (p.src_kind == 1) fin(std::integral_constant<int, 1>{});
+      else fin(std::integral_constant<int, 2>{});
     }
     std::swap(x, y);
   }

@@ -223,7 +223,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   lce_plan_backward(s, x);
   at::Tensor dz = at::empty({N, x.ldz}, w.options()), dbp, slab;
   x.dz = m16(dz);
-  if (need_b) {
+  if (bias) {
     dbp = at::empty({2 * cdiv(N, s.tile), x.ldz}, f32);
     x.dbp = dbp.data_ptr<float>();
   }
