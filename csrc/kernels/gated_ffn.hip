@@ -205,7 +205,7 @@ void up_gate(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, 
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch<g16::KC, g16::KC, true>(g16::plan(s.N, 2 * (int64_t)s.F, s.K, 1, 1, false, false).tile, a, EpiGate<ACT>{g, u, h, s.F8}, st);
+  g16::launch<g16::KC, g16::KC, true>(g16::plan(s.N, 2 * (int64_t)s.F, s.K, 1, 1, false, false, 1.5).tile, a, EpiGate<ACT>{g, u, h, s.F8}, st);
 }
 
 template <int ACT>
@@ -217,7 +217,7 @@ void grad_gate(const FfnShape& s, const u16* dy, int64_t lddy, const FfnWeights&
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch_tile<g16::KC, g16::KS, 128, 128, 2, 2>(a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
+  g16::launch_tile<g16::KC, g16::KS, 128, 2, false>(a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
 }
 
 }  // namespace

@@ -113,6 +113,10 @@ __device__ __forceinline__ void dma16(const char* base, uint32_t off, uint32_t l
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(lds), "v"(off), "s"(base) );
 }
+__device__ __forceinline__ void dma16_if(const char* base, uint32_t off, uint32_t lds, uint64_t live) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+               :: "s"(lds), "v"(off), "s"(base), "s"(live));
+}
 __device__ __forceinline__ void dma16_at(const char* addr, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(addr) );
@@ -146,6 +150,13 @@ __device__ __forceinline__ void mfma4(f32x4& c0, f32x4& c1, f32x4& c2, f32x4& c3
   else
     asm volatile(MIHVD_G16_ASM : "+v"(c0), "+v"(c1), "+v"(c2), "+v"(c3) : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
 #undef MIHVD_G16_ASM
+}
+// Two by two, for waves of 32 x 32.
+__device__ __forceinline__ void mfma2x2(f32x4& c00, f32x4& c01, f32x4& c10, f32x4& c11, const bf16x8& a0, const bf16x8& a1,
+                                        const bf16x8& b0, const bf16x8& b1) {
+  asm volatile("s_nop 1\n\t" MIHVD_G16_MFMA " %0, %4, %6, %0\n\t" MIHVD_G16_MFMA " %1, %4, %7, %1\n\t" MIHVD_G16_MFMA
+               " %2, %5, %6, %2\n\t" MIHVD_G16_MFMA " %3, %5, %7, %3"
+               : "+v"(c00), "+v"(c01), "+v"(c10), "+v"(c11) : "v"(a0), "v"(a1), "v"(b0), "v"(b1));
 }
 // The same with one or two of the tile's copies between them, each no longer than an MFMA: from base +
 // off to LDS l + at, by all lanes or none (`live`: a loop body then needs no branch around its copies;
@@ -197,8 +208,12 @@ __device__ __forceinline__ void mfma_done(f32x4& c0, f32x4& c1, f32x4& c2, f32x4
 // compiler copies all of them to vector registers at once, which do not suffice).
 template <int NI, int MI>
 __device__ __forceinline__ void pin(f32x4 (&acc)[NI][MI], int j) {
+  if constexpr (NI == 2) {
+    asm volatile("" : "+v"(acc[0][j]), "+v"(acc[1][j]));
+    return;
+  }
 #pragma unroll
-  for (int i = 0; i < NI; i += 4) {
+  for (int i = 0; i + 3 < NI; i += 4) {
     if constexpr (NI * MI > 16) asm volatile("" : "+a"(acc[i][j]), "+a"(acc[i + 1][j]), "+a"(acc[i + 2][j]), "+a"(acc[i + 3][j]));
     else asm volatile("" : "+v"(acc[i][j]), "+v"(acc[i + 1][j]), "+v"(acc[i + 2][j]), "+v"(acc[i + 3][j]));
   }
@@ -209,6 +224,11 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The same with the newest N copies (of later tiles) still on their way.
+template <int N>
+__device__ __forceinline__ void tile_barrier_but() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+}
 __device__ __forceinline__ void tile_barrier_landed() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
@@ -352,22 +372,22 @@ __device__ __forceinline__ bool tile_at(const Args& a, int tiles_m, int kts, int
   return true;
 }
 
-// k tiles are double buffered. While tile t is multiplied, tile t + 1 is on its way or has landed;
-// after the barrier in the middle of tile t nobody reads its buffer any more (the fragments of its
-// second half are in registers), so the copies of tile t + 2 go out there, between the MFMAs, and the
-// first fragments of tile t + 1 are read: one barrier a tile, a whole tile's time for the copies,
-// and no MFMA waits on an LDS read that was not issued half a tile earlier.
+// k tiles go through S buffers. While tile t is multiplied, the tiles up to t + S - 1 are on their way or
+// have landed; after the barrier in the middle of tile t nobody reads its buffer any more (the
+// fragments of its second half are in registers), so the copies of tile t + S go out there, between the
+// MFMAs, and the first fragments of tile t + 1 are read: one barrier a tile, S - 1 tiles' time for the
+// copies, and no MFMA waits on an LDS read that was not issued half a tile earlier.
 //
 // The stream of k tiles runs on from one output tile to the next: while the epilogue works, the next
 // output tile's first two k tiles are already in LDS and its first fragments in registers, and the
 // epilogue's stores drain under the next products.
-template <int LM, int LN, int TM, int TN, int WM, int WN, bool DUAL, class Epi>
-__global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gemm16_kernel(const Args a, const Epi epi) {
-  constexpr int NT = 64 * WM * WN, WTM = TM / WM, WTN = TN / WN, MI = WTM / 16, NI = WTN / 16;
+template <int LM, int LN, int TM, int TN, int S, bool DUAL, class Epi>
+__global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) gemm16_kernel(const Args a, const Epi epi) {
+  constexpr int WM = 2, WN = 2, NT = 64 * WM * WN, WTM = TM / WM, WTN = TN / WN, MI = WTM / 16, NI = WTN / 16;
   constexpr int BUF = (TM + TN) * BK;  // elements of one buffer
   constexpr bool BIG = TM * TN > 128 * 128;
   constexpr int STAGE = 16 * (WTN + 8);  // a wave's RowStage
-  __shared__ __attribute__((aligned(128))) u16 lds[2 * BUF + WM * WN * STAGE];
+  __shared__ __attribute__((aligned(128))) u16 lds[S * BUF + WM * WN * STAGE];
   const int M = uni(a.dyn_m ? *a.dyn_m : a.M);
   const int K = uni(a.dyn_k ? *a.dyn_k : a.K);
   const int tiles_m = a.dyn_m ? (M + TM - 1) / TM : a.tiles_m;
@@ -425,7 +445,7 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
   const uint32_t ldsb = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u16*)lds;
   const uint32_t lds0 = ldsb + (uint32_t)wave * 1024u;
   // the next k tile as a whole, ahead of the loop or where the run ends
-  auto issue = [&](uint32_t l) {
+  auto issue = [&](uint32_t l) -> bool {
     if (run == 0 && !partial) next_run();
     if (run > 0) {
       sm.all(pm, nullptr, l);
@@ -434,11 +454,15 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
       pn += stepn * 2;
       if (DUAL) pa += stepn * 2;
       --run;
-    } else if (partial) {
+      return true;
+    }
+    if (partial) {
       sm.tail(pm, nullptr, l, t, krem);
       sn.tail(pn, pa, l + TM * BK * 2, t, krem);
       partial = false;
+      return true;
     }
+    return false;
   };
   Frags<LM, TM, MI, false> gm;
   Frags<LN, TN, NI, DUAL> gn;
@@ -459,35 +483,42 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
   // waited for at the barrier
   auto ahead = [](int x) constexpr { return x * NF * 4 / (3 * NX) < NF ? x * NF * 4 / (3 * NX) : NF; };
   bf16x8 fm[2][MI], fn[2][NI];
+  // the copies of the last S - 2 tiles may be on their way across a barrier; not once a tile was not
+  // issued (the end is near: then everything has to land)
+  bool flowing = true;
   nxt = cur;
   enter();
-  issue(lds0);
-  tile_barrier();
-  issue(lds0 + BUF * 2);
+  for (int q = 0; q < S; ++q) flowing &= issue(lds0 + q * (BUF * 2));
+  if (flowing) tile_barrier_but<(S - 1) * NQ>();
+  else tile_barrier();
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
     else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
   }
-  uint32_t lq = lds0, hop = BUF * 2;  // where the next copies go; to the other buffer
-  bool landed = false;                // the copies in flight were waited for ahead of an epilogue
+  uint32_t lq = lds0;  // the buffer being read, where the next copies go
+  const uint32_t lds_last = lds0 + (S - 1) * (BUF * 2);
+  int landed = 0;      // that many tiles were waited for ahead of an epilogue
 
-  auto first_half = [&]() {
-#pragma unroll
-    for (int x = 0; x < NX; x += 4) {
+  auto first_half = [&](uint32_t hop) {
+    unroll<NX / 4>([&](auto B) {
+      constexpr int x = B.value * 4, i = x / MI, j = x % MI;
 #pragma unroll
       for (int f = ahead(x); f < ahead(x + 4); ++f) {
         if (f < MI) fm[1][f < MI ? f : 0] = gm.get(f, 1);
         else fn[1][f < MI ? 0 : f - MI] = gn.get(f - MI, 1);
       }
-      const int i = x / MI, j = x % MI;
-      mfma4<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[0][i], fm[0][j], fm[0][j + 1], fm[0][j + 2],
-                 fm[0][j + 3]);
-      if (x + 8 == NX) {
+      if constexpr (MI == 2) {
+        mfma2x2(acc[0][0], acc[0][1], acc[1][0], acc[1][1], fn[0][0], fn[0][1], fm[0][0], fm[0][1]);
+      } else {
+        mfma4<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[0][i], fm[0][j], fm[0][j + 1], fm[0][j + 2],
+                   fm[0][j + 3]);
+      }
+      if (x + 8 == NX || NX == 4) {
         gm.move(hop);
         gn.move(hop);
       }
-    }
+    });
   };
   // the next k tile's copies between the MFMAs
   auto second_half = [&](uint64_t live) {
@@ -499,36 +530,45 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
         if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
         else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
       }
-      constexpr int PER = NQ * 4 / NX;  // copies among four MFMAs
-      static_assert(PER == 1 || PER == 2, "copies per four MFMAs");
-      constexpr int JM = decltype(sm)::J, q = x * NQ / NX, q2 = q + PER - 1;
-      constexpr int at1 = q < JM ? q * NT * 16 : TM * BK * 2 + (q - JM) * NT * 16;
-      constexpr int at2 = q2 < JM ? q2 * NT * 16 : TM * BK * 2 + (q2 - JM) * NT * 16;
-      const uint32_t o1 = q < JM ? sm.off[q < JM ? q : 0] : sn.off[q < JM ? 0 : q - JM];
-      const uint32_t o2 = q2 < JM ? sm.off[q2 < JM ? q2 : 0] : sn.off[q2 < JM ? 0 : q2 - JM];
-      const char* b1 = q < JM ? pm : sn.is_alt(q < JM ? 0 : q - JM) ? pa : pn;
-      const char* b2 = q2 < JM ? pm : sn.is_alt(q2 < JM ? 0 : q2 - JM) ? pa : pn;
-      if constexpr (PER == 1)
-        mfma4_copy<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
-                        fm[1][j + 2], fm[1][j + 3], lq, live, at1, o1, b1);
-      else
-        mfma4_copy2<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
-                         fm[1][j + 2], fm[1][j + 3], lq, live, at1, o1, b1, at2, o2, b2);
+      constexpr int JM = decltype(sm)::J;
+      auto lds_at = [](int q) constexpr { return q < JM ? q * NT * 16 : TM * BK * 2 + (q - JM) * NT * 16; };
+      auto off_at = [&](int q) { return q < JM ? sm.off[q < JM ? q : 0] : sn.off[q < JM ? 0 : q - JM]; };
+      auto base_at = [&](int q) { return q < JM ? pm : sn.is_alt(q < JM ? 0 : q - JM) ? pa : pn; };
+      if constexpr (MI == 2) {
+        mfma2x2(acc[0][0], acc[0][1], acc[1][0], acc[1][1], fn[1][0], fn[1][1], fm[1][0], fm[1][1]);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) dma16_if(base_at(q), off_at(q), lq + lds_at(q), live);
+      } else {
+        constexpr int PER = NQ * 4 / NX, q = x * NQ / NX, q2 = q + PER - 1;  // copies among four MFMAs
+        static_assert(PER == 1 || PER == 2, "copies per four MFMAs");
+        constexpr int at1 = lds_at(q), at2 = lds_at(q2);
+        if constexpr (PER == 1)
+          mfma4_copy<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
+                          fm[1][j + 2], fm[1][j + 3], lq, live, at1, off_at(q), base_at(q));
+        else
+          mfma4_copy2<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
+                           fm[1][j + 2], fm[1][j + 3], lq, live, at1, off_at(q), base_at(q), at2, off_at(q2), base_at(q2));
+      }
     });
-    lq += hop;
-    hop = 0u - hop;
   };
   for (;;) {
     for (int n = max(1, cur.end - cur.it); n > 0; --n) {
-      first_half();
-      if (__builtin_expect(landed, 0)) tile_barrier_landed();
-      else tile_barrier();
-      landed = false;
+      const uint32_t hop = S == 2 ? (lq == lds0 ? BUF * 2 : 0u - BUF * 2) : (lq == lds_last ? 0u - (S - 1) * (BUF * 2) : BUF * 2);
+      first_half(hop);
+      if (__builtin_expect(landed > 0, 0)) {
+        tile_barrier_landed();
+        --landed;
+      } else if (S == 2 || __builtin_expect(!flowing, 0)) {
+        tile_barrier();
+      } else {
+        tile_barrier_but<(S - 2) * NQ>();
+      }
       const int go = run > 0 ? -1 : 0;
-      if (__builtin_expect(!go, 0)) issue(lq);  // a run's end: this k tile in one go, or nothing
+      if (__builtin_expect(!go, 0)) flowing &= issue(lq);  // a run's end: this k tile in one go, or nothing
       uint64_t live;  // all lanes or none, in scalar registers
       asm volatile("v_cmp_ne_u32 %0, 0, %1" : "=s"(live) : "v"(go));
       second_half(live);
+      lq += hop;
       run += go;
       pm += (stepm * 2) & (int64_t)go;
       pn += (stepn * 2) & (int64_t)go;
@@ -546,17 +586,20 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
     c.batch = cur.batch;
     c.split = cur.split;
     c.lane = lane;
-    c.stage = lds + 2 * BUF + wave * STAGE;
+    c.stage = lds + S * BUF + wave * STAGE;
     typename Epi::template Pre<NI, MI> pre;
     epi.load(c, pre);
     // the copies in flight land before the epilogue stores anything, so that the next barrier need
     // not wait for those stores
     copies_landed();
-    landed = true;
+    landed = S - 1;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < MI; j += 4) mfma_done<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+      for (int j = 0; j < MI; j += 4) {
+        if constexpr (MI == 2) mfma_done<BIG>(acc[i][0], acc[i][1], acc[i ^ 1][0], acc[i ^ 1][1]);
+        else mfma_done<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+      }
     epi.template run<NI, MI>(c, pre, acc);
     l_mul += hops;
     if (!tile_at(a, tiles_m, kts, l_mul, cur)) break;
@@ -567,46 +610,53 @@ __global__ void __launch_bounds__(64 * WM * WN, TM * TN > 128 * 128 ? 1 : 2) gem
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 
-// Output tiles. Both shapes run four waves, two along each side.
-enum { T128 = 128, T256 = 256 };
+// Output tiles; every shape runs four waves, two along each side. T256 and T128 double buffer (one and
+// two blocks a CU); T64 keeps four buffers (two blocks a CU): for products with few tiles, whose time is
+// the copies' latency.
+enum { T64 = 64, T128 = 128, T256 = 256 };
 
-template <int LM, int LN, int TM, int TN, int WM, int WN, bool DUAL = false, class Epi>
+template <int LM, int LN, int T, int S, bool DUAL, class Epi>
 void launch_tile(Args a, const Epi& e, hipStream_t stream) {
-  a.tiles_m = cdiv(a.M, TM);
-  a.tiles_n = cdiv(a.N, DUAL ? TN / 2 : TN);
+  a.tiles_m = cdiv(a.M, T);
+  a.tiles_n = cdiv(a.N, DUAL ? T / 2 : T);
   const int64_t tiles = a.sym ? (int64_t)a.tiles_m * (a.tiles_m + 1) / 2 : (int64_t)a.tiles_m * a.tiles_n;
-  const int64_t slots = (int64_t)device_cu_count() * (TM * TN > 128 * 128 ? 1 : 2);  // resident blocks
+  const int64_t slots = (int64_t)device_cu_count() * (T > 128 ? 1 : 2);  // resident blocks
   const int64_t blocks = std::min<int64_t>(tiles * a.splits * a.batch, slots);
   if (blocks <= 0) return;
-  gemm16_kernel<LM, LN, TM, TN, WM, WN, DUAL, Epi><<<dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream>>>(a, e);
+  gemm16_kernel<LM, LN, T, T, S, DUAL, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, e);
 }
 
 template <int LM, int LN, bool DUAL = false, class Epi>
 void launch(int tile, const Args& a, const Epi& e, hipStream_t stream) {
-  if (tile == T256) launch_tile<LM, LN, 256, 256, 2, 2, DUAL>(a, e, stream);
-  else launch_tile<LM, LN, 128, 128, 2, 2, DUAL>(a, e, stream);
+  if (tile == T256) launch_tile<LM, LN, 256, 2, DUAL>(a, e, stream);
+  else if (DUAL || tile == T128) launch_tile<LM, LN, 128, 2, DUAL>(a, e, stream);
+  else launch_tile<LM, LN, 64, 4, false>(a, e, stream);
 }
 
-// How to run a product: the tile and the k splits with the least estimated time. One 64-wide k tile
-// costs a block about 1.5 us at 256x256 (one block a CU) and 0.9 us at 128x128 (two a CU); a block's
-// start and its epilogue cost about three of them; splits pay for their slabs' way through memory.
+// How to run a product: the tile and the k splits with the least estimated time, in us. Measured on
+// MI355X (16-bit operands, K = 768 and more): a 64-wide k tile takes 1.45 at 256x256; at 128x128 0.67 with
+// one block on a CU and 0.93 with two; at 64x64 0.3 and 0.57. A tile's end costs about 7, 4 and 1.5
+// more (`epi` scales it for epilogues that compute), a launch 4; splits pay a second launch and their
+// slabs' way through memory at 4 TB/s.
 struct Plan {
   int tile, splits;
 };
-inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym, bool may_split) {
+inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym, bool may_split, double epi = 1.0) {
   Plan best{T128, 1};
   double best_t = 1e30;
   const int64_t kt = (int64_t)cdiv(K, BK) * nseg;
   const int cus = device_cu_count();
-  for (int tile : {T256, T128}) {
+  for (int tile : {T256, T128, T64}) {
     const int64_t tm = cdiv(M, tile), tn = cdiv(N, tile);
     const int64_t tiles = (sym ? tm * (tm + 1) / 2 : tm * tn) * batch;
-    const int64_t slots = tile == T256 ? cus : 2 * cus;
-    const double unit = tile == T256 ? 1.5 : 0.9;
     for (int s = 1; s <= 64 && (s == 1 || (may_split && kt / s >= 4)); ++s) {
-      const int64_t rounds = (tiles * s + slots - 1) / slots;
-      double t = (double)rounds * ((double)((kt + s - 1) / s) + 3.0) * unit;
-      if (s > 1) t += 3.0 + (double)M * N * batch * (s + 0.5) * 8.0 / 4e6;
+      const bool two = tile != T256 && tiles * s > cus;  // blocks on a CU
+      const int64_t slots = two ? 2 * cus : cus;
+      const double unit = tile == T256 ? 1.45 : tile == T128 ? (two ? 0.93 : 0.67) : (two ? 0.57 : 0.3);
+      const double end = epi * (tile == T256 ? 7.0 : tile == T128 ? 4.0 : 1.5);
+      const double rounds = (double)((tiles * s + slots - 1) / slots);
+      double t = 4.0 + rounds * ((double)((kt + s - 1) / s) * unit + end);
+      if (s > 1) t += 4.0 + (double)M * N * batch * (s + 0.5) * 8.0 / 4e6;
       if (t < best_t) {
         best_t = t;
         best = {tile, s};

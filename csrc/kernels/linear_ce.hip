@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(256) lce_dh(const float* __restrict__ slab, in
 
 #ifndef MIHVD_F16
 void lce_plan(LceShape& s) {
-  s.tile = g16::plan(s.N, s.V, s.K, 1, 1, false, false).tile;
+  s.tile = g16::plan(s.N, s.V, s.K, 1, 1, false, false, 1.5).tile;
   s.npart = g16::cdiv(s.V, s.tile) * 2;
 }
 void lce_plan_backward(LceShape& s, LceScratch& x) {
