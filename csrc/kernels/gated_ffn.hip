@@ -217,7 +217,7 @@ void grad_gate(const FfnShape& s, const u16* dy, int64_t lddy, const FfnWeights&
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch_tile<g16::KC, g16::KS, 128, 2, false>(a, EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
+  g16::launch_tile<g16::KC, g16::KS, 128, 2, false, 0>(a, g16::Ragged(), EpiGateGrad<ACT>{g, u, dgu, s.F8}, st);
 }
 
 }  // namespace

@@ -38,9 +38,21 @@ static __device__ __attribute__((aligned(16))) const unsigned zeros16[4] = {0, 0
 struct Side {
   const u16* p[3] = {nullptr, nullptr, nullptr};  // one base per segment
   const u16* alt = nullptr;                       // DUAL: the second matrix of interleaved rows
+  int pl[3] = {0, 0, 0};                          // RAG: plane per segment
   int64_t ld = 0;                                 // elements between rows (KC) / between k (KS)
   int64_t bs = 0;                                 // elements between batch entries
   int ext = 0;                                    // rows (KC); storage extent, a multiple of 8 (KS)
+};
+
+// A ragged batch (template parameter RAG): entry b is a matrix of `rows` x len[b], in planes of that size
+// one behind the other from element off[b] on; a side's segment s reads plane pl[s].
+//   RAG 1: both sides are such matrices along k (K = len[b]);  RAG 2: the n side is one, K-strided (N = len[b])
+constexpr int RAG_MAX = 32;
+struct Ragged {
+  int rows = 0, count = 0;
+  int len[RAG_MAX];
+  int64_t off[RAG_MAX];
+  int start[RAG_MAX + 1];  // RAG 2: first tile of each entry; filled by launch()
 };
 
 struct Args {
@@ -60,6 +72,8 @@ struct Ctx {
   int mt, nt;      // tile indices
   int wm, wn;      // wave position in the tile
   int batch, split, lane;
+  int64_t off;     // RAG 2: the entry's first element and row length
+  int len;
   u16* stage;      // this wave's LDS for RowStage
 };
 
@@ -241,18 +255,18 @@ struct Stage {
   static_assert(J * NT == R * 8 && NT % 64 == 0, "whole chunks per thread");
   uint32_t off[J];
 
-  __device__ __forceinline__ void init(const Side& s, int x0, int t) {
+  __device__ __forceinline__ void init(int64_t ld, int ext, int x0, int t) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int i = t + j * NT;
       if constexpr (LAYOUT == KC) {
         const int row = i >> 3, src = (i & 7) ^ (row & 7);
         const int r = DUAL ? ((row >> 7) << 6) + (row & 63) : row;  // 64 rows of p, 64 of alt, ...
-        off[j] = (uint32_t)min(r, s.ext - 1 - x0) * (uint32_t)s.ld * 2u + (uint32_t)src * 16u;
+        off[j] = (uint32_t)min(r, ext - 1 - x0) * (uint32_t)ld * 2u + (uint32_t)src * 16u;
       } else {
         constexpr int RC = R / 8;
         const int k = i / RC, src = (i % RC) ^ (2 * ks_h<R>(k));
-        off[j] = (uint32_t)k * (uint32_t)s.ld * 2u + (uint32_t)min(8 * src, s.ext - 8 - x0) * 2u;
+        off[j] = (uint32_t)k * (uint32_t)ld * 2u + (uint32_t)min(8 * src, ext - 8 - x0) * 2u;
       }
     }
   }
@@ -331,22 +345,34 @@ struct Frags {
 // One output tile of one k split: where it is and its k tiles [it, end).
 struct Tile {
   int batch, split, mt, nt, it, end;
+  int K, N;  // of the batch entry
 };
 
 // Tile order. Blocks are persistent: the blocks of one XCD (every eighth block) walk a contiguous
 // run of tiles together, in groups of eight m tiles, so that the tiles an XCD has in flight share rows
 // of both operands in its L2. `l` counts within the XCD's run; false past its end.
-__device__ __forceinline__ bool tile_at(const Args& a, int tiles_m, int kts, int l, Tile& t) {
+template <int RAG, int TN>
+__device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tiles_m, int K, int l, Tile& t) {
   const int tiles = a.sym ? tiles_m * (tiles_m + 1) / 2 : tiles_m * a.tiles_n;
-  const int nb = tiles * a.splits * a.batch, x = blockIdx.x & 7;
+  const int nb = RAG == 2 ? g.start[g.count] : tiles * a.splits * a.batch, x = blockIdx.x & 7;
   const int q = nb >> 3, r = nb & 7;
   if (l >= q + (x < r ? 1 : 0)) return false;
-  int pos = x * q + min(x, r) + l, mt, nt, batch = 0, split = 0;
-  if (a.batch > 1 || a.splits > 1) {
+  int pos = x * q + min(x, r) + l, mt, nt, batch = 0, split = 0, tiles_n = a.tiles_n;
+  t.K = K;
+  t.N = a.N;
+  if constexpr (RAG == 2) {
+    while (pos >= g.start[batch + 1]) ++batch;
+    pos -= g.start[batch];
+    t.N = g.len[batch];
+    tiles_n = (t.N + TN - 1) / TN;
+  } else if (a.batch > 1 || a.splits > 1) {
     const int e = pos / tiles;
     pos -= e * tiles;
     batch = e / a.splits;
     split = e - batch * a.splits;
+    if constexpr (RAG == 1) t.K = g.len[batch];
+  } else if constexpr (RAG == 1) {
+    t.K = g.len[0];
   }
   if (a.sym) {
     mt = 0;
@@ -357,9 +383,9 @@ __device__ __forceinline__ bool tile_at(const Args& a, int tiles_m, int kts, int
     nt = mt + pos;
   } else {
     constexpr int G = 8;
-    const int g = pos / (G * a.tiles_n), first = g * G;
+    const int grp = pos / (G * tiles_n), first = grp * G;
     const int gs = min(G, tiles_m - first);
-    pos -= g * G * a.tiles_n;
+    pos -= grp * G * tiles_n;
     nt = pos / gs;
     mt = first + pos - nt * gs;
   }
@@ -367,6 +393,8 @@ __device__ __forceinline__ bool tile_at(const Args& a, int tiles_m, int kts, int
   t.split = uni(split);
   t.mt = uni(mt);
   t.nt = uni(nt);
+  t.K = uni(t.K);
+  const int kts = (t.K + BK - 1) / BK * a.nseg;
   t.it = a.splits == 1 ? 0 : uni((int)((int64_t)kts * t.split / a.splits));
   t.end = a.splits == 1 ? kts : uni((int)((int64_t)kts * (t.split + 1) / a.splits));
   return true;
@@ -381,8 +409,9 @@ __device__ __forceinline__ bool tile_at(const Args& a, int tiles_m, int kts, int
 // The stream of k tiles runs on from one output tile to the next: while the epilogue works, the next
 // output tile's first two k tiles are already in LDS and its first fragments in registers, and the
 // epilogue's stores drain under the next products.
-template <int LM, int LN, int TM, int TN, int S, bool DUAL, class Epi>
-__global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) gemm16_kernel(const Args a, const Epi epi) {
+template <int LM, int LN, int TM, int TN, int S, bool DUAL, int RAG, class Epi>
+__global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
+    gemm16_kernel(const Args a, const typename std::conditional<RAG != 0, Ragged, int>::type rag, const Epi epi) {
   constexpr int WM = 2, WN = 2, NT = 64 * WM * WN, WTM = TM / WM, WTN = TN / WN, MI = WTM / 16, NI = WTN / 16;
   constexpr int BUF = (TM + TN) * BK;  // elements of one buffer
   constexpr bool BIG = TM * TN > 128 * 128;
@@ -391,17 +420,19 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) gemm16_kerne
   const int M = uni(a.dyn_m ? *a.dyn_m : a.M);
   const int K = uni(a.dyn_k ? *a.dyn_k : a.K);
   const int tiles_m = a.dyn_m ? (M + TM - 1) / TM : a.tiles_m;
-  const int kt = (K + BK - 1) / BK, kts = kt * a.nseg;
+  const Ragged* gp = nullptr;
+  if constexpr (RAG != 0) gp = &rag;
+  const Ragged& g = *gp;  // (not read without RAG)
   const int hops = (int)(gridDim.x >> 3) + ((blockIdx.x & 7) < (gridDim.x & 7) ? 1 : 0);
   int l_mul = blockIdx.x >> 3, l_cpy = l_mul;  // the tile being multiplied, the tile being copied
   Tile cur, nxt;
-  if (!tile_at(a, tiles_m, kts, l_mul, cur)) return;
+  if (!tile_at<RAG, TN>(a, g, tiles_m, K, l_mul, cur)) return;
   const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
   Stage<LM, TM, NT, false> sm;
   Stage<LN, TN, NT, DUAL> sn;
-  const int64_t stepm = LM == KC ? BK : BK * a.m.ld, stepn = LN == KC ? BK : BK * a.n.ld;
+  int64_t stepm = LM == KC ? BK : BK * a.m.ld, stepn = LN == KC ? BK : BK * a.n.ld;
 
   // The next k tile to copy: `run` whole ones lie ahead at (pm, pn), one step apart; then, with run == 0,
   // what `next_run` finds: a partial tile (krem > 0 of its k positions, none for a split without any k),
@@ -411,34 +442,41 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) gemm16_kerne
   bool partial = false, more = true;
   auto locate = [&](int kp) {
     const int x0m = nxt.mt * TM, x0n = nxt.nt * (DUAL ? TN / 2 : TN);
-    const int64_t tm0 = a.m.bs * nxt.batch + (LM == KC ? (int64_t)x0m * a.m.ld : x0m);
-    const int64_t tn0 = a.n.bs * nxt.batch + (LN == KC ? (int64_t)x0n * a.n.ld : x0n);
+    const int64_t len = RAG ? g.len[nxt.batch] : 0, plane = RAG ? len * g.rows : 0;
+    const int64_t ldm = RAG == 1 ? len : a.m.ld, ldn = RAG ? len : a.n.ld;
+    int64_t tm0 = (RAG == 1 ? g.off[nxt.batch] : a.m.bs * nxt.batch) + (LM == KC ? (int64_t)x0m * ldm : x0m);
+    int64_t tn0 = (RAG ? g.off[nxt.batch] : a.n.bs * nxt.batch) + (LN == KC ? (int64_t)x0n * ldn : x0n);
+    if constexpr (RAG == 1) tm0 += plane * (seg == 0 ? a.m.pl[0] : seg == 1 ? a.m.pl[1] : a.m.pl[2]);
+    if constexpr (RAG != 0) tn0 += plane * (seg == 0 ? a.n.pl[0] : seg == 1 ? a.n.pl[1] : a.n.pl[2]);
     const u16* bm = seg == 0 ? a.m.p[0] : seg == 1 ? a.m.p[1] : a.m.p[2];
     const u16* bn = seg == 0 ? a.n.p[0] : seg == 1 ? a.n.p[1] : a.n.p[2];
+    if constexpr (RAG == 2) stepn = LN == KC ? BK : BK * len;
     pm = (const char*)(bm + tm0 + kp * stepm);
     pn = (const char*)(bn + tn0 + kp * stepn);
     if (DUAL) pa = (const char*)(a.n.alt + tn0 + kp * stepn);
-    const int whole = K / BK - kp;  // whole tiles of this segment from here on
+    const int whole = nxt.K / BK - kp;  // whole tiles of this segment from here on
     run = min(whole, nxt.end - nxt.it);
     partial = run == 0;
-    krem = nxt.it < nxt.end ? K - kp * BK : 0;
+    krem = nxt.it < nxt.end ? nxt.K - kp * BK : 0;
     nxt.it += max(run, 1);
   };
   auto enter = [&]() {  // the copies reach output tile nxt
-    sm.init(a.m, nxt.mt * TM, t);
-    sn.init(a.n, nxt.nt * (DUAL ? TN / 2 : TN), t);
+    const int len = RAG ? g.len[nxt.batch] : 0;
+    sm.init(RAG == 1 ? len : a.m.ld, a.m.ext, nxt.mt * TM, t);
+    sn.init(RAG ? len : a.n.ld, RAG == 2 ? len : a.n.ext, nxt.nt * (DUAL ? TN / 2 : TN), t);
+    const int kt = (nxt.K + BK - 1) / BK;
     seg = a.nseg == 1 ? 0 : uni(kt > 0 ? nxt.it / kt : 0);
     locate(nxt.it - seg * kt);
   };
   auto next_run = [&]() {
     if (!more) return;
     if (nxt.it < nxt.end) {
-      const int kp = nxt.it - seg * kt;
+      const int kt = (nxt.K + BK - 1) / BK, kp = nxt.it - seg * kt;
       if (kp == kt) ++seg;
       locate(kp == kt ? 0 : kp);
     } else {
       l_cpy += hops;
-      more = tile_at(a, tiles_m, kts, l_cpy, nxt);
+      more = tile_at<RAG, TN>(a, g, tiles_m, K, l_cpy, nxt);
       if (more) enter();
     }
   };
@@ -578,7 +616,9 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) gemm16_kerne
     c.m0 = cur.mt * TM + wm * WTM;
     c.n0 = cur.nt * (DUAL ? TN / 2 : TN) + wn * (DUAL ? WTN / 2 : WTN);
     c.M = M;
-    c.N = a.N;
+    c.N = cur.N;
+    c.off = RAG == 2 ? g.off[cur.batch] : 0;
+    c.len = RAG == 2 ? cur.N : 0;
     c.mt = cur.mt;
     c.nt = cur.nt;
     c.wm = wm;
@@ -602,7 +642,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) gemm16_kerne
       }
     epi.template run<NI, MI>(c, pre, acc);
     l_mul += hops;
-    if (!tile_at(a, tiles_m, kts, l_mul, cur)) break;
+    if (!tile_at<RAG, TN>(a, g, tiles_m, K, l_mul, cur)) break;
     clear();
   }
 }
@@ -615,22 +655,32 @@ inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 // the copies' latency.
 enum { T64 = 64, T128 = 128, T256 = 256 };
 
-template <int LM, int LN, int T, int S, bool DUAL, class Epi>
-void launch_tile(Args a, const Epi& e, hipStream_t stream) {
+template <int LM, int LN, int T, int S, bool DUAL, int RAG, class Epi>
+void launch_tile(Args a, Ragged g, const Epi& e, hipStream_t stream) {
   a.tiles_m = cdiv(a.M, T);
   a.tiles_n = cdiv(a.N, DUAL ? T / 2 : T);
-  const int64_t tiles = a.sym ? (int64_t)a.tiles_m * (a.tiles_m + 1) / 2 : (int64_t)a.tiles_m * a.tiles_n;
+  int64_t tiles = a.sym ? (int64_t)a.tiles_m * (a.tiles_m + 1) / 2 : (int64_t)a.tiles_m * a.tiles_n;
+  tiles *= a.splits * a.batch;
+  if (RAG == 2) {
+    tiles = 0;
+    for (int b = 0; b < g.count; ++b) {
+      g.start[b] = (int)tiles;
+      tiles += (int64_t)a.tiles_m * cdiv(g.len[b], T);
+    }
+    g.start[g.count] = (int)tiles;
+  }
   const int64_t slots = (int64_t)device_cu_count() * (T > 128 ? 1 : 2);  // resident blocks
-  const int64_t blocks = std::min<int64_t>(tiles * a.splits * a.batch, slots);
+  const int64_t blocks = std::min<int64_t>(tiles, slots);
   if (blocks <= 0) return;
-  gemm16_kernel<LM, LN, T, T, S, DUAL, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, e);
+  if constexpr (RAG != 0) gemm16_kernel<LM, LN, T, T, S, DUAL, RAG, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, g, e);
+  else gemm16_kernel<LM, LN, T, T, S, DUAL, 0, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, 0, e);
 }
 
-template <int LM, int LN, bool DUAL = false, class Epi>
-void launch(int tile, const Args& a, const Epi& e, hipStream_t stream) {
-  if (tile == T256) launch_tile<LM, LN, 256, 2, DUAL>(a, e, stream);
-  else if (DUAL || tile == T128) launch_tile<LM, LN, 128, 2, DUAL>(a, e, stream);
-  else launch_tile<LM, LN, 64, 4, false>(a, e, stream);
+template <int LM, int LN, bool DUAL = false, int RAG = 0, class Epi>
+void launch(int tile, const Args& a, const Epi& e, hipStream_t stream, const Ragged& g = Ragged()) {
+  if (tile == T256) launch_tile<LM, LN, 256, 2, DUAL, RAG>(a, g, e, stream);
+  else if (DUAL || tile == T128) launch_tile<LM, LN, 128, 2, DUAL, RAG>(a, g, e, stream);
+  else if constexpr (!DUAL) launch_tile<LM, LN, 64, 4, false, RAG>(a, g, e, stream);
 }
 
 // How to run a product: the tile and the k splits with the least estimated time, in us. Measured on

@@ -151,40 +151,35 @@ struct EpiStats {
   }
 };
 
-// Joins the pairs of every row: 16 lanes a row. Writes lse (compact) and the row's loss (all rows).
+// Joins the pairs of every row: one wave a row, so that a handful of rows still has its loads in flight
+// together. Writes lse (compact) and the row's loss (all rows).
 __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ part, int npart,
                                                   const float* __restrict__ zlab, const int* __restrict__ label,
                                                   const int* __restrict__ inv, int N, int V, float* __restrict__ lse,
                                                   float* __restrict__ rows) {
-  const int l = threadIdx.x & 15;
-  const int r = blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int c = r < N ? inv[r] : -1;
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= N) return;
+  const int c = inv[r];
   if (c < 0) {
-    if (r < N && l == 0) rows[r] = 0.f;
+    if (lane == 0) rows[r] = 0.f;
     return;
   }
-  float mx = -INFINITY, s = 0.f;
-  for (int p = l; p < npart; p += 16) {
-    const float2 q = part[(int64_t)c * npart + p];
-    const float m2 = fmaxf(mx, q.x);
-    const float ref = m2 == -INFINITY ? 0.f : m2;
-    s = s * __expf(mx - ref) + q.y * __expf(q.x - ref);
-    mx = m2;
-  }
-#pragma unroll
-  for (int x = 1; x < 16; x <<= 1) {
-    const float om = __shfl_xor(mx, x), os = __shfl_xor(s, x);
-    const float m2 = fmaxf(mx, om);
-    const float ref = m2 == -INFINITY ? 0.f : m2;
-    s = s * __expf(mx - ref) + os * __expf(om - ref);
-    mx = m2;
-  }
-  if (l == 0) {
+  const float2* q = part + (int64_t)c * npart;
+  float mx = -INFINITY;
+  for (int p = lane; p < npart; p += 64) mx = fmaxf(mx, q[p].x);
+  mx = wave_max(mx);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float s = 0.f;
+  for (int p = lane; p < npart; p += 64) s += q[p].y * __expf(q[p].x - ref);
+  s = wave_sum(s);
+  if (lane == 0) {
     const int y = label[c];
     // a label outside the vocabulary has no loss: NaN, and NaN gradients through lse
-    const float v = (y >= 0 && y < V) ? logf(s) + mx : NAN;
+    const bool in = y >= 0 && y < V;
+    const float v = in ? logf(s) + mx : NAN;
     lse[c] = v;
-    rows[r] = v - (y >= 0 && y < V ? zlab[c] : 0.f);
+    rows[r] = v - (in ? zlab[c] : 0.f);
   }
 }
 
@@ -326,6 +321,16 @@ __global__ void __launch_bounds__(256) lce_dh(const float* __restrict__ slab, in
   g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
 }
 
+template <bool BIAS, class Epi>
+void dz_launch(int tile, const g16::Args& a, const Epi& e, hipStream_t st) {
+  if constexpr (BIAS) {
+    if (tile == g16::T128) g16::launch_tile<g16::KC, g16::KC, 128, 2, false, 0>(a, g16::Ragged(), e, st);
+    else g16::launch_tile<g16::KC, g16::KC, 64, 4, false, 0>(a, g16::Ragged(), e, st);
+  } else {
+    g16::launch<g16::KC, g16::KC>(tile, a, e, st);
+  }
+}
+
 }  // namespace
 
 #ifndef MIHVD_F16
@@ -333,8 +338,11 @@ void lce_plan(LceShape& s) {
   s.tile = g16::plan(s.N, s.V, s.K, 1, 1, false, false, 1.5).tile;
   s.npart = g16::cdiv(s.V, s.tile) * 2;
 }
-void lce_plan_backward(LceShape& s, LceScratch& x) {
-  lce_plan(s);
+void lce_plan_backward(LceShape& s, LceScratch& x, bool bias) {
+  // the bias gradient's sums on top of the accumulators spill at 256x256 (135 us a piece against 84
+  // without them, at 1229 x 30522 x 768); at 128x128 they fit
+  x.dz_tile = g16::plan(s.N, std::min(x.piece, s.V), s.K, 1, 1, false, false, 1.5).tile;
+  if (bias && x.dz_tile == g16::T256) x.dz_tile = g16::T128;
   const g16::Plan p = g16::plan(s.N, s.K, x.piece, 1, 1, false, true);
   x.dh_tile = p.tile;
   x.splits = p.splits;
@@ -359,7 +367,7 @@ void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t 
   a.dyn_m = rw.cnt;
   if (bias) g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<true>{bias, bias_kind, rw.label, part, s.npart, zlab}, st);
   else g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<false>{nullptr, 0, rw.label, part, s.npart, zlab}, st);
-  lce_finish<<<g16::cdiv(s.N, 16), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
+  lce_finish<<<g16::cdiv(s.N, 4), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
   if (loss) lce_reduce<<<1, 1024, 0, st>>>(rows, s.N, rw.cnt, mean, loss);
 }
 
@@ -384,7 +392,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       const void* b = bias ? static_cast<const char*>(bias) + (int64_t)v0 * (bias_kind == 1 ? 4 : 2) : nullptr;
       auto go = [&](auto B, auto R) {
         EpiDz<B.value, R.value> e{b, bias_kind, rw.label, lse, g.rowscale, v0, x.dz, x.ldz, x.dbp};
-        g16::launch<g16::KC, g16::KC>(s.tile, a, e, st);
+        dz_launch<B.value>(x.dz_tile, a, e, st);
       };
       if (bias && g.rowscale) go(std::true_type{}, std::true_type{});
       else if (bias) go(std::true_type{}, std::false_type{});
@@ -393,7 +401,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
     }
     if (db) {
       const int esz = bias_kind == 1 ? 4 : 2;
-      lce_db<<<g16::cdiv(nv, 256), 256, 0, st>>>(x.dbp, x.ldz, rw.cnt, s.tile, 2, nv, g.scale,
+      lce_db<<<g16::cdiv(nv, 256), 256, 0, st>>>(x.dbp, x.ldz, rw.cnt, x.dz_tile, 2, nv, g.scale,
                                                  static_cast<char*>(db) + (int64_t)v0 * esz, bias_kind);
     }
     if (dw) {

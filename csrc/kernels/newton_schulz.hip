@@ -1,7 +1,8 @@
 // Orthogonalising a matrix by Newton-Schulz steps, and the weight update made of it.
 //
 //   X = u / (|u|_F + eps);   per step  A = X X^T,  B = b A + c A A,  X <- a X + B X
-// (for more rows than columns the same on the other side: A = X^T X, X <- a X + X B).
+// with the smaller side of the matrix as X's rows (a tall one is turned on the way in and out), so that
+// matrices of different lengths, wide or tall, run in one batch wherever their smaller sides agree.
 //
 // X, A and B are bounded (singular values stay below ~1.3), so they are held in fp16 scaled by 2^12:
 // the MFMA rate of bf16 with three more bits. fp32 values are held as two fp16 planes hi + lo (22
@@ -24,71 +25,126 @@ namespace {
 
 constexpr float S = 4096.f, INV_S = 1.f / 4096.f;
 
-struct NsTable {
-  const void* src[NS_MAX];
-  float* mom[NS_MAX];
-};
-struct NsOut {
-  void* dst[NS_MAX];
-};
-
-__device__ __forceinline__ float load_src(const void* p, int kind, int64_t i) {
-  if (kind == 0) return static_cast<const float*>(p)[i];
+template <int KIND>
+__device__ __forceinline__ float load_src(const void* p, int64_t i) {
+  if constexpr (KIND == 0) return static_cast<const float*>(p)[i];
   const u16 h = static_cast<const u16*>(p)[i];
-  return kind == 1 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+  return KIND == 1 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+}
+// four consecutive values (the caller has checked the alignment)
+template <int KIND>
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
+  if constexpr (KIND == 0) {
+    return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const u16*>(p) + i);
+    const u16 h[4] = {(u16)w.x, (u16)(w.x >> 16), (u16)w.y, (u16)(w.y >> 16)};
+    f32x4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = KIND == 1 ? __uint_as_float((uint32_t)h[k] << 16) : (float)__builtin_bit_cast(_Float16, h[k]);
+    return v;
+  }
 }
 
 // Sum of squares of each matrix, NS_PART partial sums; for Muon the momentum is updated on the way:
-// m = mu m + g, u = g + mu m (nesterov) or m.
-__global__ void __launch_bounds__(256) ns_norm(const NsTable t, int64_t n, int kind, int muon, float mu, int nesterov,
-                                               float* __restrict__ partial) {
+// m = mu m + g, u = g + mu m (nesterov) or m. Bound by memory: one read of each input, one write of m.
+template <int KIND>
+__global__ void __launch_bounds__(256) ns_norm(const NsGroup t, int muon, float mu, int nesterov, float* __restrict__ partial) {
   __shared__ float sh[4];
-  const int b = blockIdx.y;
-  float s = 0.f;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float v = load_src(t.src[b], kind, i);
-    if (muon) {
-      const float m = fmaf(mu, t.mom[b][i], v);
-      t.mom[b][i] = m;
-      v = nesterov ? fmaf(mu, m, v) : m;
-    }
-    s = fmaf(v, v, s);
-  }
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) partial[b * NS_PART + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
-}
-
-// planes of S * v: hi, and lo = the rest
-__device__ __forceinline__ void put_planes(u16* p, int64_t plane, int planes, float v) {
-  const u16 hi = f2bf(v);
-  p[0] = hi;
-  if (planes == 2) p[plane] = f2bf(v - bf2f(hi));
-}
-
-__global__ void __launch_bounds__(256) ns_scale(const NsTable t, int rows, int cols, int rp, int cp, int planes, int kind,
-                                                int muon, float mu, int nesterov, float eps,
-                                                const float* __restrict__ partial, u16* __restrict__ x) {
-  const int b = blockIdx.y, lane = threadIdx.x & 63;
-  const float norm = sqrtf(wave_sum(partial[b * NS_PART + lane]));
-  const float inv = S / (norm + eps);
-  const int64_t plane = (int64_t)rp * cp;
-  u16* o = x + (int64_t)b * planes * plane;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cp;
-    const int c = (int)(i - r * cp);
-    float v = 0.f;
-    if (r < rows && c < cols) {
-      const int64_t k = r * cols + c;
-      v = load_src(t.src[b], kind, k);
+  const NsMat& q = t.m[blockIdx.y];
+  const int64_t n = (int64_t)q.rows * q.cols, stride = (int64_t)gridDim.x * 1024;
+  const bool vec = n % 4 == 0 && ((uintptr_t)q.src & (KIND ? 7 : 15)) == 0 && (!muon || ((uintptr_t)q.mom & 15) == 0);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (vec) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += stride) {
+      f32x4 v = load4<KIND>(q.src, i);
       if (muon) {
-        const float m = t.mom[b][k];
+        f32x4 m = *reinterpret_cast<f32x4*>(q.mom + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          m[k] = fmaf(mu, m[k], v[k]);
+          v[k] = nesterov ? fmaf(mu, m[k], v[k]) : m[k];
+        }
+        *reinterpret_cast<f32x4*>(q.mom + i) = m;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] = fmaf(v[k], v[k], s[k]);
+    }
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride / 4) {
+      float v = load_src<KIND>(q.src, i);
+      if (muon) {
+        const float m = fmaf(mu, q.mom[i], v);
+        q.mom[i] = m;
         v = nesterov ? fmaf(mu, m, v) : m;
       }
-      v *= inv;
+      s[0] = fmaf(v, v, s[0]);
     }
-    put_planes(o + i, plane, planes, v);
+  }
+  const float w = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.y * NS_PART + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// X = S u / (|u| + eps) into planes, with the smaller side as rows: a 64 x 64 tile a block, turned in LDS
+// where the matrix is tall; zeros in the padding.
+template <int KIND>
+__global__ void __launch_bounds__(256) ns_scale(const NsGroup t, int muon, float mu, int nesterov, float eps,
+                                                const float* __restrict__ partial, u16* __restrict__ x) {
+  __shared__ float sh[64][65];
+  const NsMat& q = t.m[blockIdx.y];
+  const int tl = q.len / 64, tiles = t.side / 64 * tl;
+  const float inv = S / (sqrtf(wave_sum(partial[blockIdx.y * NS_PART + (threadIdx.x & 63)])) + eps);
+  const bool tall = q.rows > q.cols;
+  const int64_t plane = (int64_t)t.side * q.len;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int ts = tile / tl * 64, tn = tile % tl * 64;  // along the side, along the length
+    const int r0 = tall ? tn : ts, c0 = tall ? ts : tn;
+    const bool vec = q.cols % 4 == 0 && ((uintptr_t)q.src & (KIND ? 7 : 15)) == 0 && (!muon || ((uintptr_t)q.mom & 15) == 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = threadIdx.x / 16 + i * 16, c = (threadIdx.x & 15) * 4;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (r0 + r < q.rows) {
+        const int64_t at = (int64_t)(r0 + r) * q.cols + c0 + c;
+        if (vec && c0 + c < q.cols) {
+          v = load4<KIND>(q.src, at);
+          if (muon) {
+            const f32x4 m = *reinterpret_cast<const f32x4*>(q.mom + at);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = nesterov ? fmaf(mu, m[k], v[k]) : m[k];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c0 + c + k < q.cols) {
+              v[k] = load_src<KIND>(q.src, at + k);
+              if (muon) v[k] = nesterov ? fmaf(mu, q.mom[at + k], v[k]) : q.mom[at + k];
+            }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sh[r][c + k] = v[k] * inv;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = threadIdx.x / 8 + i * 32, c = (threadIdx.x & 7) * 8;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = tall ? sh[c + k][r] : sh[r][c + k];
+      u16* o = x + q.off + (int64_t)(ts + r) * q.len + tn + c;
+      const uint2 h0 = pack4bf(v[0], v[1], v[2], v[3]), h1 = pack4bf(v[4], v[5], v[6], v[7]);
+      *reinterpret_cast<uint4*>(o) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+      if (t.planes == 2) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] -= bf2f(f2bf(v[k]));
+        const uint2 l0 = pack4bf(v[0], v[1], v[2], v[3]), l1 = pack4bf(v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<uint4*>(o + plane) = make_uint4(l0.x, l0.y, l1.x, l1.y);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -98,7 +154,7 @@ template <bool IN>
 struct EpiPlanes {
   u16* out;
   const u16* in;
-  int64_t ld, plane;
+  int64_t ld_, plane_;  // 0: a ragged batch's
   int planes, sym;
   float alpha, beta;
   template <int NI, int MI>
@@ -107,8 +163,10 @@ struct EpiPlanes {
   __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
   template <int NI, int MI>
   __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
-    u16* o = out + (int64_t)c.batch * planes * plane;
-    const u16* q = IN ? in + (int64_t)c.batch * planes * plane : nullptr;
+    const int64_t ld = ld_ ? ld_ : c.len, plane = ld_ ? plane_ : (int64_t)c.M * c.len;
+    const int64_t first = ld_ ? (int64_t)c.batch * planes * plane : c.off;
+    u16* o = out + first;
+    const u16* q = IN ? in + first : nullptr;
     const g16::RowStage<NI * 16> st{c.stage, c.lane};
     constexpr int G = st.GETS;
     uint4 iq[2][G];
@@ -193,32 +251,51 @@ struct EpiPlanes {
 };
 
 // The last step: v = alpha * acc + beta * X, unscaled, into the result (KIND 0 fp32, 1 bf16, 2 fp16) or the
-// weight (3: w = w * decay - step * v).
+// weight (3: w = w * decay - step * v); column n of X is a row of a tall matrix.
+struct NsOut {
+  void* dst[NS_MAX];
+  int rows[NS_MAX], cols[NS_MAX];
+  float step[NS_MAX];
+};
+template <int KIND>
+__device__ __forceinline__ void put_out(void* o, int64_t at, float v, float decay, float step) {
+  if constexpr (KIND == 3) {
+    float* w = static_cast<float*>(o) + at;
+    *w = fmaf(-step, v, *w * decay);
+  } else if constexpr (KIND == 0) {
+    static_cast<float*>(o)[at] = v;
+  } else {
+    static_cast<u16*>(o)[at] = KIND == 1 ? __builtin_bit_cast(u16, (__bf16)v) : f2bf(v);
+  }
+}
 template <int KIND>
 struct EpiFinal {
   NsOut out;
   const u16* in;
-  int64_t ld, plane;
-  int planes, rows, cols;
-  float alpha, beta, decay, step;
+  int planes;
+  float alpha, beta, decay;
   template <int NI, int MI>
   struct Pre {};
   template <int NI, int MI>
   __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
   template <int NI, int MI>
   __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
-    const u16* q = in + (int64_t)c.batch * planes * plane;
+    const int64_t ld = c.len, plane = (int64_t)c.M * c.len;
+    const u16* q = in + c.off;
     void* o = out.dst[c.batch];
-    const bool vec = cols % 4 == 0;
+    const int rows = out.rows[c.batch], cols = out.cols[c.batch];
+    const float step = out.step[c.batch];
+    const bool tall = rows > cols, vec = cols % 4 == 0 && ((uintptr_t)o & 15) == 0;
+    const int side = min(rows, cols), len = max(rows, cols);
     g16::unroll<MI>([&](auto J) {
       constexpr int j = J.value;
       g16::pin(acc, j);
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= rows) return;
+      if (m >= side) return;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        if (n >= cols) continue;
+        if (n >= len) continue;
         const uint2 h = *reinterpret_cast<const uint2*>(q + (int64_t)m * ld + n);
         uint2 l = make_uint2(0, 0);
         if (planes == 2) l = *reinterpret_cast<const uint2*>(q + plane + (int64_t)m * ld + n);
@@ -227,143 +304,137 @@ struct EpiFinal {
         f32x4 v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = fmaf(beta, x[k], alpha * acc[i][j][k]);
-        const int64_t at = (int64_t)m * cols + n;
-        if constexpr (KIND == 0 || KIND == 3) {
-          float* w = static_cast<float*>(o) + at;
-          if (vec && ((uintptr_t)o & 15) == 0) {
-            f32x4 r = v;
-            if constexpr (KIND == 3) r = *reinterpret_cast<f32x4*>(w) * decay - v * step;
-            *reinterpret_cast<f32x4*>(w) = r;
-          } else {
+        if (tall) {  // 16 lanes write 16 neighbours of one row
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (n + k < cols) w[k] = KIND == 3 ? fmaf(-step, v[k], w[k] * decay) : v[k];
+          for (int k = 0; k < 4; ++k)
+            if (n + k < len) put_out<KIND>(o, (int64_t)(n + k) * cols + m, v[k], decay, step);
+        } else if (vec && (KIND == 0 || KIND == 3)) {
+          f32x4* w = reinterpret_cast<f32x4*>(static_cast<float*>(o) + (int64_t)m * cols + n);
+          if constexpr (KIND == 3) {
+            f32x4 r = *w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[k] = fmaf(-step, v[k], r[k] * decay);
+            *w = r;
+          } else {
+            *w = v;
           }
-        } else {
-          u16* w = static_cast<u16*>(o) + at;
-          u16 r[4];
+        } else if (vec) {
+          uint32_t r[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) r[k] = KIND == 1 ? __builtin_bit_cast(u16, (__bf16)v[k]) : f2bf(v[k]);
-          if (vec && ((uintptr_t)o & 7) == 0) {
-            *reinterpret_cast<uint2*>(w) = make_uint2((uint32_t)r[0] | ((uint32_t)r[1] << 16), (uint32_t)r[2] | ((uint32_t)r[3] << 16));
-          } else {
+          *reinterpret_cast<uint2*>(static_cast<u16*>(o) + (int64_t)m * cols + n) = make_uint2(r[0] | (r[1] << 16), r[2] | (r[3] << 16));
+        } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (n + k < cols) w[k] = r[k];
-          }
+          for (int k = 0; k < 4; ++k)
+            if (n + k < len) put_out<KIND>(o, (int64_t)m * cols + n + k, v[k], decay, step);
         }
       }
     });
   }
 };
 
-// steps == 0: the normalised matrix itself
-__global__ void __launch_bounds__(256) ns_copy_out(const u16* __restrict__ x, const NsOut out, int rows, int cols, int rp,
-                                                   int cp, int planes, int kind, int muon, float decay, float step) {
-  const int b = blockIdx.y;
-  const int64_t plane = (int64_t)rp * cp, n = (int64_t)rows * cols;
-  const u16* q = x + (int64_t)b * planes * plane;
+// no steps: the normalised matrix itself
+template <int KIND>
+__global__ void __launch_bounds__(256) ns_copy_out(const NsGroup t, const u16* __restrict__ x, const NsOut out, float decay) {
+  const NsMat& q = t.m[blockIdx.y];
+  const int64_t plane = (int64_t)t.side * q.len, n = (int64_t)q.rows * q.cols;
+  const bool tall = q.rows > q.cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols, at = r * cp + (i - r * cols);
-    float v = bf2f(q[at]);
-    if (planes == 2) v += bf2f(q[plane + at]);
-    v *= INV_S;
-    if (muon) {
-      float* w = static_cast<float*>(out.dst[b]) + i;
-      *w = fmaf(-step, v, *w * decay);
-    } else if (kind == 0) {
-      static_cast<float*>(out.dst[b])[i] = v;
-    } else if (kind == 1) {
-      static_cast<u16*>(out.dst[b])[i] = __builtin_bit_cast(u16, (__bf16)v);
-    } else {
-      static_cast<u16*>(out.dst[b])[i] = f2bf(v);
-    }
+    const int64_t r = i / q.cols, c = i - r * q.cols, at = q.off + (tall ? c * q.len + r : r * q.len + c);
+    float v = bf2f(x[at]);
+    if (t.planes == 2) v += bf2f(x[plane + at]);
+    put_out<KIND>(out.dst[blockIdx.y], i, v * INV_S, decay, out.step[blockIdx.y]);
   }
 }
 
-g16::Side plane_side(const u16* x, int64_t ld, int ext, int64_t plane, int planes, bool second) {
+g16::Side square_side(const u16* x, int64_t side, int planes, bool second) {
   // segments hi hi, hi lo, lo hi
   g16::Side s;
+  const int64_t plane = side * side;
   s.p[0] = x;
   s.p[1] = second ? x + plane : x;
   s.p[2] = second ? x : x + plane;
-  s.ld = ld;
+  s.ld = side;
   s.bs = planes * plane;
-  s.ext = ext;
+  s.ext = (int)side;
   return s;
+}
+g16::Side ragged_side(const u16* x, int side, bool second) {
+  g16::Side s;
+  s.p[0] = s.p[1] = s.p[2] = x;
+  s.pl[1] = second ? 1 : 0;
+  s.pl[2] = second ? 0 : 1;
+  s.ext = side;
+  return s;
+}
+
+template <class F>
+void with_kind(const NsParams& p, F&& f) {
+  if (p.src_kind == 0) f(std::integral_constant<int, 0>{});
+  else if (p.src_kind == 1) f(std::integral_constant<int, 1>{});
+  else f(std::integral_constant<int, 2>{});
 }
 
 }  // namespace
 
 void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_t st) {
   using namespace g16;
-  NsTable tab;
-  NsOut out;
-  for (int i = 0; i < NS_MAX; ++i) {
-    tab.src[i] = g.src[i];
-    tab.mom[i] = g.mom[i];
-    out.dst[i] = g.dst[i];
+  NsOut out{};
+  Ragged rg;
+  rg.rows = g.side;
+  rg.count = g.count;
+  int64_t most = 0, total = 0;
+  for (int i = 0; i < g.count; ++i) {
+    out.dst[i] = g.m[i].dst;
+    out.rows[i] = g.m[i].rows;
+    out.cols[i] = g.m[i].cols;
+    out.step[i] = g.m[i].step;
+    rg.len[i] = g.m[i].len;
+    rg.off[i] = g.m[i].off;
+    most = std::max<int64_t>(most, g.m[i].len);
+    total += g.m[i].len;
   }
-  const int64_t n = (int64_t)g.rows * g.cols, px = (int64_t)g.rp * g.cp, pa = (int64_t)g.sp * g.sp;
-  const int grid = (int)std::min<int64_t>(512, (px + 255) / 256);
-  ns_norm<<<dim3(NS_PART, g.count), 256, 0, st>>>(tab, n, p.src_kind, p.muon, p.momentum, p.nesterov, sc.partial);
-  ns_scale<<<dim3(grid, g.count), 256, 0, st>>>(tab, g.rows, g.cols, g.rp, g.cp, g.planes, p.src_kind, p.muon, p.momentum,
-                                               p.nesterov, p.eps, sc.partial, sc.x0);
-  const float step = p.lr * p.scale;
-  if (p.steps == 0) {
-    ns_copy_out<<<dim3(grid, g.count), 256, 0, st>>>(sc.x0, out, g.rows, g.cols, g.rp, g.cp, g.planes, p.src_kind, p.muon,
-                                                     p.decay, step);
-    return;
-  }
-  // All sides are padded to 64 with zeros, which the products keep: a zero row or column of X gives zero
+  const int grid = (int)std::min<int64_t>(2048, g.side / 64 * (most / 64));
+  with_kind(p, [&](auto K) {
+    ns_norm<K.value><<<dim3(NS_PART, g.count), 256, 0, st>>>(g, p.muon, p.momentum, p.nesterov, sc.partial);
+    ns_scale<K.value><<<dim3(grid, g.count), 256, 0, st>>>(g, p.muon, p.momentum, p.nesterov, p.eps, sc.partial, sc.x0);
+    if (p.steps == 0) {
+      if (p.muon) ns_copy_out<3><<<dim3(grid, g.count), 256, 0, st>>>(g, sc.x0, out, p.decay);
+      else ns_copy_out<K.value><<<dim3(grid, g.count), 256, 0, st>>>(g, sc.x0, out, p.decay);
+    }
+  });
+  // The sides are padded to 64 with zeros, which the products keep: a zero row or column of X gives zero
   // rows and columns of A, B and the next X.
-  const bool tall = g.rp > g.cp;
   const int nseg = g.planes == 2 ? 3 : 1;
-  const int big = std::max(g.rp, g.cp);
-  const int t_gram = plan(g.sp, g.sp, big, nseg, g.count, true, false).tile;
-  const int t_poly = plan(g.sp, g.sp, g.sp, nseg, g.count, true, false).tile;
-  const int t_upd = plan(g.rp, g.cp, g.sp, nseg, g.count, false, false).tile;
+  const int64_t sp = g.side, pa = sp * sp;
+  const int t_gram = plan(sp, sp, total / g.count, nseg, g.count, true, false).tile;
+  const int t_poly = plan(sp, sp, sp, nseg, g.count, true, false).tile;
+  const int t_upd = plan(sp, total, sp, nseg, 1, false, false).tile;
   u16 *x = sc.x0, *y = sc.x1;
   for (int it = 0; it < p.steps; ++it) {
     Args a;
     a.batch = g.count;
     a.nseg = nseg;
     a.sym = 1;
-    a.M = a.N = g.sp;
-    a.K = big;
-    const Side xk = plane_side(x, g.cp, g.rp, px, g.planes, false);       // rows of X
-    const Side xk2 = plane_side(x, g.cp, g.rp, px, g.planes, true);
-    const Side xs = plane_side(x, g.cp, g.cp, px, g.planes, false);       // columns of X
-    const Side xs2 = plane_side(x, g.cp, g.cp, px, g.planes, true);
-    const EpiPlanes<false> gram{sc.gram, nullptr, g.sp, pa, g.planes, 1, INV_S, 0.f};
-    a.m = tall ? xs : xk;
-    a.n = tall ? xs2 : xk2;
-    if (tall) launch<KS, KS>(t_gram, a, gram, st);
-    else launch<KC, KC>(t_gram, a, gram, st);
-    a.K = g.sp;
-    a.m = plane_side(sc.gram, g.sp, g.sp, pa, g.planes, false);
-    a.n = plane_side(sc.gram, g.sp, g.sp, pa, g.planes, true);
-    launch<KC, KC>(t_poly, a, EpiPlanes<true>{sc.poly, sc.gram, g.sp, pa, g.planes, 1, p.c * INV_S, p.b}, st);
+    a.M = a.N = g.side;
+    a.m = ragged_side(x, g.side, false);
+    a.n = ragged_side(x, g.side, true);
+    launch<KC, KC, false, 1>(t_gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f}, st, rg);
+    a.K = g.side;
+    a.m = square_side(sc.gram, sp, g.planes, false);
+    a.n = square_side(sc.gram, sp, g.planes, true);
+    launch<KC, KC>(t_poly, a, EpiPlanes<true>{sc.poly, sc.gram, sp, pa, g.planes, 1, p.c * INV_S, p.b}, st);
     a.sym = 0;
-    a.M = g.rp;
-    a.N = g.cp;
-    // tall: X B, rows of X against rows of the symmetric B; else B X
-    a.m = tall ? xk : plane_side(sc.poly, g.sp, g.sp, pa, g.planes, false);
-    a.n = tall ? plane_side(sc.poly, g.sp, g.sp, pa, g.planes, true) : xs2;
+    a.m = square_side(sc.poly, sp, g.planes, false);
+    a.n = ragged_side(x, 0, true);
     if (it + 1 < p.steps) {
-      const EpiPlanes<true> upd{y, x, g.cp, px, g.planes, 0, INV_S, p.a};
-      if (tall) launch<KC, KC>(t_upd, a, upd, st);
-      else launch<KC, KS>(t_upd, a, upd, st);
+      launch<KC, KS, false, 2>(t_upd, a, EpiPlanes<true>{y, x, 0, 0, g.planes, 0, INV_S, p.a}, st, rg);
     } else {
-      auto fin = [&](auto KIND) {
-        const EpiFinal<KIND.value> e{out, x, g.cp, px, g.planes, g.rows, g.cols, INV_S * INV_S, p.a * INV_S, p.decay, step};
-        if (tall) launch<KC, KC>(t_upd, a, e, st);
-        else launch<KC, KS>(t_upd, a, e, st);
+      auto fin = [&](auto K) {
+        launch<KC, KS, false, 2>(t_upd, a, EpiFinal<K.value>{out, x, g.planes, INV_S * INV_S, p.a * INV_S, p.decay}, st, rg);
       };
       if (p.muon) fin(std::integral_constant<int, 3>{});
-      else if (p.src_kind == 0) fin(std::integral_constant<int, 0>{});
-      else if (p.src_kind == 1) fin(std::integral_constant<int, 1>{});
-      else fin(std::integral_constant<int, 2>{});
+      else with_kind(p, fin);
     }
     std::swap(x, y);
   }

@@ -32,13 +32,13 @@ struct LceScratch {
   int64_t ldz;   // row stride of dz, a multiple of 8
   u16* dz;       // [N][ldz]
   float* dbp;    // [2 * tiles of rows][ldz]
-  int splits, dh_tile, dw_tile;
+  int splits, dz_tile, dh_tile, dw_tile;
   float* slab;   // [splits][N][K8]
 };
 
 // How the products of a shape run (tiles, k splits of the hidden gradient); x.piece is set.
 void lce_plan(LceShape& s);
-void lce_plan_backward(LceShape& s, LceScratch& x);
+void lce_plan_backward(LceShape& s, LceScratch& x, bool bias);
 
 #define MIHVD_TRANSFORMER_DECLS                                                                                        \
   void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t hs0, int64_t hs1, const u16* w,      \
@@ -68,26 +68,33 @@ namespace f16 {
 MIHVD_TRANSFORMER_DECLS
 }
 
-// Newton-Schulz (newton_schulz.hip): one group of equally shaped matrices.
+// Newton-Schulz (newton_schulz.hip): matrices whose smaller sides are alike, padded to the products' k
+// tile of 64. X of each is held with the smaller side as rows: [planes][side][len], one matrix behind the
+// other.
 constexpr int NS_MAX = 32;
+struct NsMat {
+  const void* src;  // the matrix (orthogonalize) / gradient (Muon), [rows][cols]
+  void* dst;        // result / weight
+  float* mom;       // Muon: momentum
+  int rows, cols, len;
+  int64_t off;      // of X, in elements
+  float step;       // Muon: lr * scale
+};
 struct NsGroup {
-  int count, rows, cols;
-  int rp, cp, sp;  // rows, cols and the smaller of them, padded to the products' k tile of 64
-  int planes;                           // 1: fp16; 2: fp16 hi + lo
-  const void* src[NS_MAX];              // u (orthogonalize) / gradient (Muon)
-  void* dst[NS_MAX];                    // result / weight
-  float* mom[NS_MAX];                   // Muon: momentum
+  int count, side;
+  int planes;  // 1: fp16; 2: fp16 hi + lo
+  NsMat m[NS_MAX];
 };
 struct NsParams {
   int steps;
   float a, b, c, eps;
   int src_kind;  // 0 fp32, 1 bf16, 2 fp16
-  int muon;
-  float lr, momentum, decay, scale;  // p = p * decay - lr * scale * O
-  int nesterov;
+  int muon, nesterov;
+  float momentum, decay;  // p = p * decay - step * O
 };
 struct NsScratch {
-  u16 *x0, *x1, *gram, *poly;  // planes: [count][planes][...]
+  u16 *x0, *x1;       // X before and after a step
+  u16 *gram, *poly;   // [count][planes][side][side]
   float* partial;              // [count][NS_PART]
 };
 constexpr int NS_PART = 64;

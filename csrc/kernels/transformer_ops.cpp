@@ -220,11 +220,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   x.piece = (int)std::min<int64_t>(up8(V), std::max<int64_t>(256, DZ_BYTES / (2 * N) / 256 * 256));
   x.ldz = up8(x.piece);
   LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0};
-  lce_plan_backward(s, x);
+  lce_plan_backward(s, x, bias.has_value());
   at::Tensor dz = at::empty({N, x.ldz}, w.options()), dbp, slab;
   x.dz = m16(dz);
   if (bias) {
-    dbp = at::empty({2 * cdiv(N, s.tile), x.ldz}, f32);
+    dbp = at::empty({2 * cdiv(N, x.dz_tile), x.ldz}, f32);
     x.dbp = dbp.data_ptr<float>();
   }
   if (need_h) {
@@ -328,27 +328,37 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
 
 constexpr int64_t NS_ELEMS = int64_t(1) << 28;  // elements of X per launch group (bounds the workspace)
 
-void ns_group(NsGroup& g, NsParams& p, const at::TensorOptions& opt) {
-  const int64_t px = (int64_t)g.rp * g.cp, pa = (int64_t)g.sp * g.sp, k = (int64_t)g.count * g.planes;
-  const auto h = opt.dtype(at::kHalf);
-  at::Tensor x0 = at::empty({k * px}, h), x1, gram, poly;
-  if (p.steps > 0) {
-    gram = at::empty({k * pa}, h);
-    poly = at::empty({k * pa}, h);
-  }
-  if (p.steps > 1) x1 = at::empty({k * px}, h);
-  at::Tensor part = at::empty({g.count * NS_PART}, opt.dtype(at::kFloat));
-  ns_run(g, p, NsScratch{m16(x0), m16(x1), m16(gram), m16(poly), part.data_ptr<float>()}, cur_stream());
+inline int64_t up64(int64_t x) { return cdiv(x, 64) * 64; }
+
+// Adds a matrix to the group, unless it is full.
+bool ns_add(NsGroup& g, int64_t rows, int64_t cols, const void* src, void* dst, float* mom, float step) {
+  const int64_t len = up64(std::max(rows, cols)), side = up64(std::min(rows, cols));
+  const int64_t off = g.count ? g.m[g.count - 1].off + (int64_t)g.planes * g.side * g.m[g.count - 1].len : 0;
+  if (g.count && (g.count == NS_MAX || g.side != side || off / g.planes + side * len > NS_ELEMS)) return false;
+  g.side = (int)side;
+  g.m[g.count++] = NsMat{src, dst, mom, (int)rows, (int)cols, (int)len, off, step};
+  return true;
 }
 
-void ns_shape(NsGroup& g, int64_t rows, int64_t cols, bool split) {
+void ns_launch(NsGroup& g, const NsParams& p, const at::TensorOptions& opt) {
+  if (!g.count) return;
+  const NsMat& last = g.m[g.count - 1];
+  const int64_t all = last.off + (int64_t)g.planes * g.side * last.len;
+  const int64_t sq = (int64_t)g.count * g.planes * g.side * g.side;
+  const auto h = opt.dtype(at::kHalf);
+  at::Tensor x0 = at::empty({all}, h), x1, gram, poly;
+  if (p.steps > 0) {
+    gram = at::empty({sq}, h);
+    poly = at::empty({sq}, h);
+  }
+  if (p.steps > 1) x1 = at::empty({all}, h);
+  at::Tensor part = at::empty({g.count * NS_PART}, opt.dtype(at::kFloat));
+  ns_run(g, p, NsScratch{m16(x0), m16(x1), m16(gram), m16(poly), part.data_ptr<float>()}, cur_stream());
+  g.count = 0;
+}
+
+void ns_check_sides(int64_t rows, int64_t cols) {
   TORCH_CHECK_VALUE(rows <= MAX_LD && cols <= MAX_LD, "orthogonalize: sides above ", MAX_LD, " are not supported");
-  g.rows = (int)rows;
-  g.cols = (int)cols;
-  g.rp = (int)cdiv(rows, 64) * 64;
-  g.cp = (int)cdiv(cols, 64) * 64;
-  g.sp = std::min(g.rp, g.cp);
-  g.planes = split ? 2 : 1;
 }
 
 at::Tensor newton_schulz(const at::Tensor& x_in, int64_t steps, double a, double b, double c, double eps, bool split) {
@@ -364,18 +374,21 @@ at::Tensor newton_schulz(const at::Tensor& x_in, int64_t steps, double a, double
   p.steps = (int)steps;
   p.a = (float)a, p.b = (float)b, p.c = (float)c, p.eps = (float)eps;
   p.src_kind = ty == at::kFloat ? 0 : ty == at::kBFloat16 ? 1 : 2;
-  const int64_t B = x.size(0), n = x.size(1) * x.size(2), bytes = n * x.element_size();
-  const int64_t per = std::max<int64_t>(1, std::min<int64_t>(NS_MAX, NS_ELEMS / n));
-  for (int64_t i0 = 0; i0 < B; i0 += per) {
-    NsGroup g{};
-    g.count = (int)std::min(per, B - i0);
-    ns_shape(g, x.size(1), x.size(2), split);
-    for (int i = 0; i < g.count; ++i) {
-      g.src[i] = static_cast<const char*>(x.data_ptr()) + (i0 + i) * bytes;
-      g.dst[i] = static_cast<char*>(out.data_ptr()) + (i0 + i) * bytes;
+  const int64_t B = x.size(0), bytes = x.size(1) * x.size(2) * x.element_size();
+  ns_check_sides(x.size(1), x.size(2));
+  NsGroup g{};
+  g.planes = split ? 2 : 1;
+  for (int64_t i = 0; i < B; ++i) {
+    auto add = [&] {
+      return ns_add(g, x.size(1), x.size(2), static_cast<const char*>(x.data_ptr()) + i * bytes,
+                    static_cast<char*>(out.data_ptr()) + i * bytes, nullptr, 0.f);
+    };
+    if (!add()) {
+      ns_launch(g, p, x.options());
+      add();
     }
-    ns_group(g, p, x.options());
   }
+  ns_launch(g, p, x.options());
   return out;
 }
 
@@ -385,8 +398,8 @@ void muon_step(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vect
                int64_t scale_mode, bool split) {
   TORCH_CHECK_VALUE(ps.size() == gs.size() && ps.size() == ms.size(), "muon_step: list lengths");
   TORCH_CHECK_VALUE(steps >= 0 && steps <= 100, "muon_step: steps must be within 0..100");
-  // matrices of one shape run together
-  std::map<std::tuple<int, int64_t, int64_t>, std::vector<size_t>> groups;
+  // matrices whose smaller sides agree (padded) run together
+  std::map<std::tuple<int, int64_t>, std::vector<size_t>> groups;
   for (size_t i = 0; i < ps.size(); ++i) {
     TORCH_CHECK_VALUE(ps[i].dim() >= 2, "muon_step: parameters must be matrices");
     for (const at::Tensor* t : {&ps[i], &gs[i], &ms[i]})
@@ -394,34 +407,35 @@ void muon_step(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vect
                             t->sizes() == ps[i].sizes() && t->device() == ps[i].device(),
                         "muon_step: contiguous fp32 GPU tensors of equal shapes expected");
     if (ps[i].numel() == 0) continue;
-    const int64_t rows = ps[i].size(0);
-    groups[{(int)ps[i].get_device(), rows, ps[i].numel() / rows}].push_back(i);
+    const int64_t rows = ps[i].size(0), cols = ps[i].numel() / rows;
+    ns_check_sides(rows, cols);
+    groups[{(int)ps[i].get_device(), up64(std::min(rows, cols))}].push_back(i);
   }
+  NsParams p{};
+  p.steps = (int)steps;
+  p.a = (float)a, p.b = (float)b, p.c = (float)c, p.eps = (float)eps;
+  p.muon = 1;
+  p.momentum = (float)momentum, p.decay = (float)(1.0 - lr * weight_decay);
+  p.nesterov = nesterov;
   for (const auto& kv : groups) {
-    const int64_t rows = std::get<1>(kv.first), cols = std::get<2>(kv.first);
-    const auto& list = kv.second;
-    c10::DeviceGuard guard(ps[list[0]].device());
-    NsParams p{};
-    p.steps = (int)steps;
-    p.a = (float)a, p.b = (float)b, p.c = (float)c, p.eps = (float)eps;
-    p.muon = 1;
-    p.lr = (float)lr, p.momentum = (float)momentum, p.decay = (float)(1.0 - lr * weight_decay);
-    p.scale = scale_mode == 0 ? (float)std::sqrt(std::max(1.0, (double)rows / (double)cols))
-                              : (float)(0.2 * std::sqrt((double)std::max(rows, cols)));
-    p.nesterov = nesterov;
-    const size_t per = (size_t)std::max<int64_t>(1, std::min<int64_t>(NS_MAX, NS_ELEMS / (rows * cols)));
-    for (size_t i0 = 0; i0 < list.size(); i0 += per) {
-      NsGroup g{};
-      g.count = (int)std::min(per, list.size() - i0);
-      ns_shape(g, rows, cols, split);
-      for (int i = 0; i < g.count; ++i) {
-        const size_t k = list[i0 + i];
-        g.src[i] = gs[k].data_ptr<float>();
-        g.dst[i] = ps[k].data_ptr<float>();
-        g.mom[i] = ms[k].data_ptr<float>();
+    const at::TensorOptions opt = ps[kv.second[0]].options();
+    c10::DeviceGuard guard(opt.device());
+    NsGroup g{};
+    g.planes = split ? 2 : 1;
+    for (const size_t k : kv.second) {
+      const int64_t rows = ps[k].size(0), cols = ps[k].numel() / rows;
+      const double s = scale_mode == 0 ? std::sqrt(std::max(1.0, (double)rows / (double)cols))
+                                       : 0.2 * std::sqrt((double)std::max(rows, cols));
+      auto add = [&] {
+        return ns_add(g, rows, cols, gs[k].data_ptr<float>(), ps[k].data_ptr<float>(), ms[k].data_ptr<float>(),
+                      (float)(lr * s));
+      };
+      if (!add()) {
+        ns_launch(g, p, opt);
+        add();
       }
-      ns_group(g, p, ps[list[0]].options());
     }
+    ns_launch(g, p, opt);
   }
 }
 
