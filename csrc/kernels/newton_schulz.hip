@@ -1,6 +1,8 @@
 // Orthogonalising a matrix by Newton-Schulz steps, and the weight update made of it.
 //
-//   X = u / (|u|_F + eps);   per step  A = X X^T,  B = b A + c A A,  X <- a X + B X
+//   X = u / (|u|_F + eps);   per step  A = X X^T,  B = a I + b A + c A A,  X <- B X
+// (a X + (b A + c A A) X with the first term inside the product: X is read once a step, and B's entries
+// get smaller, hence their rounding: near singular values of one its diagonal is 0.7, not -2.7)
 // with the smaller side of the matrix as X's rows (a tall one is turned on the way in and out), so that
 // matrices of different lengths, wide or tall, run in one batch wherever their smaller sides agree.
 //
@@ -148,15 +150,15 @@ __global__ void __launch_bounds__(256) ns_scale(const NsGroup t, int muon, float
   }
 }
 
-// out planes [batch][planes][rows][ld] = alpha * acc + beta * in (planes of the same layout); symmetric
-// ones off the diagonal are stored a second time with rows and columns exchanged. N is a multiple of 64.
+// out planes [batch][planes][rows][ld] = alpha * acc (+ beta * in + diag on the diagonal, `in` being planes of
+// the same layout); symmetric ones off the diagonal are stored a second time with rows and columns exchanged. N is a multiple of 64.
 template <bool IN>
 struct EpiPlanes {
   u16* out;
   const u16* in;
   int64_t ld_, plane_;  // 0: a ragged batch's
   int planes, sym;
-  float alpha, beta;
+  float alpha, beta, diag;
   template <int NI, int MI>
   struct Pre {};
   template <int NI, int MI>
@@ -212,6 +214,14 @@ struct EpiPlanes {
           st.turn();
         }
         if (j + 1 < MI) fetch(j + 1);
+        const int d = c.m0 + j * 16 + (c.lane & 15) - c.n0 - 4 * (c.lane >> 4);  // the diagonal's column here
+        if (d >= 0 && d < NI * 16 && (d & 15) < 4) {
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (d == i * 16 + k) acc[i][j][k] += diag;
+        }
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) st.put(i, pack4bf(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]));
@@ -250,8 +260,9 @@ struct EpiPlanes {
   __device__ __forceinline__ static float rest(float v) { return v - bf2f(f2bf(v)); }
 };
 
-// The last step: v = alpha * acc + beta * X, unscaled, into the result (KIND 0 fp32, 1 bf16, 2 fp16) or the
-// weight (3: w = w * decay - step * v); column n of X is a row of a tall matrix.
+// The last step: v = alpha * acc, unscaled, into the result (KIND 0 fp32, 1 bf16, 2 fp16) or the weight
+// (3: w = w * decay - step * v). Column n of X is a row of a tall matrix: those are turned in LDS, eight
+// at a time, so that both kinds write whole rows.
 struct NsOut {
   void* dst[NS_MAX];
   int rows[NS_MAX], cols[NS_MAX];
@@ -268,68 +279,80 @@ __device__ __forceinline__ void put_out(void* o, int64_t at, float v, float deca
     static_cast<u16*>(o)[at] = KIND == 1 ? __builtin_bit_cast(u16, (__bf16)v) : f2bf(v);
   }
 }
+// four in a row, of which `n` exist
+template <int KIND>
+__device__ __forceinline__ void put4(void* o, int64_t at, f32x4 v, int n, bool vec, float decay, float step) {
+  if (vec && n >= 4) {
+    if constexpr (KIND == 0 || KIND == 3) {
+      f32x4* w = reinterpret_cast<f32x4*>(static_cast<float*>(o) + at);
+      if constexpr (KIND == 3) {
+        const f32x4 r = *w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(-step, v[k], r[k] * decay);
+      }
+      *w = v;
+    } else {
+      uint32_t r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[k] = KIND == 1 ? __builtin_bit_cast(u16, (__bf16)v[k]) : f2bf(v[k]);
+      *reinterpret_cast<uint2*>(static_cast<u16*>(o) + at) = make_uint2(r[0] | (r[1] << 16), r[2] | (r[3] << 16));
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < n) put_out<KIND>(o, at + k, v[k], decay, step);
+}
 template <int KIND>
 struct EpiFinal {
   NsOut out;
-  const u16* in;
-  int planes;
-  float alpha, beta, decay;
+  float alpha, decay;
   template <int NI, int MI>
   struct Pre {};
   template <int NI, int MI>
   __device__ __forceinline__ void load(const g16::Ctx&, Pre<NI, MI>&) const {}
   template <int NI, int MI>
   __device__ __forceinline__ void run(const g16::Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
-    const int64_t ld = c.len, plane = (int64_t)c.M * c.len;
-    const u16* q = in + c.off;
     void* o = out.dst[c.batch];
     const int rows = out.rows[c.batch], cols = out.cols[c.batch];
     const float step = out.step[c.batch];
-    const bool tall = rows > cols, vec = cols % 4 == 0 && ((uintptr_t)o & 15) == 0;
-    const int side = min(rows, cols), len = max(rows, cols);
-    g16::unroll<MI>([&](auto J) {
-      constexpr int j = J.value;
-      g16::pin(acc, j);
-      const int m = c.m0 + j * 16 + (c.lane & 15);
-      if (m >= side) return;
+    const bool vec = cols % 4 == 0 && ((uintptr_t)o & 15) == 0;
+    if (rows <= cols) {
+      g16::unroll<MI>([&](auto J) {
+        constexpr int j = J.value;
+        g16::pin(acc, j);
+        const int m = c.m0 + j * 16 + (c.lane & 15);
+        if (m >= rows) return;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
-        if (n >= len) continue;
-        const uint2 h = *reinterpret_cast<const uint2*>(q + (int64_t)m * ld + n);
-        uint2 l = make_uint2(0, 0);
-        if (planes == 2) l = *reinterpret_cast<const uint2*>(q + plane + (int64_t)m * ld + n);
-        const float x[4] = {bf2f((u16)h.x) + bf2f((u16)l.x), bf2f((u16)(h.x >> 16)) + bf2f((u16)(l.x >> 16)),
-                            bf2f((u16)h.y) + bf2f((u16)l.y), bf2f((u16)(h.y >> 16)) + bf2f((u16)(l.y >> 16))};
-        f32x4 v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = fmaf(beta, x[k], alpha * acc[i][j][k]);
-        if (tall) {  // 16 lanes write 16 neighbours of one row
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n + k < len) put_out<KIND>(o, (int64_t)(n + k) * cols + m, v[k], decay, step);
-        } else if (vec && (KIND == 0 || KIND == 3)) {
-          f32x4* w = reinterpret_cast<f32x4*>(static_cast<float*>(o) + (int64_t)m * cols + n);
-          if constexpr (KIND == 3) {
-            f32x4 r = *w;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) r[k] = fmaf(-step, v[k], r[k] * decay);
-            *w = r;
-          } else {
-            *w = v;
-          }
-        } else if (vec) {
-          uint32_t r[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) r[k] = KIND == 1 ? __builtin_bit_cast(u16, (__bf16)v[k]) : f2bf(v[k]);
-          *reinterpret_cast<uint2*>(static_cast<u16*>(o) + (int64_t)m * cols + n) = make_uint2(r[0] | (r[1] << 16), r[2] | (r[3] << 16));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n + k < len) put_out<KIND>(o, (int64_t)m * cols + n + k, v[k], decay, step);
+        for (int i = 0; i < NI; ++i) {
+          const int n = c.n0 + i * 16 + 4 * (c.lane >> 4);
+          put4<KIND>(o, (int64_t)m * cols + n, acc[i][j] * alpha, cols - n, vec, decay, step);
         }
+      });
+      return;
+    }
+    constexpr int RS = MI * 16 + 4, CH = MI * 4, GT = 8 * CH / 64;  // floats a row, float4 a row, float4 a lane
+    static_assert(8 * RS * 4 <= 16 * (NI * 16 + 8) * 2, "the stage holds eight rows");
+    float* sh = reinterpret_cast<float*>(c.stage);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            sh[((c.lane >> 4) * 2 + k) * RS + j * 16 + (c.lane & 15)] = acc[i][j][half * 2 + k] * alpha;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+          const int q = c.lane + g * 64, r = q / CH, m = (q % CH) * 4;
+          const f32x4 v = *reinterpret_cast<const f32x4*>(sh + r * RS + m);
+          const int n = c.n0 + i * 16 + (r >> 1) * 4 + half * 2 + (r & 1);
+          if (n < rows) put4<KIND>(o, (int64_t)n * cols + c.m0 + m, v, cols - c.m0 - m, vec, decay, step);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-    });
   }
 };
 
@@ -410,6 +433,7 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
   const int t_gram = plan(sp, sp, total / g.count, nseg, g.count, true, false).tile;
   const int t_poly = plan(sp, sp, sp, nseg, g.count, true, false).tile;
   const int t_upd = plan(sp, total, sp, nseg, 1, false, false).tile;
+  const int t_fin = t_upd == T256 ? T128 : t_upd;  // (turning 256 accumulators does not fit the registers)
   u16 *x = sc.x0, *y = sc.x1;
   for (int it = 0; it < p.steps; ++it) {
     Args a;
@@ -419,19 +443,19 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     a.M = a.N = g.side;
     a.m = ragged_side(x, g.side, false);
     a.n = ragged_side(x, g.side, true);
-    launch<KC, KC, false, 1>(t_gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f}, st, rg);
+    launch<KC, KC, false, 1>(t_gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f, 0.f}, st, rg);
     a.K = g.side;
     a.m = square_side(sc.gram, sp, g.planes, false);
     a.n = square_side(sc.gram, sp, g.planes, true);
-    launch<KC, KC>(t_poly, a, EpiPlanes<true>{sc.poly, sc.gram, sp, pa, g.planes, 1, p.c * INV_S, p.b}, st);
+    launch<KC, KC>(t_poly, a, EpiPlanes<true>{sc.poly, sc.gram, sp, pa, g.planes, 1, p.c * INV_S, p.b, p.a * S}, st);
     a.sym = 0;
     a.m = square_side(sc.poly, sp, g.planes, false);
     a.n = ragged_side(x, 0, true);
     if (it + 1 < p.steps) {
-      launch<KC, KS, false, 2>(t_upd, a, EpiPlanes<true>{y, x, 0, 0, g.planes, 0, INV_S, p.a}, st, rg);
+      launch<KC, KS, false, 2>(t_upd, a, EpiPlanes<false>{y, nullptr, 0, 0, g.planes, 0, INV_S, 0.f, 0.f}, st, rg);
     } else {
       auto fin = [&](auto K) {
-        launch<KC, KS, false, 2>(t_upd, a, EpiFinal<K.value>{out, x, g.planes, INV_S * INV_S, p.a * INV_S, p.decay}, st, rg);
+        launch<KC, KS, false, 2>(t_fin, a, EpiFinal<K.value>{out, INV_S * INV_S, p.decay}, st, rg);
       };
       if (p.muon) fin(std::integral_constant<int, 3>{});
       else with_kind(p, fin);
