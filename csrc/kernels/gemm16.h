@@ -7,7 +7,7 @@
 // Each side is stored K-contiguous ("KC", [row][k]) or K-strided ("KS", [k][row]), so no operand is
 // ever transposed in memory: forward products are KC x KC, products with a weight along its other
 // axis KC x KS, weight gradients KS x KS. Segments concatenate products along k (the two halves of
-// a gated input gradient; the three products hi*hi + hi*lo + lo*hi of split fp32 values).
+// a gated input gradient).
 //
 // The n side feeds the MFMA's A operand and the m side its B operand, so a lane's four accumulators
 // are four consecutive n of one m (v_mfma_f32_16x16x32: C[4*(l>>4)+i][l&15]): packed 8-byte stores
@@ -36,16 +36,15 @@ constexpr int BK = 64;
 static __device__ __attribute__((aligned(16))) const unsigned zeros16[4] = {0, 0, 0, 0};
 
 struct Side {
-  const u16* p[3] = {nullptr, nullptr, nullptr};  // one base per segment
+  const u16* p[2] = {nullptr, nullptr};           // one base per segment, or plane
   const u16* alt = nullptr;                       // DUAL: the second matrix of interleaved rows
-  int pl[3] = {0, 0, 0};                          // RAG: plane per segment
   int64_t ld = 0;                                 // elements between rows (KC) / between k (KS)
   int64_t bs = 0;                                 // elements between batch entries
   int ext = 0;                                    // rows (KC); storage extent, a multiple of 8 (KS)
 };
 
 // A ragged batch (template parameter RAG): entry b is a matrix of `rows` x len[b], in planes of that size
-// one behind the other from element off[b] on; a side's segment s reads plane pl[s].
+// one behind the other from element off[b] on.
 //   RAG 1: both sides are such matrices along k (K = len[b]);  RAG 2: the n side is one, K-strided (N = len[b])
 constexpr int RAG_MAX = 32;
 struct Ragged {
@@ -320,15 +319,16 @@ struct Frags {
     const int col = w * (COUNT / 2) * 16 + (i % (COUNT / 2)) * 16;
     return ((col >> 6) << 7) + (i >= COUNT / 2 ? 64 : 0) + (col & 63);
   }
-  __device__ __forceinline__ bf16x8 get(int i, int kk) const {
+  // pl: the image `pl` rows-images further on (PL 2: the low halves)
+  __device__ __forceinline__ bf16x8 get(int i, int kk, int pl = 0) const {
     typedef __attribute__((address_space(3))) const bf16x8 LV;
     if constexpr (LAYOUT == KC) {
       // DUAL: a wave's columns lie in one block of 64, so its rows differ from row_dual(w, 0) by constants
       const uint32_t o = DUAL ? (uint32_t)((i % (COUNT / 2)) * 16 + (i >= COUNT / 2 ? 64 : 0)) * 128u : (uint32_t)i * 2048u;
-      return *(LV*)(uintptr_t)(at[kk] + o);
+      return *(LV*)(uintptr_t)(at[kk] + o + (uint32_t)pl * (R * 128u));
     } else {
       typedef __attribute__((address_space(3))) short4_t TV;
-      const uint32_t p = at[i] + (uint32_t)kk * (32u * R * 2u);
+      const uint32_t p = at[i] + (uint32_t)kk * (32u * R * 2u) + (uint32_t)pl * (R * 128u);
       const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TV*)(uintptr_t)p);
       const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TV*)(uintptr_t)(p + 8u * R));
       typedef short short8_t __attribute__((ext_vector_type(8)));
@@ -357,7 +357,8 @@ __device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tile
   const int nb = RAG == 2 ? g.start[g.count] : tiles * a.splits * a.batch, x = blockIdx.x & 7;
   const int q = nb >> 3, r = nb & 7;
   if (l >= q + (x < r ? 1 : 0)) return false;
-  int pos = x * q + min(x, r) + l, mt, nt, batch = 0, split = 0, tiles_n = a.tiles_n;
+  // (an XCD's run goes up through the entries: the search starts where the last one ended)
+  int pos = x * q + min(x, r) + l, mt, nt, batch = RAG == 2 ? t.batch : 0, split = 0, tiles_n = a.tiles_n;
   t.K = K;
   t.N = a.N;
   if constexpr (RAG == 2) {
@@ -409,11 +410,15 @@ __device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tile
 // The stream of k tiles runs on from one output tile to the next: while the epilogue works, the next
 // output tile's first two k tiles are already in LDS and its first fragments in registers, and the
 // epilogue's stores drain under the next products.
-template <int LM, int LN, int TM, int TN, int S, bool DUAL, int RAG, class Epi>
-__global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
+//
+// PL 2: both sides are split values, in two planes (segments 0 and 1 of a side are its high and low
+// halves), and the three products hi hi + hi lo + lo hi run on one staging of the four images: a third
+// of the k tiles that three segments would take, two thirds of their LDS reads.
+template <int LM, int LN, int TM, int TN, int S, int PL, bool DUAL, int RAG, class Epi>
+__global__ void __launch_bounds__(256, TM * TN > 128 * 128 || PL == 2 ? 1 : 2)
     gemm16_kernel(const Args a, const typename std::conditional<RAG != 0, Ragged, int>::type rag, const Epi epi) {
   constexpr int WM = 2, WN = 2, NT = 64 * WM * WN, WTM = TM / WM, WTN = TN / WN, MI = WTM / 16, NI = WTN / 16;
-  constexpr int BUF = (TM + TN) * BK;  // elements of one buffer
+  constexpr int BUF = PL * (TM + TN) * BK;  // elements of one buffer
   constexpr bool BIG = TM * TN > 128 * 128;
   constexpr int STAGE = 16 * (WTN + 8);  // a wave's RowStage
   __shared__ __attribute__((aligned(128))) u16 lds[S * BUF + WM * WN * STAGE];
@@ -426,6 +431,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
   const int hops = (int)(gridDim.x >> 3) + ((blockIdx.x & 7) < (gridDim.x & 7) ? 1 : 0);
   int l_mul = blockIdx.x >> 3, l_cpy = l_mul;  // the tile being multiplied, the tile being copied
   Tile cur, nxt;
+  cur.batch = 0;
   if (!tile_at<RAG, TN>(a, g, tiles_m, K, l_mul, cur)) return;
   const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
   const int wm = wave % WM, wn = wave / WM;
@@ -437,23 +443,25 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
   // The next k tile to copy: `run` whole ones lie ahead at (pm, pn), one step apart; then, with run == 0,
   // what `next_run` finds: a partial tile (krem > 0 of its k positions, none for a split without any k),
   // the next segment, the next output tile, or the end.
-  const char *pm = nullptr, *pn = nullptr, *pa = nullptr;
+  const char *pm = nullptr, *pn = nullptr, *pa = nullptr, *pm2 = nullptr, *pn2 = nullptr;
   int run = 0, seg = 0, krem = 0;
   bool partial = false, more = true;
   auto locate = [&](int kp) {
     const int x0m = nxt.mt * TM, x0n = nxt.nt * (DUAL ? TN / 2 : TN);
     const int64_t len = RAG ? g.len[nxt.batch] : 0, plane = RAG ? len * g.rows : 0;
     const int64_t ldm = RAG == 1 ? len : a.m.ld, ldn = RAG ? len : a.n.ld;
-    int64_t tm0 = (RAG == 1 ? g.off[nxt.batch] : a.m.bs * nxt.batch) + (LM == KC ? (int64_t)x0m * ldm : x0m);
-    int64_t tn0 = (RAG ? g.off[nxt.batch] : a.n.bs * nxt.batch) + (LN == KC ? (int64_t)x0n * ldn : x0n);
-    if constexpr (RAG == 1) tm0 += plane * (seg == 0 ? a.m.pl[0] : seg == 1 ? a.m.pl[1] : a.m.pl[2]);
-    if constexpr (RAG != 0) tn0 += plane * (seg == 0 ? a.n.pl[0] : seg == 1 ? a.n.pl[1] : a.n.pl[2]);
-    const u16* bm = seg == 0 ? a.m.p[0] : seg == 1 ? a.m.p[1] : a.m.p[2];
-    const u16* bn = seg == 0 ? a.n.p[0] : seg == 1 ? a.n.p[1] : a.n.p[2];
+    const int64_t tm0 = (RAG == 1 ? g.off[nxt.batch] : a.m.bs * nxt.batch) + (LM == KC ? (int64_t)x0m * ldm : x0m);
+    const int64_t tn0 = (RAG ? g.off[nxt.batch] : a.n.bs * nxt.batch) + (LN == KC ? (int64_t)x0n * ldn : x0n);
+    const u16* bm = seg == 0 ? a.m.p[0] : a.m.p[1];
+    const u16* bn = seg == 0 ? a.n.p[0] : a.n.p[1];
     if constexpr (RAG == 2) stepn = LN == KC ? BK : BK * len;
     pm = (const char*)(bm + tm0 + kp * stepm);
     pn = (const char*)(bn + tn0 + kp * stepn);
     if (DUAL) pa = (const char*)(a.n.alt + tn0 + kp * stepn);
+    if constexpr (PL == 2) {
+      pm2 = RAG == 1 ? pm + plane * 2 : (const char*)(a.m.p[1] + tm0 + kp * stepm);
+      pn2 = RAG ? pn + plane * 2 : (const char*)(a.n.p[1] + tn0 + kp * stepn);
+    }
     const int whole = nxt.K / BK - kp;  // whole tiles of this segment from here on
     run = min(whole, nxt.end - nxt.it);
     partial = run == 0;
@@ -482,21 +490,33 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
   };
   const uint32_t ldsb = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u16*)lds;
   const uint32_t lds0 = ldsb + (uint32_t)wave * 1024u;
+  auto step_on = [&](int64_t mask) {
+    pm += (stepm * 2) & mask;
+    pn += (stepn * 2) & mask;
+    if (DUAL) pa += (stepn * 2) & mask;
+    if (PL == 2) {
+      pm2 += (stepm * 2) & mask;
+      pn2 += (stepn * 2) & mask;
+    }
+  };
+  constexpr uint32_t IMG_M = TM * BK * 2, IMG_N = TN * BK * 2;  // bytes of an image
   // the next k tile as a whole, ahead of the loop or where the run ends
   auto issue = [&](uint32_t l) -> bool {
     if (run == 0 && !partial) next_run();
     if (run > 0) {
       sm.all(pm, nullptr, l);
-      sn.all(pn, pa, l + TM * BK * 2);
-      pm += stepm * 2;
-      pn += stepn * 2;
-      if (DUAL) pa += stepn * 2;
+      if (PL == 2) sm.all(pm2, nullptr, l + IMG_M);
+      sn.all(pn, pa, l + PL * IMG_M);
+      if (PL == 2) sn.all(pn2, nullptr, l + PL * IMG_M + IMG_N);
+      step_on(-1);
       --run;
       return true;
     }
     if (partial) {
       sm.tail(pm, nullptr, l, t, krem);
-      sn.tail(pn, pa, l + TM * BK * 2, t, krem);
+      if (PL == 2) sm.tail(pm2, nullptr, l + IMG_M, t, krem);
+      sn.tail(pn, pa, l + PL * IMG_M, t, krem);
+      if (PL == 2) sn.tail(pn2, nullptr, l + PL * IMG_M + IMG_N, t, krem);
       partial = false;
       return true;
     }
@@ -505,7 +525,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
   Frags<LM, TM, MI, false> gm;
   Frags<LN, TN, NI, DUAL> gn;
   gm.init(ldsb, wm, lane);
-  gn.init(ldsb + TM * BK * 2, wn, lane);
+  gn.init(ldsb + PL * IMG_M, wn, lane);
 
   f32x4 acc[NI][MI];
   auto clear = [&]() {
@@ -516,11 +536,18 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
   };
   clear();
 
-  constexpr int NF = MI + NI, NQ = sm.J + sn.J, NX = NI * MI;
-  // fragments read before MFMA x of a half tile: all within its first three quarters, so that none is
-  // waited for at the barrier
-  auto ahead = [](int x) constexpr { return x * NF * 4 / (3 * NX) < NF ? x * NF * 4 / (3 * NX) : NF; };
-  bf16x8 fm[2][MI], fn[2][NI];
+  // A half tile: B4 blocks of four MFMAs (block b: accumulators from 4 (b / PR) on, product b % PR), among
+  // which go the next half's NF fragment reads, all within the first three quarters so that none is
+  // waited for at the barrier, and (second half) the NQ copies.
+  constexpr int JM = decltype(sm)::J, JN = decltype(sn)::J, NF = PL * (MI + NI), NQ = PL * (JM + JN), NX = NI * MI;
+  constexpr int PR = PL == 2 ? 3 : 1, B4 = NX / 4 * PR;
+  auto ahead = [](int b) constexpr { return b * NF * 4 / (3 * B4) < NF ? b * NF * 4 / (3 * B4) : NF; };
+  bf16x8 fm[2][PL][MI], fn[2][PL][NI];
+  auto read = [&](int f, int set, int kk) {
+    const int pl = f / (MI + NI), r = f % (MI + NI);
+    if (r < MI) fm[set][pl][r < MI ? r : 0] = gm.get(r, kk, pl);
+    else fn[set][pl][r < MI ? 0 : r - MI] = gn.get(r - MI, kk, pl);
+  };
   // the copies of the last S - 2 tiles may be on their way across a barrier; not once a tile was not
   // issued (the end is near: then everything has to land)
   bool flowing = true;
@@ -530,62 +557,63 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
   if (flowing) tile_barrier_but<(S - 1) * NQ>();
   else tile_barrier();
 #pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
-    else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
-  }
+  for (int f = 0; f < NF; ++f) read(f, 0, 0);
   uint32_t lq = lds0;  // the buffer being read, where the next copies go
   const uint32_t lds_last = lds0 + (S - 1) * (BUF * 2);
   int landed = 0;      // that many tiles were waited for ahead of an epilogue
 
   auto first_half = [&](uint32_t hop) {
-    unroll<NX / 4>([&](auto B) {
-      constexpr int x = B.value * 4, i = x / MI, j = x % MI;
+    unroll<B4>([&](auto B) {
+      constexpr int b = B.value, x = b / PR * 4, i = x / MI, j = x % MI, pn_ = b % PR == 1 ? 1 : 0, pm_ = b % PR == 2 ? 1 : 0;
 #pragma unroll
-      for (int f = ahead(x); f < ahead(x + 4); ++f) {
-        if (f < MI) fm[1][f < MI ? f : 0] = gm.get(f, 1);
-        else fn[1][f < MI ? 0 : f - MI] = gn.get(f - MI, 1);
-      }
-      if constexpr (MI == 2) {
-        mfma2x2(acc[0][0], acc[0][1], acc[1][0], acc[1][1], fn[0][0], fn[0][1], fm[0][0], fm[0][1]);
-      } else {
-        mfma4<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[0][i], fm[0][j], fm[0][j + 1], fm[0][j + 2],
-                   fm[0][j + 3]);
-      }
-      if (x + 8 == NX || NX == 4) {
+      for (int f = ahead(b); f < ahead(b + 1); ++f) read(f, 1, 1);
+      if constexpr (MI == 2)
+        mfma2x2(acc[0][0], acc[0][1], acc[1][0], acc[1][1], fn[0][pn_][0], fn[0][pn_][1], fm[0][pm_][0], fm[0][pm_][1]);
+      else
+        mfma4<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[0][pn_][i], fm[0][pm_][j], fm[0][pm_][j + 1],
+                   fm[0][pm_][j + 2], fm[0][pm_][j + 3]);
+      if constexpr (ahead(b + 1) == NF && (b == 0 || ahead(b) < NF)) {  // the last read of this tile is out
         gm.move(hop);
         gn.move(hop);
       }
     });
   };
-  // the next k tile's copies between the MFMAs
+  // with the next k tile's copies between the MFMAs
   auto second_half = [&](uint64_t live) {
-    unroll<NX / 4>([&](auto B) {
-      constexpr int x = B.value * 4, i = x / MI, j = x % MI;
+    unroll<B4>([&](auto B) {
+      constexpr int b = B.value, x = b / PR * 4, i = x / MI, j = x % MI, pn_ = b % PR == 1 ? 1 : 0, pm_ = b % PR == 2 ? 1 : 0;
       // the next tile's first fragments (after the last tile: not used)
 #pragma unroll
-      for (int f = ahead(x); f < ahead(x + 4); ++f) {
-        if (f < MI) fm[0][f < MI ? f : 0] = gm.get(f, 0);
-        else fn[0][f < MI ? 0 : f - MI] = gn.get(f - MI, 0);
-      }
-      constexpr int JM = decltype(sm)::J;
-      auto lds_at = [](int q) constexpr { return q < JM ? q * NT * 16 : TM * BK * 2 + (q - JM) * NT * 16; };
-      auto off_at = [&](int q) { return q < JM ? sm.off[q < JM ? q : 0] : sn.off[q < JM ? 0 : q - JM]; };
-      auto base_at = [&](int q) { return q < JM ? pm : sn.is_alt(q < JM ? 0 : q - JM) ? pa : pn; };
+      for (int f = ahead(b); f < ahead(b + 1); ++f) read(f, 0, 0);
+      // copy q: m (high, low), then n (high, low)
+      auto lds_at = [](int q) constexpr {
+        return q < PL * JM ? (q / JM) * (int)IMG_M + q % JM * NT * 16
+                           : PL * (int)IMG_M + (q - PL * JM) / JN * (int)IMG_N + (q - PL * JM) % JN * NT * 16;
+      };
+      auto off_at = [&](int q) { return q < PL * JM ? sm.off[q % JM] : sn.off[(q - PL * JM < 0 ? 0 : q - PL * JM) % JN]; };
+      auto base_at = [&](int q) {
+        if (q < PL * JM) return q / JM ? pm2 : pm;
+        const int r = q - PL * JM;
+        return r / JN ? pn2 : sn.is_alt(r % JN) ? pa : pn;
+      };
+      constexpr int q0 = b * NQ / B4, q1 = (b + 1) * NQ / B4;
       if constexpr (MI == 2) {
-        mfma2x2(acc[0][0], acc[0][1], acc[1][0], acc[1][1], fn[1][0], fn[1][1], fm[1][0], fm[1][1]);
+        mfma2x2(acc[0][0], acc[0][1], acc[1][0], acc[1][1], fn[1][pn_][0], fn[1][pn_][1], fm[1][pm_][0], fm[1][pm_][1]);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) dma16_if(base_at(q), off_at(q), lq + lds_at(q), live);
+        for (int q = q0; q < q1; ++q) dma16_if(base_at(q), off_at(q), lq + lds_at(q), live);
+      } else if constexpr (q1 == q0) {
+        mfma4<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][pn_][i], fm[1][pm_][j], fm[1][pm_][j + 1],
+                   fm[1][pm_][j + 2], fm[1][pm_][j + 3]);
+      } else if constexpr (q1 == q0 + 1) {
+        constexpr int at1 = lds_at(q0);
+        mfma4_copy<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][pn_][i], fm[1][pm_][j],
+                        fm[1][pm_][j + 1], fm[1][pm_][j + 2], fm[1][pm_][j + 3], lq, live, at1, off_at(q0), base_at(q0));
       } else {
-        constexpr int PER = NQ * 4 / NX, q = x * NQ / NX, q2 = q + PER - 1;  // copies among four MFMAs
-        static_assert(PER == 1 || PER == 2, "copies per four MFMAs");
-        constexpr int at1 = lds_at(q), at2 = lds_at(q2);
-        if constexpr (PER == 1)
-          mfma4_copy<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
-                          fm[1][j + 2], fm[1][j + 3], lq, live, at1, off_at(q), base_at(q));
-        else
-          mfma4_copy2<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][i], fm[1][j], fm[1][j + 1],
-                           fm[1][j + 2], fm[1][j + 3], lq, live, at1, off_at(q), base_at(q), at2, off_at(q2), base_at(q2));
+        static_assert(q1 == q0 + 2, "copies among four MFMAs");
+        constexpr int at1 = lds_at(q0), at2 = lds_at(q0 + 1);
+        mfma4_copy2<BIG>(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3], fn[1][pn_][i], fm[1][pm_][j],
+                         fm[1][pm_][j + 1], fm[1][pm_][j + 2], fm[1][pm_][j + 3], lq, live, at1, off_at(q0), base_at(q0), at2,
+                         off_at(q0 + 1), base_at(q0 + 1));
       }
     });
   };
@@ -608,9 +636,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2)
       second_half(live);
       lq += hop;
       run += go;
-      pm += (stepm * 2) & (int64_t)go;
-      pn += (stepn * 2) & (int64_t)go;
-      if (DUAL) pa += (stepn * 2) & (int64_t)go;
+      step_on(go);
     }
     Ctx c;
     c.m0 = cur.mt * TM + wm * WTM;
@@ -655,7 +681,7 @@ inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 // the copies' latency.
 enum { T64 = 64, T128 = 128, T256 = 256 };
 
-template <int LM, int LN, int T, int S, bool DUAL, int RAG, class Epi>
+template <int LM, int LN, int T, int S, bool DUAL, int RAG, int PL = 1, class Epi>
 void launch_tile(Args a, Ragged g, const Epi& e, hipStream_t stream) {
   a.tiles_m = cdiv(a.M, T);
   a.tiles_n = cdiv(a.N, DUAL ? T / 2 : T);
@@ -669,11 +695,11 @@ void launch_tile(Args a, Ragged g, const Epi& e, hipStream_t stream) {
     }
     g.start[g.count] = (int)tiles;
   }
-  const int64_t slots = (int64_t)device_cu_count() * (T > 128 ? 1 : 2);  // resident blocks
+  const int64_t slots = (int64_t)device_cu_count() * (T > 128 || PL == 2 ? 1 : 2);  // resident blocks
   const int64_t blocks = std::min<int64_t>(tiles, slots);
   if (blocks <= 0) return;
-  if constexpr (RAG != 0) gemm16_kernel<LM, LN, T, T, S, DUAL, RAG, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, g, e);
-  else gemm16_kernel<LM, LN, T, T, S, DUAL, 0, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, 0, e);
+  if constexpr (RAG != 0) gemm16_kernel<LM, LN, T, T, S, PL, DUAL, RAG, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, g, e);
+  else gemm16_kernel<LM, LN, T, T, S, PL, DUAL, 0, Epi><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, 0, e);
 }
 
 template <int LM, int LN, bool DUAL = false, int RAG = 0, class Epi>
@@ -681,6 +707,27 @@ void launch(int tile, const Args& a, const Epi& e, hipStream_t stream, const Rag
   if (tile == T256) launch_tile<LM, LN, 256, 2, DUAL, RAG>(a, g, e, stream);
   else if (DUAL || tile == T128) launch_tile<LM, LN, 128, 2, DUAL, RAG>(a, g, e, stream);
   else if constexpr (!DUAL) launch_tile<LM, LN, 64, 4, false, RAG>(a, g, e, stream);
+}
+
+// without 256x256 tiles: epilogues that need more registers than those leave
+template <int LM, int LN, int RAG = 0, class Epi>
+void launch_small(int tile, const Args& a, const Epi& e, hipStream_t stream, const Ragged& g = Ragged()) {
+  if (tile == T64) launch_tile<LM, LN, 64, 4, false, RAG>(a, g, e, stream);
+  else launch_tile<LM, LN, 128, 2, false, RAG>(a, g, e, stream);
+}
+
+// Split values (PL 2): one block a CU at either tile. A k tile, with its three products, takes about 0.85 us
+// at 128x128 and 0.42 at 64x64.
+inline int plan_split(int64_t tiles128, int64_t tiles64, int64_t K) {
+  const int cus = device_cu_count();
+  const double kt = cdiv(K, BK);
+  const double t128 = cdiv(tiles128, cus) * (kt * 0.85 + 7.0), t64 = cdiv(tiles64, cus) * (kt * 0.42 + 3.0);
+  return t64 < t128 ? T64 : T128;
+}
+template <int LM, int LN, int RAG = 0, class Epi>
+void launch_split(int tile, const Args& a, const Epi& e, hipStream_t stream, const Ragged& g = Ragged()) {
+  if (tile == T64) launch_tile<LM, LN, 64, 4, false, RAG, 2>(a, g, e, stream);
+  else launch_tile<LM, LN, 128, 2, false, RAG, 2>(a, g, e, stream);
 }
 
 // How to run a product: the tile and the k splits with the least estimated time, in us. Measured on

@@ -323,12 +323,8 @@ __global__ void __launch_bounds__(256) lce_dh(const float* __restrict__ slab, in
 
 template <bool BIAS, class Epi>
 void dz_launch(int tile, const g16::Args& a, const Epi& e, hipStream_t st) {
-  if constexpr (BIAS) {
-    if (tile == g16::T128) g16::launch_tile<g16::KC, g16::KC, 128, 2, false, 0>(a, g16::Ragged(), e, st);
-    else g16::launch_tile<g16::KC, g16::KC, 64, 4, false, 0>(a, g16::Ragged(), e, st);
-  } else {
-    g16::launch<g16::KC, g16::KC>(tile, a, e, st);
-  }
+  if constexpr (BIAS) g16::launch_small<g16::KC, g16::KC>(tile, a, e, st);
+  else g16::launch<g16::KC, g16::KC>(tile, a, e, st);
 }
 
 }  // namespace

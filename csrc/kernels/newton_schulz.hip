@@ -8,8 +8,8 @@
 //
 // X, A and B are bounded (singular values stay below ~1.3), so they are held in fp16 scaled by 2^12:
 // the MFMA rate of bf16 with three more bits. fp32 values are held as two fp16 planes hi + lo (22
-// bits) and multiplied as hi hi + hi lo + lo hi, three k segments of one product; the dropped lo lo
-// is below 2^-22. A and B are symmetric: only tiles on and above the diagonal are computed, and
+// bits) and multiplied as hi hi + hi lo + lo hi in one pass over both planes; the dropped lo lo is below
+// 2^-22. A and B are symmetric: only tiles on and above the diagonal are computed, and
 // stored twice.
 //
 // Elements below 2^-26 of the norm lose relative precision in the scaled planes (fp16's smallest
@@ -370,25 +370,28 @@ __global__ void __launch_bounds__(256) ns_copy_out(const NsGroup t, const u16* _
   }
 }
 
-g16::Side square_side(const u16* x, int64_t side, int planes, bool second) {
-  // segments hi hi, hi lo, lo hi
+g16::Side square_side(const u16* x, int64_t side, int planes) {
   g16::Side s;
-  const int64_t plane = side * side;
   s.p[0] = x;
-  s.p[1] = second ? x + plane : x;
-  s.p[2] = second ? x : x + plane;
+  s.p[1] = x + side * side;
   s.ld = side;
-  s.bs = planes * plane;
+  s.bs = planes * side * side;
   s.ext = (int)side;
   return s;
 }
-g16::Side ragged_side(const u16* x, int side, bool second) {
+g16::Side ragged_side(const u16* x, int side) {
   g16::Side s;
-  s.p[0] = s.p[1] = s.p[2] = x;
-  s.pl[1] = second ? 1 : 0;
-  s.pl[2] = second ? 0 : 1;
+  s.p[0] = x;
   s.ext = side;
   return s;
+}
+
+// one product: fp16 (tiles by `plan`) or split (by `plan_split`)
+template <int LM, int LN, int RAG, bool SMALL, class Epi>
+void run_product(int planes, int tile, const g16::Args& a, const Epi& e, hipStream_t st, const g16::Ragged& rg) {
+  if (planes == 2) g16::launch_split<LM, LN, RAG>(tile, a, e, st, rg);
+  else if constexpr (SMALL) g16::launch_small<LM, LN, RAG>(tile, a, e, st, rg);
+  else g16::launch<LM, LN, false, RAG>(tile, a, e, st, rg);
 }
 
 template <class F>
@@ -428,34 +431,44 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
   });
   // The sides are padded to 64 with zeros, which the products keep: a zero row or column of X gives zero
   // rows and columns of A, B and the next X.
-  const int nseg = g.planes == 2 ? 3 : 1;
   const int64_t sp = g.side, pa = sp * sp;
-  const int t_gram = plan(sp, sp, total / g.count, nseg, g.count, true, false).tile;
-  const int t_poly = plan(sp, sp, sp, nseg, g.count, true, false).tile;
-  const int t_upd = plan(sp, total, sp, nseg, 1, false, false).tile;
-  const int t_fin = t_upd == T256 ? T128 : t_upd;  // (turning 256 accumulators does not fit the registers)
+  auto half = [&](int t) { return (int64_t)cdiv(sp, t) * (cdiv(sp, t) + 1) / 2 * g.count; };  // tiles of a symmetric product
+  auto full = [&](int t) {
+    int64_t n = 0;
+    for (int i = 0; i < g.count; ++i) n += (int64_t)cdiv(sp, t) * cdiv(g.m[i].len, t);
+    return n;
+  };
+  int t_gram, t_poly, t_upd;
+  if (g.planes == 2) {
+    t_gram = plan_split(half(128), half(64), total / g.count);
+    t_poly = plan_split(half(128), half(64), sp);
+    t_upd = plan_split(full(128), full(64), sp);
+  } else {
+    t_gram = plan(sp, sp, total / g.count, 1, g.count, true, false).tile;
+    t_poly = plan(sp, sp, sp, 1, g.count, true, false).tile;
+    t_upd = plan(sp, total, sp, 1, 1, false, false).tile;
+  }
   u16 *x = sc.x0, *y = sc.x1;
   for (int it = 0; it < p.steps; ++it) {
     Args a;
     a.batch = g.count;
-    a.nseg = nseg;
     a.sym = 1;
     a.M = a.N = g.side;
-    a.m = ragged_side(x, g.side, false);
-    a.n = ragged_side(x, g.side, true);
-    launch<KC, KC, false, 1>(t_gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f, 0.f}, st, rg);
+    a.m = a.n = ragged_side(x, g.side);
+    run_product<KC, KC, 1, false>(g.planes, t_gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f, 0.f},
+                                  st, rg);
     a.K = g.side;
-    a.m = square_side(sc.gram, sp, g.planes, false);
-    a.n = square_side(sc.gram, sp, g.planes, true);
-    launch<KC, KC>(t_poly, a, EpiPlanes<true>{sc.poly, sc.gram, sp, pa, g.planes, 1, p.c * INV_S, p.b, p.a * S}, st);
+    a.m = a.n = square_side(sc.gram, sp, g.planes);
+    run_product<KC, KC, 0, true>(g.planes, t_poly, a,
+                                 EpiPlanes<true>{sc.poly, sc.gram, sp, pa, g.planes, 1, p.c * INV_S, p.b, p.a * S}, st, rg);
     a.sym = 0;
-    a.m = square_side(sc.poly, sp, g.planes, false);
-    a.n = ragged_side(x, 0, true);
+    a.m = square_side(sc.poly, sp, g.planes);
+    a.n = ragged_side(x, 0);
     if (it + 1 < p.steps) {
-      launch<KC, KS, false, 2>(t_upd, a, EpiPlanes<false>{y, nullptr, 0, 0, g.planes, 0, INV_S, 0.f, 0.f}, st, rg);
+      run_product<KC, KS, 2, false>(g.planes, t_upd, a, EpiPlanes<false>{y, nullptr, 0, 0, g.planes, 0, INV_S, 0.f, 0.f}, st, rg);
     } else {
       auto fin = [&](auto K) {
-        launch<KC, KS, false, 2>(t_fin, a, EpiFinal<K.value>{out, INV_S * INV_S, p.decay}, st, rg);
+        run_product<KC, KS, 2, true>(g.planes, t_upd, a, EpiFinal<K.value>{out, INV_S * INV_S, p.decay}, st, rg);
       };
       if (p.muon) fin(std::integral_constant<int, 3>{});
       else with_kind(p, fin);
