@@ -39,14 +39,45 @@ def parse():
     ap.add_argument("--seq-len", type=int, default=512)
     ap.add_argument("--compression", choices=["none", "fp16", "bf16"], default="")
     ap.add_argument("--fusion-mib", type=float, default=0, help="fusion threshold (0 = engine default)")
-    ap.add_argument("--optimizer", choices=["torch", "fused"], default="fused",
-                    help="fused: mihvd multi-tensor HIP optimizer (FusedSGD / FusedAdam(adamw))")
+    ap.add_argument("--optimizer", choices=["torch", "fused", "muon"], default="fused",
+                    help="fused: mihvd multi-tensor HIP optimizer (FusedSGD / FusedAdam(adamw)); muon: bert-base, "
+                         "mihvd.optim.Muon for the encoder's matrices beside FusedAdam for the rest")
+    ap.add_argument("--bert-ffn", choices=["gelu", "geglu", "swiglu"], default="gelu",
+                    help="bert-base: the feed-forward block (gated ones through mihvd.ops.gated_ffn, 2048 columns)")
+    ap.add_argument("--bert-loss", choices=["torch", "fused"], default="torch",
+                    help="bert-base: fused = mihvd.ops.linear_cross_entropy")
     ap.add_argument("--graph", action="store_true", help="capture the whole step in one HIP graph")
     ap.add_argument("--no-dp", action="store_true",
                     help="plain optimizer without mihvd's DistributedOptimizer (world size 1: engine overhead)")
     ap.add_argument("--mlm-all-positions", action="store_true",
                     help="bert-base: MLM head on every position (default: the masked positions only)")
-    return ap.parse_args()
+    args = ap.parse_args()
+    if args.optimizer == "muon" and args.model != "bert-base":
+        ap.error("--optimizer muon needs --model bert-base")
+    return args
+
+
+class _Both:
+    """Two optimizers over disjoint parameters, stepped as one."""
+
+    def __init__(self, *opts):
+        self.opts = opts
+
+    @property
+    def buckets(self):
+        return [b for o in self.opts for b in getattr(o, "buckets", [])]
+
+    @property
+    def _buckets(self):
+        return [b for o in self.opts for b in o._buckets]
+
+    def zero_grad(self, set_to_none=True):
+        for o in self.opts:
+            o.zero_grad(set_to_none=set_to_none)
+
+    def step(self):
+        for o in self.opts:
+            o.step()
 
 
 def main():
@@ -86,8 +117,9 @@ def main():
         from mihvd.models.bert import BertConfig, BertForMaskedLM, synthetic_mlm_batch
 
         B = args.batch_size or 16
+        gated = {} if args.bert_ffn == "gelu" else {"ffn": 2048, "ffn_impl": args.bert_ffn}
         c = BertConfig(max_len=max(512, args.seq_len), attn_impl=os.environ.get("MIHVD_BERT_ATTN", "sdpa"),
-                       embedding_impl=os.environ.get("MIHVD_BERT_EMBEDDING", "gather"))
+                       embedding_impl=os.environ.get("MIHVD_BERT_EMBEDDING", "gather"), loss_impl=args.bert_loss, **gated)
         model = BertForMaskedLM(c).to(dev)
         ids, labels = synthetic_mlm_batch(B, args.seq_len, c.vocab_size, dev, generator=g)
         from mihvd.models.bert import masked_positions
@@ -97,6 +129,13 @@ def main():
             from mihvd.optim import FusedAdam
 
             base = FusedAdam(model.parameters(), lr=1e-4 * n, weight_decay=0.01, adamw=True)
+        elif args.optimizer == "muon":
+            from mihvd.models.bert import muon_parameters
+            from mihvd.optim import FusedAdam, Muon
+
+            matrices, others = muon_parameters(model)
+            base = (Muon(matrices, lr=1e-4 * n, weight_decay=0.01, scale="rms"),
+                    FusedAdam(others, lr=1e-4 * n, weight_decay=0.01, adamw=True))
         else:
             base = torch.optim.AdamW(model.parameters(), lr=1e-4 * n, weight_decay=0.01,
                                      **({"capturable": True} if args.graph else {}))
@@ -112,10 +151,18 @@ def main():
         if n > 1:
             raise SystemExit("--no-dp is a world-size-1 measurement")
         opt = base
-        opt.buckets = []
+        if isinstance(base, tuple):
+            opt = _Both(*base)
+        else:
+            opt.buckets = []
     else:
-        opt = hvd.DistributedOptimizer(base, named_parameters=model.named_parameters(), compression=comp,
-                                       fusion_threshold=int(args.fusion_mib * 2 ** 20) if args.fusion_mib else None)
+        def wrap(o):
+            mine = {id(p) for g in o.param_groups for p in g["params"]}
+            return hvd.DistributedOptimizer(
+                o, named_parameters=[(k, p) for k, p in model.named_parameters() if id(p) in mine], compression=comp,
+                fusion_threshold=int(args.fusion_mib * 2 ** 20) if args.fusion_mib else None)
+
+        opt = _Both(*map(wrap, base)) if isinstance(base, tuple) else wrap(base)
 
     def step():
         opt.zero_grad(set_to_none=False)
@@ -167,6 +214,7 @@ def main():
                     "distributed_optimizer": not args.no_dp})
         if args.model == "bert-base":
             cfg["mlm_head"] = "all positions" if args.mlm_all_positions else "masked positions"
+            cfg.update({"ffn": args.bert_ffn, "loss": args.bert_loss})
         print(json.dumps({"metric": metric, "value": round(args.steps * B * per_sample * n / el, 1), "unit": unit,
                           "n_gpus": n, "steps": args.steps, "warmup": args.warmup,
                           "ms_per_step": round(el / args.steps * 1e3, 3), "higher_is_better": True,

@@ -4,7 +4,8 @@ fusion + fp16 allreduce compression)" stretch configuration of BASELINE.json: 11
 compression stress test of the DP engine.
 
 Built from stock PyTorch-ROCm ops (``scaled_dot_product_attention``, hipBLASLt GEMMs) under bf16
-autocast. Not part of the reference repo (whose only model is the MNIST CNN).
+autocast; ``BertConfig.ffn_impl`` and ``loss_impl`` choose the framework's own gated feed-forward block
+and vocabulary loss (mihvd.ops). Not part of the reference repo (whose only model is the MNIST CNN).
 """
 from __future__ import annotations
 
@@ -14,6 +15,8 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops import gated_ffn, linear_cross_entropy
 
 
 @dataclasses.dataclass
@@ -34,6 +37,13 @@ class BertConfig:
     # that partition kernel faults (memory aperture violation) when a whole BERT step is replayed
     # from a HIP graph on this ROCm build with MLM data (many repeated [MASK] ids)
     embedding_impl: str = "gather"
+    # "gelu": fc2(gelu(fc1(x))); "geglu" / "swiglu": the gated block fc_down(act(fc_gate(x)) * fc_up(x)) with
+    # ``ffn`` columns and no biases, on the GPU through mihvd.ops.gated_ffn (16-bit: under autocast, or
+    # a model in bf16 / fp16)
+    ffn_impl: str = "gelu"
+    # "torch": logits and F.cross_entropy; "fused": mihvd.ops.linear_cross_entropy on the GPU (16-bit, as
+    # above), which keeps no logits and skips the positions without a label
+    loss_impl: str = "torch"
 
 
 class BertLayer(nn.Module):
@@ -43,13 +53,28 @@ class BertLayer(nn.Module):
         self.qkv = nn.Linear(c.hidden, 3 * c.hidden)
         self.proj = nn.Linear(c.hidden, c.hidden)
         self.ln1 = nn.LayerNorm(c.hidden, eps=c.eps)
-        self.fc1 = nn.Linear(c.hidden, c.ffn)
-        self.fc2 = nn.Linear(c.ffn, c.hidden)
+        if c.ffn_impl == "gelu":
+            self.fc1 = nn.Linear(c.hidden, c.ffn)
+            self.fc2 = nn.Linear(c.ffn, c.hidden)
+        elif c.ffn_impl in ("geglu", "swiglu"):
+            self.fc_gate = nn.Linear(c.hidden, c.ffn, bias=False)
+            self.fc_up = nn.Linear(c.hidden, c.ffn, bias=False)
+            self.fc_down = nn.Linear(c.ffn, c.hidden, bias=False)
+        else:
+            raise ValueError("BertConfig.ffn_impl must be 'gelu', 'geglu' or 'swiglu' (got %r)" % (c.ffn_impl,))
         self.ln2 = nn.LayerNorm(c.hidden, eps=c.eps)
         self.drop = nn.Dropout(c.dropout)
 
     def _attn_p(self):
         return self.c.dropout if self.c.attn_dropout is None else self.c.attn_dropout
+
+    def _ffn(self, x):
+        if self.c.ffn_impl == "gelu":
+            return self.fc2(F.gelu(self.fc1(x)))
+        act = "gelu" if self.c.ffn_impl == "geglu" else "silu"
+        if x.is_cuda:
+            return gated_ffn(x, self.fc_gate.weight, self.fc_up.weight, self.fc_down.weight, activation=act)
+        return self.fc_down((F.gelu if act == "gelu" else F.silu)(self.fc_gate(x)) * self.fc_up(x))
 
     def forward(self, x, mask=None):
         B, S, H = x.shape
@@ -65,13 +90,15 @@ class BertLayer(nn.Module):
             a = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, dropout_p=p)
         a = a.transpose(1, 2).reshape(B, S, H)
         x = self.ln1(x + self.drop(self.proj(a)))  # post-LN, as in BERT
-        return self.ln2(x + self.drop(self.fc2(F.gelu(self.fc1(x)))))
+        return self.ln2(x + self.drop(self._ffn(x)))
 
 
 class BertForMaskedLM(nn.Module):
     def __init__(self, c: BertConfig | None = None):
         super().__init__()
         c = c or BertConfig()
+        if c.loss_impl not in ("torch", "fused"):
+            raise ValueError("BertConfig.loss_impl must be 'torch' or 'fused' (got %r)" % (c.loss_impl,))
         self.c = c
         self.tok = nn.Embedding(c.vocab_size, c.hidden)
         self.pos = nn.Embedding(c.max_len, c.hidden)
@@ -112,10 +139,20 @@ class BertForMaskedLM(nn.Module):
             if labels is not None:
                 labels = labels.reshape(-1).index_select(0, masked_positions)
         h = self.head_ln(F.gelu(self.head_dense(x)))
+        if labels is not None and self.c.loss_impl == "fused" and h.is_cuda:
+            return linear_cross_entropy(h, self.tok.weight, labels.reshape(h.shape[:-1]), self.head_bias)
         logits = h @ self.tok.weight.t() + self.head_bias
         if labels is None:
             return logits
         return F.cross_entropy(logits.float().view(-1, logits.size(-1)), labels.reshape(-1), ignore_index=-100)
+
+
+def muon_parameters(model: BertForMaskedLM):
+    """(matrices, others): the encoder layers' weight matrices, which ``mihvd.optim.Muon`` updates, and the
+    embeddings, head, norms and biases, which stay with another optimizer."""
+    matrices = [p for layer in model.layers for p in layer.parameters() if p.dim() == 2]
+    chosen = {id(p) for p in matrices}
+    return matrices, [p for p in model.parameters() if id(p) not in chosen]
 
 
 def masked_positions(labels: torch.Tensor) -> torch.Tensor:
@@ -135,6 +172,7 @@ def synthetic_mlm_batch(batch: int, seq: int, vocab: int, device, generator=None
 
 def flops_per_token(c: BertConfig, seq: int) -> float:
     """Training FLOPs per token (6·params for the dense parts + attention scores)."""
-    dense = c.layers * (4 * c.hidden * c.hidden + 2 * c.hidden * c.ffn) + c.hidden * c.vocab_size
+    mats = 2 if c.ffn_impl == "gelu" else 3
+    dense = c.layers * (4 * c.hidden * c.hidden + mats * c.hidden * c.ffn) + c.hidden * c.vocab_size
     attn = c.layers * 2 * seq * c.hidden
     return 6.0 * dense + 6.0 * attn if math.isfinite(seq) else float("nan")
