@@ -792,20 +792,28 @@ __device__ __forceinline__ void store8(u16* row, int n, int N, bool vec, uint4 v
     if (n + k < N) row[n + k] = (u16)(w[k >> 1] >> (16 * (k & 1)));
 }
 
+// A factor that lives on the device: *f, or 1, over an optional count (0 if that is 0).
+__device__ __forceinline__ float scalar(const float* f, const int* count) {
+  const float v = f ? *f : 1.f;
+  if (!count) return v;
+  return *count > 0 ? v / (float)*count : 0.f;
+}
+
 // out[batch][m][n] = alpha * acc, rounded once to the 16-bit format; alpha times an optional device
-// scalar. `out[]` holds one base per batch entry.
+// scalar over an optional device count. `out[]` holds one base per batch entry.
 struct EpiStore {
   u16* out[2];
   int64_t ld;
   float alpha;
   const float* dev_alpha;
+  const int* dev_count;
   template <int NI, int MI>
   struct Pre {};
   template <int NI, int MI>
   __device__ __forceinline__ void load(const Ctx&, Pre<NI, MI>&) const {}
   template <int NI, int MI>
   __device__ __forceinline__ void run(const Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
-    const float al = dev_alpha ? alpha * *dev_alpha : alpha;
+    const float al = alpha * scalar(dev_alpha, dev_count);
     u16* o = c.batch == 0 ? out[0] : out[1];
     const bool vec = (ld & 7) == 0;
     const RowStage<NI * 16> st{c.stage, c.lane};

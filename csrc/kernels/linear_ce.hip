@@ -30,15 +30,68 @@ constexpr float DZ_SCALE = 16384.f;
 constexpr float DZ_SCALE = 1.f;
 #endif
 
-// Row r of the compact hidden matrix; one wave per row, 16 bytes a lane where the row allows it.
-__global__ void __launch_bounds__(256) lce_gather(const u16* __restrict__ h, int64_t s0, int64_t s1,
-                                                  const int* __restrict__ idx, const int* __restrict__ cnt, int K, int K8,
-                                                  u16* __restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= *cnt) return;
-  const u16* src = h + (int64_t)idx[r] * s0;
-  u16* dst = out + (int64_t)r * K8;
+// Sum of n over a block of 1024, for every thread.
+__device__ __forceinline__ int count_block(int n, int* sh) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
+  __syncthreads();
+  int tot = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) tot += sh[i];
+  return tot;
+}
+
+// Labelled rows of each chunk of rows.
+__global__ void __launch_bounds__(1024) lce_count(const int64_t* __restrict__ labels, int N, int64_t ignore, int chunk,
+                                                  int* __restrict__ counts) {
+  __shared__ int sh[16];
+  const int64_t r0 = (int64_t)blockIdx.x * chunk, r1 = min((int64_t)N, r0 + chunk);
+  int n = 0;
+  for (int64_t r = r0 + threadIdx.x; r < r1; r += 1024) n += labels[r] != ignore;
+  const int tot = count_block(n, sh);
+  if (threadIdx.x == 0) counts[blockIdx.x] = tot;
+}
+
+// Compacts the labelled rows: their row numbers, their labels in 32 bits (-1: outside the vocabulary),
+// every row's place among them, their count, and their hidden vectors. A block takes 16 rows, a wave
+// each, and counts the labels ahead of them by itself: of all rows (up to 16384 of them: 64 KB a block on
+// average, out of L2), or of its chunk on top of the chunks' counts.
+__global__ void __launch_bounds__(1024) lce_gather(const int64_t* __restrict__ labels, int N, int V, int64_t ignore,
+                                                   const int* __restrict__ counts, int chunk, const u16* __restrict__ h,
+                                                   int64_t s0, int64_t s1, int K, int K8, const LceRowsOut rw,
+                                                   u16* __restrict__ out) {
+  __shared__ int sh[16], own[16];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int64_t first = (int64_t)blockIdx.x * 16;
+  int n = 0;
+  int64_t from = 0;
+  if (counts) {
+    const int c = (int)(first / chunk);
+    for (int i = t; i < c; i += 1024) n += counts[i];
+    from = (int64_t)c * chunk;
+  }
+  for (int64_t r = from + t; r < first; r += 1024) n += labels[r] != ignore;
+  const int64_t r = first + w;
+  const int64_t y = r < N ? labels[r] : ignore;
+  const bool on = y != ignore;
+  if (lane == 0) own[w] = on;
+  int pos = count_block(n, sh);  // its barriers publish own[] too
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < w) pos += own[i];
+  if (lane == 0 && r < N) {
+    rw.inv[r] = on ? pos : -1;
+    if (on) {
+      rw.idx[pos] = (int)r;
+      rw.label[pos] = y >= 0 && y < V ? (int)y : -1;
+    }
+    if (r == N - 1) *rw.cnt = pos + (on ? 1 : 0);
+    if (r == 0) *rw.done = 0;
+  }
+  if (!on) return;
+  const u16* src = h + r * s0;
+  u16* dst = out + (int64_t)pos * K8;
   if (s1 == 1 && (s0 & 7) == 0 && ((uintptr_t)h & 15) == 0 && K == K8) {
     for (int k = lane * 8; k < K; k += 512) *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
   } else {
@@ -151,50 +204,92 @@ struct EpiStats {
   }
 };
 
-// Joins the pairs of every row: one wave a row, so that a handful of rows still has its loads in flight
-// together. Writes lse (compact) and the row's loss (all rows).
+// Joins the pairs of every row: WPR waves a row, four where there are few rows, so that their loads are in
+// flight together. Writes lse (compact) and the row's loss (all rows), and into `out`, if given, their sum
+// or mean: every block adds up its rows, and the block that ends last adds up the blocks, both in a fixed
+// order.
+template <int WPR>
 __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ part, int npart,
                                                   const float* __restrict__ zlab, const int* __restrict__ label,
                                                   const int* __restrict__ inv, int N, int V, float* __restrict__ lse,
-                                                  float* __restrict__ rows) {
-  const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= N) return;
-  const int c = inv[r];
-  if (c < 0) {
-    if (lane == 0) rows[r] = 0.f;
-    return;
+                                                  float* __restrict__ rows, float* __restrict__ blocks,
+                                                  int* __restrict__ done, const int* __restrict__ cnt, int mean,
+                                                  float* __restrict__ out) {
+  constexpr int RPB = 4 / WPR;
+  __shared__ float2 sh[4];
+  __shared__ int last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % WPR;
+  float total = 0.f;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < N; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + wave / WPR;
+    const int c = r < N ? inv[r] : -1;
+    float mx = -INFINITY, s = 0.f;
+    if (c >= 0) {
+      const float2* q = part + (int64_t)c * npart;
+      auto join = [&](const float2 v) {
+        const float top = fmaxf(mx, v.x), ref = top == -INFINITY ? 0.f : top;
+        s = s * __expf(mx - ref) + v.y * __expf(v.x - ref);
+        mx = top;
+      };
+      int p = sub * 64 + lane;
+      for (; p + 3 * WPR * 64 < npart; p += 4 * WPR * 64) {  // four loads in flight
+        float2 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = q[p + k * WPR * 64];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) join(v[k]);
+      }
+      for (; p < npart; p += WPR * 64) join(q[p]);
+      const float all = wave_max(mx), ref = all == -INFINITY ? 0.f : all;
+      s = wave_sum(s * __expf(mx - ref));
+      mx = all;
+    }
+    if constexpr (WPR > 1) {
+      if (lane == 0) sh[wave] = make_float2(mx, s);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < WPR; ++i) mx = fmaxf(mx, sh[i].x);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < WPR; ++i) s += sh[i].y * __expf(sh[i].x - ref);
+      __syncthreads();
+    }
+    if (lane == 0 && sub == 0 && r < N) {
+      float v = 0.f;
+      if (c >= 0) {
+        const int y = label[c];
+        // a label outside the vocabulary has no loss: NaN, and NaN gradients through lse
+        const bool in = y >= 0 && y < V;
+        const float l = in ? logf(s) + mx : NAN;
+        lse[c] = l;
+        v = l - (in ? zlab[c] : 0.f);
+      }
+      rows[r] = v;
+      total += v;
+    }
   }
-  const float2* q = part + (int64_t)c * npart;
-  float mx = -INFINITY;
-  for (int p = lane; p < npart; p += 64) mx = fmaxf(mx, q[p].x);
-  mx = wave_max(mx);
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  float s = 0.f;
-  for (int p = lane; p < npart; p += 64) s += q[p].y * __expf(q[p].x - ref);
-  s = wave_sum(s);
-  if (lane == 0) {
-    const int y = label[c];
-    // a label outside the vocabulary has no loss: NaN, and NaN gradients through lse
-    const bool in = y >= 0 && y < V;
-    const float v = in ? logf(s) + mx : NAN;
-    lse[c] = v;
-    rows[r] = v - (in ? zlab[c] : 0.f);
+  if (!out) return;
+  if (lane == 0) sh[wave].x = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int i = 0; i < 4; ++i) t += sh[i].x;
+    __hip_atomic_store(blocks + blockIdx.x, t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
   }
-}
-
-// mean / sum over the rows, by one block in a fixed order
-__global__ void __launch_bounds__(1024) lce_reduce(const float* __restrict__ rows, int N, const int* __restrict__ cnt,
-                                                   int mean, float* __restrict__ out) {
-  __shared__ float sh[16];
-  float s = 0.f;
-  for (int r = threadIdx.x; r < N; r += 1024) s += rows[r];
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (!last) return;
+  float t = 0.f;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256)
+    t += __hip_atomic_load(blocks + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  t = wave_sum(t);
+  __syncthreads();
+  if (lane == 0) sh[wave].x = t;
   __syncthreads();
   if (threadIdx.x == 0) {
     float tot = 0.f;
-    for (int i = 0; i < 16; ++i) tot += sh[i];
+    for (int i = 0; i < 4; ++i) tot += sh[i].x;
     *out = mean ? tot / (float)*cnt : tot;
   }
 }
@@ -290,35 +385,37 @@ struct EpiDz {
   }
 };
 
-__global__ void __launch_bounds__(256) lce_db(const float* __restrict__ dbp, int64_t ld, const int* __restrict__ cnt,
-                                              int tm, int wm_per_tile, int V, const float* __restrict__ gs,
-                                              void* __restrict__ db, int kind) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
+// The ends of the two gradients that are summed up: blocks below `dh_blocks` write dh of every row, the sum of
+// its slabs or zeros where the label was ignored; the others db of a piece of the vocabulary.
+__global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __restrict__ slab, int nslab, int64_t stride,
+                                                 int64_t ld, const int* __restrict__ inv, int N, int K,
+                                                 u16* __restrict__ dh, const float* __restrict__ dbp, int64_t ldb, int tm,
+                                                 int V, void* __restrict__ db, int kind, const int* __restrict__ cnt,
+                                                 const LceGrad g) {
+  const float scale = g16::scalar(g.scale, g.div) * (1.f / DZ_SCALE);
+  if ((int)blockIdx.x < dh_blocks) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int k4 = (K + 3) / 4;
+    const int64_t r = i / k4;
+    const int k = (int)(i - r * k4) * 4;
+    if (r >= N) return;
+    const int c = inv[r];
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c >= 0) {
+      for (int q = 0; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(slab + q * stride + (int64_t)c * ld + k);
+      s *= scale;
+    }
+    g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
+    return;
+  }
+  const int64_t v = (int64_t)(blockIdx.x - dh_blocks) * 256 + threadIdx.x;
   if (v >= V) return;
-  const int n = (*cnt + tm - 1) / tm * wm_per_tile;
+  const int n = (*cnt + tm - 1) / tm * 2;  // two waves along a tile's rows
   float s = 0.f;
-  for (int i = 0; i < n; ++i) s += dbp[(int64_t)i * ld + v];
-  s *= *gs * (1.f / DZ_SCALE);
+  for (int i = 0; i < n; ++i) s += dbp[(int64_t)i * ldb + v];
+  s *= scale;
   if (kind == 1) static_cast<float*>(db)[v] = s;
   else static_cast<u16*>(db)[v] = f2bf(s);
-}
-
-// dh of every row: the sum of its slabs, or zeros where the label was ignored.
-__global__ void __launch_bounds__(256) lce_dh(const float* __restrict__ slab, int nslab, int64_t stride, int64_t ld,
-                                              const int* __restrict__ inv, int N, int K, const float* __restrict__ gs,
-                                              u16* __restrict__ dh) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int k4 = (K + 3) / 4;
-  const int64_t r = i / k4;
-  const int k = (int)(i - r * k4) * 4;
-  if (r >= N) return;
-  const int c = inv[r];
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if (c >= 0) {
-    for (int q = 0; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(slab + q * stride + (int64_t)c * ld + k);
-    s *= *gs * (1.f / DZ_SCALE);
-  }
-  g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
 }
 
 template <bool BIAS, class Epi>
@@ -346,10 +443,13 @@ void lce_plan_backward(LceShape& s, LceScratch& x, bool bias) {
 }
 #endif
 
-void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t hs0, int64_t hs1, const u16* w, int64_t ldw,
-                    const void* bias, int bias_kind, u16* hc, float2* part, float* zlab, float* lse, float* rows,
-                    float* loss, int mean, hipStream_t st) {
-  lce_gather<<<g16::cdiv(s.N, 4), 256, 0, st>>>(h, hs0, hs1, rw.idx, rw.cnt, s.K, s.K8, hc);
+void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, const LceRowsOut& rw, const u16* h,
+                    int64_t hs0, int64_t hs1, const u16* w, int64_t ldw, const void* bias, int bias_kind, u16* hc,
+                    float2* part, float* zlab, float* lse, float* rows, float* blocks, float* loss, int mean,
+                    hipStream_t st) {
+  if (s.chunk) lce_count<<<g16::cdiv(s.N, s.chunk), 1024, 0, st>>>(labels, s.N, ignore, s.chunk, rw.counts);
+  lce_gather<<<g16::cdiv(s.N, 16), 1024, 0, st>>>(labels, s.N, s.V, ignore, s.chunk ? rw.counts : nullptr, s.chunk, h, hs0,
+                                                  hs1, s.K, s.K8, rw, hc);
   g16::Args a;
   a.m.p[0] = hc;
   a.m.ld = s.K8;
@@ -363,8 +463,12 @@ void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t 
   a.dyn_m = rw.cnt;
   if (bias) g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<true>{bias, bias_kind, rw.label, part, s.npart, zlab}, st);
   else g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<false>{nullptr, 0, rw.label, part, s.npart, zlab}, st);
-  lce_finish<<<g16::cdiv(s.N, 4), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows);
-  if (loss) lce_reduce<<<1, 1024, 0, st>>>(rows, s.N, rw.cnt, mean, loss);
+  if (s.N <= 1024)
+    lce_finish<4><<<s.N, 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows, blocks, rw.done, rw.cnt,
+                                       mean, loss);
+  else
+    lce_finish<1><<<std::min(g16::cdiv(s.N, 4), LCE_BLOCKS), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V,
+                                                                           lse, rows, blocks, rw.done, rw.cnt, mean, loss);
 }
 
 void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, const u16* hc, const u16* w, int64_t ldw,
@@ -395,11 +499,6 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       else if (g.rowscale) go(std::false_type{}, std::true_type{});
       else go(std::false_type{}, std::false_type{});
     }
-    if (db) {
-      const int esz = bias_kind == 1 ? 4 : 2;
-      lce_db<<<g16::cdiv(nv, 256), 256, 0, st>>>(x.dbp, x.ldz, rw.cnt, x.dz_tile, 2, nv, g.scale,
-                                                 static_cast<char*>(db) + (int64_t)v0 * esz, bias_kind);
-    }
     if (dw) {
       g16::Args a;
       a.m.p[0] = x.dz;
@@ -412,7 +511,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       a.N = s.K;
       a.K = s.N;
       a.dyn_k = rw.cnt;
-      g16::EpiStore e{{dw + (int64_t)v0 * s.K, nullptr}, s.K, 1.f / DZ_SCALE, g.scale};
+      g16::EpiStore e{{dw + (int64_t)v0 * s.K, nullptr}, s.K, 1.f / DZ_SCALE, g.scale, g.div};
       g16::launch<g16::KS, g16::KS>(x.dw_tile, a, e, st);
     }
     if (dh) {
@@ -431,10 +530,13 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       g16::EpiSlab e{x.slab, s.K8, (int64_t)s.N * s.K8, x.splits, first ? 0 : 1};
       g16::launch<g16::KC, g16::KS>(x.dh_tile, a, e, st);
     }
-  }
-  if (dh) {
-    const int64_t work = (int64_t)s.N * ((s.K + 3) / 4);
-    lce_dh<<<g16::cdiv(work, 256), 256, 0, st>>>(x.slab, x.splits, (int64_t)s.N * s.K8, s.K8, rw.inv, s.N, s.K, g.scale, dh);
+    // the pieces' slabs add up: dh is whole behind the last one
+    const int dh_blocks = dh && v0 + nv == s.V ? g16::cdiv((int64_t)s.N * ((s.K + 3) / 4), 256) : 0;
+    const int db_blocks = db ? g16::cdiv(nv, 256) : 0;
+    void* dbv = db ? static_cast<char*>(db) + (int64_t)v0 * (bias_kind == 1 ? 4 : 2) : nullptr;
+    if (dh_blocks + db_blocks)
+      lce_grads<<<dh_blocks + db_blocks, 256, 0, st>>>(dh_blocks, x.slab, x.splits, (int64_t)s.N * s.K8, s.K8, rw.inv, s.N,
+                                                       s.K, dh, x.dbp, x.ldz, x.dz_tile, nv, dbv, bias_kind, rw.cnt, g);
   }
 }
 

@@ -15,7 +15,9 @@ typedef unsigned short u16;
 struct LceShape {
   int N, K, K8, V;  // rows, hidden size, hidden size padded to 8, vocabulary
   int tile, npart;  // of the logits: output tile, (max, sum) pairs per row (two waves along a tile)
+  int chunk;        // rows whose labels are counted ahead, or 0: each block counts for itself
 };
+constexpr int LCE_BLOCKS = 1024;  // that share the end of the forward pass: partial sums of the loss
 // The labelled rows: compact position -> row, row -> compact position or -1, their labels and count.
 struct LceRows {
   const int* idx;
@@ -23,8 +25,14 @@ struct LceRows {
   const int* label;
   const int* cnt;
 };
+struct LceRowsOut {
+  int *idx, *inv, *label, *cnt;
+  int* done;    // blocks of the last kernel that have ended
+  int* counts;  // labelled rows per chunk
+};
 struct LceGrad {
-  const float* scale;     // G (times 1 / count for the mean), one device scalar
+  const float* scale;     // G, one device scalar
+  const int* div;         // what it is divided by (the mean's count), or null
   const float* rowscale;  // g_r / G per compact row, or null
 };
 struct LceScratch {
@@ -41,9 +49,10 @@ void lce_plan(LceShape& s);
 void lce_plan_backward(LceShape& s, LceScratch& x, bool bias);
 
 #define MIHVD_TRANSFORMER_DECLS                                                                                        \
-  void lce_forward_16(const LceShape& s, const LceRows& rw, const u16* h, int64_t hs0, int64_t hs1, const u16* w,      \
-                      int64_t ldw, const void* bias, int bias_kind, u16* hc, float2* part, float* zlab, float* lse,    \
-                      float* rows, float* loss, int mean, hipStream_t st);                                             \
+  void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, const LceRowsOut& rw, const u16* h,      \
+                      int64_t hs0, int64_t hs1, const u16* w, int64_t ldw, const void* bias, int bias_kind, u16* hc,   \
+                      float2* part, float* zlab, float* lse, float* rows, float* blocks, float* loss, int mean,        \
+                      hipStream_t st);                                                                                 \
   void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, const u16* hc, const u16* w,            \
                        int64_t ldw, const void* bias, int bias_kind, const float* lse, const LceScratch& x, u16* dh,   \
                        u16* dw, void* db, hipStream_t st);                                                             \

@@ -3,10 +3,14 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/library.h>
 
 #include <map>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "common.h"
 #include "transformer.h"
@@ -67,49 +71,13 @@ void check16(const at::Tensor& t, const char* op, const char* name, const at::Te
 // ------------------------------------------------------------------------------------------ //
 // linear_cross_entropy
 
-// One block: the labelled rows in order, their labels in 32 bits (-1: outside the vocabulary), and
-// for every row its place among them.
-__global__ void __launch_bounds__(1024) lce_compact(const int64_t* __restrict__ labels, int N, int V, int64_t ignore,
-                                                    int* __restrict__ idx, int* __restrict__ inv,
-                                                    int* __restrict__ label, int* __restrict__ cnt) {
-  __shared__ int wsum[16];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  int base = 0;
-  for (int r0 = 0; r0 < N; r0 += 1024) {
-    const int r = r0 + t;
-    const int64_t y = r < N ? labels[r] : ignore;
-    const bool on = y != ignore;
-    const unsigned long long b = __ballot(on);
-    const int before = __popcll(b & ((1ull << lane) - 1));
-    if (lane == 0) wsum[w] = __popcll(b);
-    __syncthreads();
-    int off = base, tot = 0;
-    for (int i = 0; i < 16; ++i) {
-      if (i < w) off += wsum[i];
-      tot += wsum[i];
-    }
-    if (r < N) inv[r] = on ? off + before : -1;
-    if (on) {
-      idx[off + before] = r;
-      label[off + before] = y >= 0 && y < V ? (int)y : -1;
-    }
-    base += tot;
-    __syncthreads();
-  }
-  if (t == 0) *cnt = base;
-}
-
-// G (over count for the mean) and the rows' shares of it. reduction: 0 none, 1 mean, 2 sum.
-__global__ void __launch_bounds__(1024) lce_scale(const float* __restrict__ gout, int64_t gstride, int reduction,
+// Row weights: G = max |g_r| over the finite ones (an infinite one stays infinite in its own row), g_r / G.
+__global__ void __launch_bounds__(1024) lce_scale(const float* __restrict__ gout, int64_t gstride,
                                                   const int* __restrict__ idx, const int* __restrict__ cnt,
                                                   float* __restrict__ scale, float* __restrict__ rowscale) {
   const int n = *cnt;
-  if (reduction != 0) {
-    if (threadIdx.x == 0) *scale = reduction == 2 ? *gout : n > 0 ? *gout / (float)n : 0.f;
-    return;
-  }
   __shared__ float sh[16];
-  float m = 0.f;  // over the finite ones: an infinite share stays infinite in its own row
+  float m = 0.f;
   for (int c = threadIdx.x; c < n; c += 1024) {
     const float g = fabsf(gout[idx[c] * gstride]);
     if (g < INFINITY) m = fmaxf(m, g);
@@ -124,6 +92,7 @@ __global__ void __launch_bounds__(1024) lce_scale(const float* __restrict__ gout
   if (threadIdx.x == 0) *scale = G;
 }
 
+// meta: row numbers, places, labels, their count, and the forward pass's block counter and chunk counts
 LceRows rows_of(const at::Tensor& meta, int64_t N) {
   const int* p = meta.data_ptr<int>();
   return {p, p + N, p + 2 * N, p + 3 * N};
@@ -161,25 +130,33 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   const auto f32 = h.options().dtype(at::kFloat);
   c10::optional<at::Tensor> bias;
   if (bias_in) bias = bias_in->contiguous();
+  LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0, 0};
+  // Blocks that count all labels ahead of their rows for themselves read 64 KB on average at 16384 rows; past that
+  // the chunks (at most 4096) are counted ahead, which costs a launch.
+  if (N > 16384) s.chunk = (int)(cdiv(cdiv(N, 4096), 1024) * 1024);
+  const int64_t nmeta = 3 * N + 2 + (s.chunk ? cdiv(N, s.chunk) : 0);
   at::Tensor rows = at::empty({N}, f32), loss = reduction ? at::empty({}, f32) : rows;
   at::Tensor hc = at::empty({N, K8}, h.options()), lse = at::empty({N}, f32);
-  at::Tensor meta = at::empty({3 * N + 1}, h.options().dtype(at::kInt));
+  at::Tensor meta = at::empty({nmeta}, h.options().dtype(at::kInt));
   if (N == 0) {
     if (reduction) loss.fill_(reduction == 1 ? NAN : 0.f);
     meta.zero_();
     return {loss, hc, meta, lse};
   }
-  at::Tensor lab = labels.contiguous();
+  const at::Tensor lab = labels.contiguous();
   int* m = meta.data_ptr<int>();
-  lce_compact<<<1, 1024, 0, st>>>(lab.data_ptr<int64_t>(), (int)N, (int)V, ignore_index, m, m + N, m + 2 * N, m + 3 * N);
+  const LceRowsOut rw{m, m + N, m + 2 * N, m + 3 * N, m + 3 * N + 1, m + 3 * N + 2};
   const Mat wm = mat(w);
-  LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0};
   lce_plan(s);
-  at::Tensor part = at::empty({N, s.npart, 2}, f32), zlab = at::empty({N}, f32);
+  // (max, sum) pairs, the labels' logits, the blocks' sums
+  at::Tensor work = at::empty({N * (2 * (int64_t)s.npart + 1) + LCE_BLOCKS}, f32);
+  float* part = work.data_ptr<float>();
+  float *zlab = part + 2 * N * s.npart, *blocks = zlab + N;
   auto run = h.scalar_type() == at::kHalf ? &f16::lce_forward_16 : &lce_forward_16;
-  run(s, rows_of(meta, N), p16(h), h.stride(0), h.stride(1), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr,
-      bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part.data_ptr<float>()), zlab.data_ptr<float>(),
-      lse.data_ptr<float>(), rows.data_ptr<float>(), reduction ? loss.data_ptr<float>() : nullptr, reduction == 1, st);
+  run(s, lab.data_ptr<int64_t>(), ignore_index, rw, p16(h), h.stride(0), h.stride(1), wm.p, wm.ld,
+      bias ? bias->data_ptr() : nullptr, bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part), zlab,
+      lse.data_ptr<float>(), rows.data_ptr<float>(), blocks, reduction ? loss.data_ptr<float>() : nullptr, reduction == 1,
+      st);
   return {loss, hc, meta, lse};
 }
 
@@ -189,7 +166,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
                                                             int64_t reduction, bool need_h, bool need_w, bool need_b) {
   const int64_t N = lse.size(0), V = w.size(0), K = w.size(1), K8 = up8(K);
   TORCH_CHECK_VALUE(hc.dim() == 2 && hc.size(0) == N && hc.size(1) == K8 && hc.is_contiguous() &&
-                        meta.numel() == 3 * N + 1 && hc.scalar_type() == w.scalar_type(),
+                        meta.numel() >= 3 * N + 2 && hc.scalar_type() == w.scalar_type(),
                     "lce_backward: not the tensors that lce_forward returned");
   check16(w, "lce_backward", "weight", hc, 2);
   TORCH_CHECK_VALUE(gout.scalar_type() == at::kFloat && gout.device() == w.device() &&
@@ -211,15 +188,19 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
     return {dh, dw, db};
   }
   const LceRows rw = rows_of(meta, N);
-  at::Tensor scale = at::empty({1}, f32), rowscale;
-  if (reduction == 0) rowscale = at::empty({N}, f32);
-  lce_scale<<<1, 1024, 0, st>>>(gout.data_ptr<float>(), reduction ? 0 : gout.stride(0), (int)reduction, rw.idx, rw.cnt,
-                                scale.data_ptr<float>(), reduction ? nullptr : rowscale.data_ptr<float>());
+  LceGrad g{gout.data_ptr<float>(), reduction == 1 ? rw.cnt : nullptr, nullptr};
+  at::Tensor scale;
+  if (reduction == 0) {
+    scale = at::empty({N + 1}, f32);
+    float* q = scale.data_ptr<float>();
+    lce_scale<<<1, 1024, 0, st>>>(gout.data_ptr<float>(), gout.stride(0), rw.idx, rw.cnt, q, q + 1);
+    g = {q, nullptr, q + 1};
+  }
   const Mat wm = mat(w);
   LceScratch x{};
   x.piece = (int)std::min<int64_t>(up8(V), std::max<int64_t>(256, DZ_BYTES / (2 * N) / 256 * 256));
   x.ldz = up8(x.piece);
-  LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0};
+  LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0, 0};
   lce_plan_backward(s, x, bias.has_value());
   at::Tensor dz = at::empty({N, x.ldz}, w.options()), dbp, slab;
   x.dz = m16(dz);
@@ -231,7 +212,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
     slab = at::empty({x.splits, N, K8}, f32);
     x.slab = slab.data_ptr<float>();
   }
-  const LceGrad g{scale.data_ptr<float>(), reduction ? nullptr : rowscale.data_ptr<float>()};
   auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
   run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias), lse.data_ptr<float>(), x, m16(dh),
       m16(dw), need_b ? db.data_ptr() : nullptr, st);
@@ -321,6 +301,128 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
   run(s, dym.p, dym.ld, xm.p, xm.ld, wm.w, (int)act, p16(g), p16(u), p16(h), m16(dgu), m16(dx), m16(dwg), m16(dwu),
       m16(dwd), x.device(), cur_stream());
   return {dx, dwg, dwu, dwd};
+}
+
+// ------------------------------------------------------------------------------------------ //
+// Autograd. In C++, since a small call's time is the host's. A gradient that is itself to be differentiated
+// goes through Once, whose backward refuses.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Once : torch::autograd::Function<Once> {
+  static at::Tensor forward(AutogradContext*, const at::Tensor& grad, const at::Tensor&) { return grad.view_as(grad); }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "linear_cross_entropy / gated_ffn: their gradients cannot be differentiated again");
+    return {};
+  }
+};
+void once(const at::Tensor& gout, variable_list& grads) {
+  if (!at::GradMode::is_enabled()) return;
+  const at::Tensor any = gout.detach().requires_grad_(true);
+  for (at::Tensor& t : grads)
+    if (t.defined()) t = Once::apply(t, any);
+}
+
+// Called by a backward pass before anything else runs. While a stream is captured, the engine would make a
+// leaf's gradient accumulator that an eager graph on the default stream still holds wait there for the
+// captured stream, which invalidates the capture inside the engine and ends the process: refused
+// here, with the graph behind this node searched for such leaves.
+void refuse_eager_leaves(const char* op) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  C10_HIP_CHECK(hipStreamIsCapturing(cur_stream(), &status));
+  if (status == hipStreamCaptureStatusNone) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  std::vector<torch::autograd::Node*> stack{node.get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!stack.empty()) {
+    torch::autograd::Node* n = stack.back();
+    stack.pop_back();
+    if (!seen.insert(n).second) continue;
+    if (auto* acc = dynamic_cast<torch::autograd::AccumulateGrad*>(n)) {
+      const auto stream = acc->stream();
+      if (acc->variable.is_cuda())
+        TORCH_CHECK(stream && stream->id() != c10::hip::getDefaultHIPStream(acc->variable.get_device()).id(), op,
+                    ": the backward pass is being captured while an eager autograd graph of the same leaves is alive on "
+                    "the default stream; drop that graph (its loss and outputs), or run it on a side stream");
+      continue;
+    }
+    for (const auto& e : n->next_edges())
+      if (e.function) stack.push_back(e.function.get());
+  }
+}
+
+struct LceFunction : torch::autograd::Function<LceFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
+                            const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, hc, meta, lse] = lce_forward(h, w, labels, bias, ignore_index, reduction);
+    ctx->save_for_backward({hc, w, meta, lse, bias ? *bias : at::Tensor()});
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    refuse_eager_leaves("linear_cross_entropy");
+    const variable_list t = ctx->get_saved_variables();
+    c10::optional<at::Tensor> bias;
+    if (t[4].defined()) bias = t[4];
+    variable_list grads(3);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(grads[0], grads[1], grads[2]) =
+          lce_backward(gout[0], t[0], t[1], bias, t[2], t[3], ctx->saved_data["reduction"].toInt(),
+                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), bias && ctx->needs_input_grad(3));
+    }
+    once(gout[0], grads);
+    return {grads[0], grads[1], at::Tensor(), grads[2], at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor linear_cross_entropy(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
+                                const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
+  return std::get<0>(lce_forward(h, w, labels, bias, ignore_index, reduction));
+}
+at::Tensor linear_cross_entropy_autograd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
+                                         const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
+  return LceFunction::apply(h, w, labels, bias, ignore_index, reduction);
+}
+
+struct FfnFunction : torch::autograd::Function<FfnFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                            const at::Tensor& wd, int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, g, u, h] = ffn_forward(x, wg, wu, wd, act, true);
+    ctx->save_for_backward({x, wg, wu, wd, g, u, h});
+    ctx->saved_data["act"] = act;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    refuse_eager_leaves("gated_ffn");
+    const variable_list t = ctx->get_saved_variables();
+    variable_list grads(4);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(grads[0], grads[1], grads[2], grads[3]) =
+          ffn_backward(dy[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], ctx->saved_data["act"].toInt(),
+                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2),
+                       ctx->needs_input_grad(3));
+    }
+    once(dy[0], grads);
+    grads.emplace_back();
+    return grads;
+  }
+};
+
+at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t act) {
+  return std::get<0>(ffn_forward(x, wg, wu, wd, act, false));
+}
+at::Tensor gated_ffn_autograd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
+                              int64_t act) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad()))
+    return FfnFunction::apply(x, wg, wu, wd, act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return gated_ffn(x, wg, wu, wd, act);
 }
 
 // ------------------------------------------------------------------------------------------ //
@@ -443,24 +545,22 @@ void muon_step(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vect
 }  // namespace mihvd
 
 TORCH_LIBRARY_FRAGMENT(mihvd, m) {
-  m.def("lce_forward(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, int ignore_index, int reduction) -> "
-        "(Tensor, Tensor, Tensor, Tensor)");
-  m.def("lce_backward(Tensor gout, Tensor hc, Tensor weight, Tensor? bias, Tensor meta, Tensor lse, int reduction, "
-        "bool need_h, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)");
-  m.def("ffn_forward(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act, bool save) -> (Tensor, Tensor, Tensor, "
-        "Tensor)");
-  m.def("ffn_backward(Tensor dy, Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, Tensor g, Tensor u, Tensor h, "
-        "int act, bool need_x, bool need_g, bool need_u, bool need_d) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, int ignore_index, int reduction) "
+        "-> Tensor");
+  m.def("gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor");
   m.def("newton_schulz(Tensor x, int steps, float a, float b, float c, float eps, bool split) -> Tensor");
   m.def("muon_step(Tensor(a!)[] p, Tensor[] g, Tensor(b!)[] m, float lr, float momentum, bool nesterov, "
         "float weight_decay, int steps, float a, float b, float c, float eps, int scale_mode, bool split) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(mihvd, CUDA, m) {
-  m.impl("lce_forward", &mihvd::lce_forward);
-  m.impl("lce_backward", &mihvd::lce_backward);
-  m.impl("ffn_forward", &mihvd::ffn_forward);
-  m.impl("ffn_backward", &mihvd::ffn_backward);
+  m.impl("linear_cross_entropy", &mihvd::linear_cross_entropy);
+  m.impl("gated_ffn", &mihvd::gated_ffn);
   m.impl("newton_schulz", &mihvd::newton_schulz);
   m.impl("muon_step", &mihvd::muon_step);
+}
+
+TORCH_LIBRARY_IMPL(mihvd, AutogradCUDA, m) {
+  m.impl("linear_cross_entropy", &mihvd::linear_cross_entropy_autograd);
+  m.impl("gated_ffn", &mihvd::gated_ffn_autograd);
 }

@@ -1,4 +1,5 @@
-"""Autograd-facing wrappers of the transformer-step kernels (``torch.ops.mihvd.lce_* / ffn_*``).
+"""Entry points of the transformer-step kernels (``torch.ops.mihvd.linear_cross_entropy / gated_ffn``, whose
+autograd formulas are registered beside them in csrc/kernels/transformer_ops.cpp).
 
 * ``linear_cross_entropy(hidden, weight, labels, bias)`` — the vocabulary projection and its softmax
   cross entropy without materialised logits (csrc/kernels/linear_ce.hip).
@@ -34,24 +35,6 @@ def _prepare(op, *tensors):
     return list(tensors)
 
 
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, labels, ignore_index, reduction):
-        loss, hc, meta, lse = torch.ops.mihvd.lce_forward(hidden, weight, labels, bias, ignore_index, reduction)
-        ctx.save_for_backward(hc, weight, bias, meta, lse)
-        ctx.reduction = reduction
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gout):
-        hc, weight, bias, meta, lse = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dh, dw, db = torch.ops.mihvd.lce_backward(gout, hc, weight, bias, meta, lse, ctx.reduction, need[0], need[1],
-                                                  need[2])
-        return dh, dw, db, None, None, None
-
-
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                          bias: torch.Tensor | None = None, *, ignore_index: int = -100,
                          reduction: str = "mean") -> torch.Tensor:
@@ -70,7 +53,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     """
     if reduction not in _REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction must be one of %s (got %r)" % (_REDUCTIONS, reduction))
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError("linear_cross_entropy: hidden [..., K] and weight [V, K] are needed (got %s and %s)"
                          % (tuple(hidden.shape), tuple(weight.shape)))
     if labels.shape != hidden.shape[:-1]:
@@ -85,28 +68,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
             raise ValueError("linear_cross_entropy: every tensor must be on the GPU (got one on %s)" % b.device)
     else:
         h, w, y, b = _prepare("linear_cross_entropy", hidden, weight, labels, bias)
-    loss = _LinearCrossEntropy.apply(h.reshape(-1, h.shape[-1]), w, b, y.reshape(-1), int(ignore_index),
-                                     _REDUCTIONS.index(reduction))
-    return loss.view(labels.shape) if reduction == "none" else loss
-
-
-class _GatedFFN(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, act):
-        save = any(ctx.needs_input_grad)
-        y, g, u, h = torch.ops.mihvd.ffn_forward(x, w_gate, w_up, w_down, act, save)
-        if save:
-            ctx.save_for_backward(x, w_gate, w_up, w_down, g, u, h)
-            ctx.act = act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, w_gate, w_up, w_down, g, u, h = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*torch.ops.mihvd.ffn_backward(dy, x, w_gate, w_up, w_down, g, u, h, ctx.act, need[0], need[1], need[2],
-                                              need[3]), None)
+    if h.dim() != 2:
+        h, y = h.reshape(-1, h.shape[-1]), y.reshape(-1)
+    loss = torch.ops.mihvd.linear_cross_entropy(h, w, y, b, ignore_index, _REDUCTIONS.index(reduction))
+    return loss.view(labels.shape) if reduction == "none" and labels.dim() != 1 else loss
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
@@ -122,9 +87,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if activation not in ACTIVATIONS:
         raise ValueError("gated_ffn: activation must be one of %s (got %r)" % (ACTIVATIONS, activation))
     if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[1] != x.shape[-1] or w_up.shape != w_gate.shape or \
-            w_down.shape != (w_gate.shape[1], w_gate.shape[0]):
+            w_down.shape != (w_gate.shape[1], w_gate.shape[0]) or 0 in w_gate.shape:
         raise ValueError("gated_ffn: x [..., K], w_gate and w_up [F, K] and w_down [K, F] are needed (got %s, %s, %s, %s)"
                          % tuple(tuple(t.shape) for t in (x, w_gate, w_up, w_down)))
     x, w_gate, w_up, w_down = _prepare("gated_ffn", x, w_gate, w_up, w_down)
-    y = _GatedFFN.apply(x.reshape(-1, x.shape[-1]), w_gate, w_up, w_down, ACTIVATIONS.index(activation))
-    return y.view(x.shape)
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    y = torch.ops.mihvd.gated_ffn(flat, w_gate, w_up, w_down, ACTIVATIONS.index(activation))
+    return y if x.dim() == 2 else y.view(x.shape)
