@@ -54,6 +54,33 @@ struct Ragged {
   int start[RAG_MAX + 1];  // RAG 2: first tile of each entry; filled by launch()
 };
 
+// k splits of a product whose rows are counted on the device, by the count: the split with the least
+// estimated time (the terms of plan(), in 0.01 us) of those whose slabs fit.
+struct SplitRule {
+  int cap = 0;            // row tiles times splits that the slabs hold
+  int tile, tn, kt, cus;  // output tile, tiles along the columns, k tiles, compute units
+  int unit1, unit2, end;  // a k tile with one and with two blocks on a CU (0: never two), a tile's end
+  int N;
+};
+// Every lane of a wave prices one split. All waves that ask get the same answer.
+__device__ __forceinline__ int pick_splits(const SplitRule& r, int M) {
+  const int lane = threadIdx.x & 63, s = lane + 1;
+  const int64_t tm = (M + r.tile - 1) / r.tile, tiles = tm * r.tn * s;
+  const bool two = r.unit2 && tiles > r.cus;
+  const int slots = two ? 2 * r.cus : r.cus;
+  const int64_t rounds = (tiles + slots - 1) / slots;
+  int64_t cost = rounds * ((int64_t)((r.kt + s - 1) / s) * (two ? r.unit2 : r.unit1) + r.end);
+  cost += (int64_t)M * r.N * (2 * s + 1) / 10000;  // 8 (s + 1/2) bytes a value at 4 TB/s
+  if (s > 1 && (r.kt / s < 4 || tm * s > r.cap)) cost = INT64_MAX >> 8;
+  int64_t key = cost * 64 + lane;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_xor(key, d);
+    key = o < key ? o : key;
+  }
+  return __builtin_amdgcn_readfirstlane((int)(key & 63)) + 1;
+}
+
 struct Args {
   Side m, n;
   int M = 0, N = 0, K = 0;  // K: per segment
@@ -61,6 +88,7 @@ struct Args {
   int sym = 0;                  // out is symmetric (M == N): only tiles with nt >= mt run
   const int* dyn_m = nullptr;   // device count that replaces M (tiles past it do not run)
   const int* dyn_k = nullptr;   // device count that replaces K
+  SplitRule rule;               // with dyn_m: how the kernel itself chooses the k splits (rule.cap 0: `splits`)
   int tiles_m = 0, tiles_n = 0; // filled by launch()
 };
 
@@ -352,9 +380,9 @@ struct Tile {
 // run of tiles together, in groups of eight m tiles, so that the tiles an XCD has in flight share rows
 // of both operands in its L2. `l` counts within the XCD's run; false past its end.
 template <int RAG, int TN>
-__device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tiles_m, int K, int l, Tile& t) {
+__device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tiles_m, int splits, int K, int l, Tile& t) {
   const int tiles = a.sym ? tiles_m * (tiles_m + 1) / 2 : tiles_m * a.tiles_n;
-  const int nb = RAG == 2 ? g.start[g.count] : tiles * a.splits * a.batch, x = blockIdx.x & 7;
+  const int nb = RAG == 2 ? g.start[g.count] : tiles * splits * a.batch, x = blockIdx.x & 7;
   const int q = nb >> 3, r = nb & 7;
   if (l >= q + (x < r ? 1 : 0)) return false;
   // (an XCD's run goes up through the entries: the search starts where the last one ended)
@@ -366,11 +394,11 @@ __device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tile
     pos -= g.start[batch];
     t.N = g.len[batch];
     tiles_n = (t.N + TN - 1) / TN;
-  } else if (a.batch > 1 || a.splits > 1) {
+  } else if (a.batch > 1 || splits > 1) {
     const int e = pos / tiles;
     pos -= e * tiles;
-    batch = e / a.splits;
-    split = e - batch * a.splits;
+    batch = e / splits;
+    split = e - batch * splits;
     if constexpr (RAG == 1) t.K = g.len[batch];
   } else if constexpr (RAG == 1) {
     t.K = g.len[0];
@@ -396,8 +424,8 @@ __device__ __forceinline__ bool tile_at(const Args& a, const Ragged& g, int tile
   t.nt = uni(nt);
   t.K = uni(t.K);
   const int kts = (t.K + BK - 1) / BK * a.nseg;
-  t.it = a.splits == 1 ? 0 : uni((int)((int64_t)kts * t.split / a.splits));
-  t.end = a.splits == 1 ? kts : uni((int)((int64_t)kts * (t.split + 1) / a.splits));
+  t.it = splits == 1 ? 0 : uni((int)((int64_t)kts * t.split / splits));
+  t.end = splits == 1 ? kts : uni((int)((int64_t)kts * (t.split + 1) / splits));
   return true;
 }
 
@@ -425,6 +453,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 || PL == 2 ? 1 : 2)
   const int M = uni(a.dyn_m ? *a.dyn_m : a.M);
   const int K = uni(a.dyn_k ? *a.dyn_k : a.K);
   const int tiles_m = a.dyn_m ? (M + TM - 1) / TM : a.tiles_m;
+  const int splits = a.rule.cap ? pick_splits(a.rule, M) : a.splits;
   const Ragged* gp = nullptr;
   if constexpr (RAG != 0) gp = &rag;
   const Ragged& g = *gp;  // (not read without RAG)
@@ -432,7 +461,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 || PL == 2 ? 1 : 2)
   int l_mul = blockIdx.x >> 3, l_cpy = l_mul;  // the tile being multiplied, the tile being copied
   Tile cur, nxt;
   cur.batch = 0;
-  if (!tile_at<RAG, TN>(a, g, tiles_m, K, l_mul, cur)) return;
+  if (!tile_at<RAG, TN>(a, g, tiles_m, splits, K, l_mul, cur)) return;
   const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
@@ -484,7 +513,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 || PL == 2 ? 1 : 2)
       locate(kp == kt ? 0 : kp);
     } else {
       l_cpy += hops;
-      more = tile_at<RAG, TN>(a, g, tiles_m, K, l_cpy, nxt);
+      more = tile_at<RAG, TN>(a, g, tiles_m, splits, K, l_cpy, nxt);
       if (more) enter();
     }
   };
@@ -668,7 +697,7 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 || PL == 2 ? 1 : 2)
       }
     epi.template run<NI, MI>(c, pre, acc);
     l_mul += hops;
-    if (!tile_at<RAG, TN>(a, g, tiles_m, K, l_mul, cur)) break;
+    if (!tile_at<RAG, TN>(a, g, tiles_m, splits, K, l_mul, cur)) break;
     clear();
   }
 }
@@ -763,6 +792,21 @@ inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym,
   return best;
 }
 
+// The rule that plan()'s terms give a product with a device count of at most M rows.
+inline SplitRule split_rule(int64_t M, int64_t N, int64_t K, const Plan& p) {
+  SplitRule r;
+  r.tile = p.tile;
+  r.tn = cdiv(N, p.tile);
+  r.kt = cdiv(K, BK);
+  r.cus = device_cu_count();
+  r.unit1 = p.tile == T256 ? 145 : p.tile == T128 ? 67 : 30;
+  r.unit2 = p.tile == T256 ? 0 : p.tile == T128 ? 93 : 57;
+  r.end = p.tile == T256 ? 700 : p.tile == T128 ? 400 : 150;
+  r.N = (int)N;
+  r.cap = std::max(cdiv(M, p.tile) * p.splits, cdiv((p.tile == T256 ? 1 : 2) * r.cus, r.tn));
+  return r;
+}
+
 // ---- epilogues -----------------------------------------------------------------------------
 // An epilogue is a struct with `load` (what it reads from memory early, into a Pre: on its way while
 // the tile's copies land) and `run` (its work on the accumulators: acc[i][j][k] is column
@@ -835,7 +879,8 @@ struct EpiStore {
   }
 };
 
-// fp32 slab of one k split: slab[batch * splits + split][m][n] (+)= acc. ld is a multiple of 4.
+// fp32 slab of one k split: slab[batch * splits + split][m][n] (+)= acc. ld is a multiple of 4. With a stride
+// of 0 the slabs are as long as the device's count of rows.
 struct EpiSlab {
   float* slab;
   int64_t ld, stride;
@@ -846,7 +891,7 @@ struct EpiSlab {
   __device__ __forceinline__ void load(const Ctx&, Pre<NI, MI>&) const {}
   template <int NI, int MI>
   __device__ __forceinline__ void run(const Ctx& c, const Pre<NI, MI>&, f32x4 (&acc)[NI][MI]) const {
-    float* o = slab + (int64_t)(c.batch * splits + c.split) * stride;
+    float* o = slab + (int64_t)(c.batch * splits + c.split) * (stride ? stride : c.M * ld);
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
       const int m = c.m0 + j * 16 + (c.lane & 15);

@@ -220,9 +220,10 @@ __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ par
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % WPR;
   float total = 0.f;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < N; r0 += (int64_t)gridDim.x * RPB) {
+  const int n = out ? *cnt : N;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < n; r0 += (int64_t)gridDim.x * RPB) {
     const int64_t r = r0 + wave / WPR;
-    const int c = r < N ? inv[r] : -1;
+    const int c = r >= n ? -1 : out ? (int)r : inv[r];
     float mx = -INFINITY, s = 0.f;
     if (c >= 0) {
       const float2* q = part + (int64_t)c * npart;
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ par
       for (int i = 0; i < WPR; ++i) s += sh[i].y * __expf(sh[i].x - ref);
       __syncthreads();
     }
-    if (lane == 0 && sub == 0 && r < N) {
+    if (lane == 0 && sub == 0 && r < n) {
       float v = 0.f;
       if (c >= 0) {
         const int y = label[c];
@@ -265,8 +266,8 @@ __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ par
         lse[c] = l;
         v = l - (in ? zlab[c] : 0.f);
       }
-      rows[r] = v;
-      total += v;
+      if (out) total += v;
+      else rows[r] = v;
     }
   }
   if (!out) return;
@@ -387,13 +388,15 @@ struct EpiDz {
 
 // The ends of the two gradients that are summed up: blocks below `dh_blocks` write dh of every row, the sum of
 // its slabs or zeros where the label was ignored; the others db of a piece of the vocabulary.
-__global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __restrict__ slab, int nslab, int64_t stride,
-                                                 int64_t ld, const int* __restrict__ inv, int N, int K,
+__global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __restrict__ slab,
+                                                 const g16::SplitRule rule, int64_t ld, const int* __restrict__ inv, int N, int K,
                                                  u16* __restrict__ dh, const float* __restrict__ dbp, int64_t ldb, int tm,
                                                  int V, void* __restrict__ db, int kind, const int* __restrict__ cnt,
                                                  const LceGrad g) {
   const float scale = g16::scalar(g.scale, g.div) * (1.f / DZ_SCALE);
+  const int rows = *cnt;
   if ((int)blockIdx.x < dh_blocks) {
+    const int nslab = g16::pick_splits(rule, rows);
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int k4 = (K + 3) / 4;
     const int64_t r = i / k4;
@@ -402,7 +405,17 @@ __global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __r
     const int c = inv[r];
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (c >= 0) {
-      for (int q = 0; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(slab + q * stride + (int64_t)c * ld + k);
+      const int64_t stride = (int64_t)rows * ld;
+      const float* p = slab + (int64_t)c * ld + k;
+      int q = 0;
+      for (; q + 8 <= nslab; q += 8) {  // eight loads in flight
+        f32x4 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(p + (q + e) * stride);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[e];
+      }
+      for (; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(p + q * stride);
       s *= scale;
     }
     g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
@@ -410,7 +423,7 @@ __global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __r
   }
   const int64_t v = (int64_t)(blockIdx.x - dh_blocks) * 256 + threadIdx.x;
   if (v >= V) return;
-  const int n = (*cnt + tm - 1) / tm * 2;  // two waves along a tile's rows
+  const int n = (rows + tm - 1) / tm * 2;  // two waves along a tile's rows
   float s = 0.f;
   for (int i = 0; i < n; ++i) s += dbp[(int64_t)i * ldb + v];
   s *= scale;
@@ -439,6 +452,7 @@ void lce_plan_backward(LceShape& s, LceScratch& x, bool bias) {
   const g16::Plan p = g16::plan(s.N, s.K, x.piece, 1, 1, false, true);
   x.dh_tile = p.tile;
   x.splits = p.splits;
+  x.slab_rows = (int64_t)g16::split_rule(s.N, s.K, x.piece, p).cap * p.tile;
   x.dw_tile = g16::plan(std::min(x.piece, s.V), s.K, s.N, 1, 1, false, false).tile;
 }
 #endif
@@ -463,17 +477,21 @@ void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, co
   a.dyn_m = rw.cnt;
   if (bias) g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<true>{bias, bias_kind, rw.label, part, s.npart, zlab}, st);
   else g16::launch<g16::KC, g16::KC>(s.tile, a, EpiStats<false>{nullptr, 0, rw.label, part, s.npart, zlab}, st);
-  if (s.N <= 1024)
-    lce_finish<4><<<s.N, 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows, blocks, rw.done, rw.cnt,
-                                       mean, loss);
-  else
-    lce_finish<1><<<std::min(g16::cdiv(s.N, 4), LCE_BLOCKS), 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V,
-                                                                           lse, rows, blocks, rw.done, rw.cnt, mean, loss);
+  auto finish = [&](auto kernel, int grid) {
+    kernel<<<grid, 256, 0, st>>>(part, s.npart, zlab, rw.label, rw.inv, s.N, s.V, lse, rows, blocks, rw.done, rw.cnt, mean,
+                                 loss);
+  };
+  if (s.N <= LCE_BLOCKS) finish(lce_finish<4>, s.N);
+  else finish(lce_finish<1>, std::min(g16::cdiv(s.N, 4), loss ? LCE_BLOCKS : 4096));
 }
 
 void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, const u16* hc, const u16* w, int64_t ldw,
                      const void* bias, int bias_kind, const float* lse, const LceScratch& x, u16* dh, u16* dw, void* db,
                      hipStream_t st) {
+  // The slabs of all pieces add up, so one rule serves them all: as many splits as suit the labelled rows, which are
+  // often few among all (with the head over 8192 positions, 1229 of them labelled, 138 us with the
+  // splits that suit 8192 rows).
+  const g16::SplitRule rule = g16::split_rule(s.N, s.K, x.piece, {x.dh_tile, x.splits});
   for (int v0 = 0, first = 1; v0 < s.V; v0 += x.piece, first = 0) {
     const int nv = std::min(x.piece, s.V - v0);
     const u16* wp = w + (int64_t)v0 * ldw;
@@ -525,9 +543,10 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       a.M = s.N;
       a.N = s.K;
       a.K = nv;
-      a.splits = x.splits;
+      a.splits = 64;  // as many as the rule can choose: every slot gets a block
       a.dyn_m = rw.cnt;
-      g16::EpiSlab e{x.slab, s.K8, (int64_t)s.N * s.K8, x.splits, first ? 0 : 1};
+      a.rule = rule;
+      g16::EpiSlab e{x.slab, s.K8, 0, 1, first ? 0 : 1};
       g16::launch<g16::KC, g16::KS>(x.dh_tile, a, e, st);
     }
     // the pieces' slabs add up: dh is whole behind the last one
@@ -535,8 +554,8 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
     const int db_blocks = db ? g16::cdiv(nv, 256) : 0;
     void* dbv = db ? static_cast<char*>(db) + (int64_t)v0 * (bias_kind == 1 ? 4 : 2) : nullptr;
     if (dh_blocks + db_blocks)
-      lce_grads<<<dh_blocks + db_blocks, 256, 0, st>>>(dh_blocks, x.slab, x.splits, (int64_t)s.N * s.K8, s.K8, rw.inv, s.N,
-                                                       s.K, dh, x.dbp, x.ldz, x.dz_tile, nv, dbv, bias_kind, rw.cnt, g);
+      lce_grads<<<dh_blocks + db_blocks, 256, 0, st>>>(dh_blocks, x.slab, rule, s.K8, rw.inv, s.N, s.K, dh, x.dbp, x.ldz,
+                                                       x.dz_tile, nv, dbv, bias_kind, rw.cnt, g);
   }
 }
 

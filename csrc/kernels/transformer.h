@@ -17,7 +17,7 @@ struct LceShape {
   int tile, npart;  // of the logits: output tile, (max, sum) pairs per row (two waves along a tile)
   int chunk;        // rows whose labels are counted ahead, or 0: each block counts for itself
 };
-constexpr int LCE_BLOCKS = 1024;  // that share the end of the forward pass: partial sums of the loss
+constexpr int LCE_BLOCKS = 256;  // that share the end of the forward pass: partial sums of the loss
 // The labelled rows: compact position -> row, row -> compact position or -1, their labels and count.
 struct LceRows {
   const int* idx;
@@ -41,7 +41,8 @@ struct LceScratch {
   u16* dz;       // [N][ldz]
   float* dbp;    // [2 * tiles of rows][ldz]
   int splits, dz_tile, dh_tile, dw_tile;
-  float* slab;   // [splits][N][K8]
+  int64_t slab_rows;  // that the splits of dh need at any count of labelled rows
+  float* slab;        // [slab_rows][K8]
 };
 
 // How the products of a shape run (tiles, k splits of the hidden gradient); x.piece is set.

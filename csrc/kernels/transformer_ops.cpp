@@ -135,7 +135,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   // the chunks (at most 4096) are counted ahead, which costs a launch.
   if (N > 16384) s.chunk = (int)(cdiv(cdiv(N, 4096), 1024) * 1024);
   const int64_t nmeta = 3 * N + 2 + (s.chunk ? cdiv(N, s.chunk) : 0);
-  at::Tensor rows = at::empty({N}, f32), loss = reduction ? at::empty({}, f32) : rows;
+  at::Tensor loss = reduction ? at::empty({}, f32) : at::empty({N}, f32);
   at::Tensor hc = at::empty({N, K8}, h.options()), lse = at::empty({N}, f32);
   at::Tensor meta = at::empty({nmeta}, h.options().dtype(at::kInt));
   if (N == 0) {
@@ -155,8 +155,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   auto run = h.scalar_type() == at::kHalf ? &f16::lce_forward_16 : &lce_forward_16;
   run(s, lab.data_ptr<int64_t>(), ignore_index, rw, p16(h), h.stride(0), h.stride(1), wm.p, wm.ld,
       bias ? bias->data_ptr() : nullptr, bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part), zlab,
-      lse.data_ptr<float>(), rows.data_ptr<float>(), blocks, reduction ? loss.data_ptr<float>() : nullptr, reduction == 1,
-      st);
+      lse.data_ptr<float>(), reduction ? nullptr : loss.data_ptr<float>(), blocks,
+      reduction ? loss.data_ptr<float>() : nullptr, reduction == 1, st);
   return {loss, hc, meta, lse};
 }
 
@@ -209,7 +209,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
     x.dbp = dbp.data_ptr<float>();
   }
   if (need_h) {
-    slab = at::empty({x.splits, N, K8}, f32);
+    slab = at::empty({x.slab_rows, K8}, f32);
     x.slab = slab.data_ptr<float>();
   }
   auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
