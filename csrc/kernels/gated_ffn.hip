@@ -188,6 +188,111 @@ struct EpiGateGrad {
   }
 };
 
+// Few rows (serving): a block of eight waves per 16 columns, each wave an eighth of k, its fragments
+// straight from memory: a lane's 16 bytes are eight consecutive k of one weight row, and every weight is
+// read once, so LDS would only add a trip. Two launches, each a memory latency or two long: one row of
+// 768 through 2048 columns takes 7.9 us in a graph (1.2 TB/s; through the core's tiles, 64 rows high, k cut
+// by splits with a third launch, 20 us), of 2048 through 5632 22 us (3.1 TB/s). The rows are read again
+// by every block: at 32 rows 13 and 40 us (core: 22 and 48), at 64 rows 18 and 58, so up to 32 come here.
+// MB: groups of 16 rows.
+template <int MB, bool DUAL, class Out>
+__device__ __forceinline__ void few_rows(const u16* __restrict__ x, int64_t ldx, int N, const u16* __restrict__ w0,
+                                         const u16* __restrict__ w1, int64_t ldw, int F, int K, const Out& out) {
+  constexpr int W = DUAL ? 2 : 1, D = 4;  // steps of 32 k whose loads are in flight together
+  __shared__ float part[8][W][MB * 256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n0 = blockIdx.x * 16, r = lane & 15, kq = 8 * (lane >> 4);
+  const int steps = (K + 31) / 32, first = steps * wave / 8, last = steps * (wave + 1) / 8;
+  const u16* pw[W];
+  pw[0] = w0 + (int64_t)min(n0 + r, F - 1) * ldw;
+  if constexpr (DUAL) pw[1] = w1 + (int64_t)min(n0 + r, F - 1) * ldw;
+  const u16* px[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) px[b] = x + (int64_t)min(b * 16 + r, N - 1) * ldx;
+  f32x4 acc[W][MB];
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) acc[i][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = first; s < last; s += D) {
+    bf16x8 fw[D][W], fx[D][MB];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      // rows are whole up to the next multiple of 8 past K, zeros there; nothing is read behind that
+      const int k = (s + d) * 32 + kq;
+      const bool on = s + d < last && k < K;
+#pragma unroll
+      for (int i = 0; i < W; ++i) fw[d][i] = on ? *reinterpret_cast<const bf16x8*>(pw[i] + k) : bf16x8{};
+#pragma unroll
+      for (int b = 0; b < MB; ++b) fx[d][b] = on ? *reinterpret_cast<const bf16x8*>(px[b] + k) : bf16x8{};
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[i][b] = mfma16(fw[d][i], fx[d][b], acc[i][b]);
+  }
+  // acc[k]: column n0 + 4 (lane >> 4) + k of row lane & 15
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+      *reinterpret_cast<f32x4*>(&part[wave][i][(b * 16 + r) * 16 + 4 * (lane >> 4)]) = acc[i][b];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MB * 256; e += 512) {
+    float v[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      v[i] = part[0][i][e];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) v[i] += part[q][i][e];
+    }
+    if ((e >> 4) < N) out(e >> 4, n0 + (e & 15), v);
+  }
+}
+
+template <int ACT, int MB>
+__global__ void __launch_bounds__(512) ffn_gate_few(const u16* __restrict__ x, int64_t ldx, int N, const u16* __restrict__ wg,
+                                                    const u16* __restrict__ wu, int64_t ldw, int F, int F8, int K,
+                                                    u16* __restrict__ g, u16* __restrict__ u, u16* __restrict__ h) {
+  few_rows<MB, true>(x, ldx, N, wg, wu, ldw, F, K, [&](int m, int n, const float (&v)[2]) {
+    if (n >= F8) return;
+    const int64_t o = (int64_t)m * F8 + n;
+    const bool in = n < F;  // columns F..F8: zeros for the next product
+    float a, d;
+    act_both<ACT>(v[0], a, d);
+    h[o] = in ? f2bf(a * v[1]) : (u16)0;
+    if (g) {
+      g[o] = in ? f2bf(v[0]) : (u16)0;
+      u[o] = in ? f2bf(v[1]) : (u16)0;
+    }
+  });
+}
+template <int MB>
+__global__ void __launch_bounds__(512) ffn_down_few(const u16* __restrict__ h, int64_t ldh, int N, const u16* __restrict__ w,
+                                                    int64_t ldw, int K, int F, u16* __restrict__ y) {
+  few_rows<MB, false>(h, ldh, N, w, w, ldw, K, F, [&](int m, int n, const float (&v)[1]) {
+    if (n < K) y[(int64_t)m * K + n] = f2bf(v[0]);
+  });
+}
+
+template <int MB>
+void forward_few(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, int act, u16* g, u16* u, u16* h, u16* y,
+                 hipStream_t st) {
+  auto gate = [&](auto A) {
+    ffn_gate_few<A.value, MB><<<g16::cdiv(s.F8, 16), 512, 0, st>>>(x, ldx, s.N, w.gate, w.up, w.ldgu, s.F, s.F8, s.K, g, u, h);
+  };
+  switch (act) {
+    case ACT_SILU: gate(std::integral_constant<int, ACT_SILU>{}); break;
+    case ACT_GELU: gate(std::integral_constant<int, ACT_GELU>{}); break;
+    case ACT_GELU_TANH: gate(std::integral_constant<int, ACT_GELU_TANH>{}); break;
+    case ACT_RELU: gate(std::integral_constant<int, ACT_RELU>{}); break;
+    default: gate(std::integral_constant<int, ACT_SIGMOID>{}); break;
+  }
+  ffn_down_few<MB><<<g16::cdiv(s.K, 16), 512, 0, st>>>(h, s.F8, s.N, w.down, w.ldd, s.K, s.F, y);
+}
+
 g16::Side side(const u16* p, int64_t ld, int ext) {
   g16::Side s;
   s.p[0] = p;
@@ -224,6 +329,8 @@ void grad_gate(const FfnShape& s, const u16* dy, int64_t lddy, const FfnWeights&
 
 void ffn_forward_16(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, int act, u16* g, u16* u, u16* h,
                     u16* y, c10::Device dev, hipStream_t st) {
+  if (s.N <= 16) return forward_few<1>(s, x, ldx, w, act, g, u, h, y, st);
+  if (s.N <= 32) return forward_few<2>(s, x, ldx, w, act, g, u, h, y, st);
   switch (act) {
     case ACT_SILU: up_gate<ACT_SILU>(s, x, ldx, w, g, u, h, st); break;
     case ACT_GELU: up_gate<ACT_GELU>(s, x, ldx, w, g, u, h, st); break;

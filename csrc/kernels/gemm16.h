@@ -61,8 +61,9 @@ struct SplitRule {
   int tile, tn, kt, cus;  // output tile, tiles along the columns, k tiles, compute units
   int unit1, unit2, end;  // a k tile with one and with two blocks on a CU (0: never two), a tile's end
   int N;
+  int* chosen;            // where the kernel leaves its choice for the one that sums the slabs
 };
-// Every lane of a wave prices one split. All waves that ask get the same answer.
+// Every lane of a wave prices one split; all waves get the same answer.
 __device__ __forceinline__ int pick_splits(const SplitRule& r, int M) {
   const int lane = threadIdx.x & 63, s = lane + 1;
   const int64_t tm = (M + r.tile - 1) / r.tile, tiles = tm * r.tn * s;
@@ -453,7 +454,11 @@ __global__ void __launch_bounds__(256, TM * TN > 128 * 128 || PL == 2 ? 1 : 2)
   const int M = uni(a.dyn_m ? *a.dyn_m : a.M);
   const int K = uni(a.dyn_k ? *a.dyn_k : a.K);
   const int tiles_m = a.dyn_m ? (M + TM - 1) / TM : a.tiles_m;
-  const int splits = a.rule.cap ? pick_splits(a.rule, M) : a.splits;
+  int splits = a.splits;
+  if (a.rule.cap) {
+    splits = pick_splits(a.rule, M);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.rule.chosen = splits;
+  }
   const Ragged* gp = nullptr;
   if constexpr (RAG != 0) gp = &rag;
   const Ragged& g = *gp;  // (not read without RAG)
@@ -793,8 +798,9 @@ inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym,
 }
 
 // The rule that plan()'s terms give a product with a device count of at most M rows.
-inline SplitRule split_rule(int64_t M, int64_t N, int64_t K, const Plan& p) {
+inline SplitRule split_rule(int64_t M, int64_t N, int64_t K, const Plan& p, int* chosen) {
   SplitRule r;
+  r.chosen = chosen;
   r.tile = p.tile;
   r.tn = cdiv(N, p.tile);
   r.kt = cdiv(K, BK);

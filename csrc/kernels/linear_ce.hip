@@ -389,14 +389,14 @@ struct EpiDz {
 // The ends of the two gradients that are summed up: blocks below `dh_blocks` write dh of every row, the sum of
 // its slabs or zeros where the label was ignored; the others db of a piece of the vocabulary.
 __global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __restrict__ slab,
-                                                 const g16::SplitRule rule, int64_t ld, const int* __restrict__ inv, int N, int K,
+                                                 const int* __restrict__ splits, int64_t ld, const int* __restrict__ inv, int N, int K,
                                                  u16* __restrict__ dh, const float* __restrict__ dbp, int64_t ldb, int tm,
                                                  int V, void* __restrict__ db, int kind, const int* __restrict__ cnt,
                                                  const LceGrad g) {
   const float scale = g16::scalar(g.scale, g.div) * (1.f / DZ_SCALE);
   const int rows = *cnt;
   if ((int)blockIdx.x < dh_blocks) {
-    const int nslab = g16::pick_splits(rule, rows);
+    const int nslab = *splits;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int k4 = (K + 3) / 4;
     const int64_t r = i / k4;
@@ -452,7 +452,7 @@ void lce_plan_backward(LceShape& s, LceScratch& x, bool bias) {
   const g16::Plan p = g16::plan(s.N, s.K, x.piece, 1, 1, false, true);
   x.dh_tile = p.tile;
   x.splits = p.splits;
-  x.slab_rows = (int64_t)g16::split_rule(s.N, s.K, x.piece, p).cap * p.tile;
+  x.slab_rows = (int64_t)g16::split_rule(s.N, s.K, x.piece, p, nullptr).cap * p.tile;
   x.dw_tile = g16::plan(std::min(x.piece, s.V), s.K, s.N, 1, 1, false, false).tile;
 }
 #endif
@@ -491,7 +491,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
   // The slabs of all pieces add up, so one rule serves them all: as many splits as suit the labelled rows, which are
   // often few among all (with the head over 8192 positions, 1229 of them labelled, 138 us with the
   // splits that suit 8192 rows).
-  const g16::SplitRule rule = g16::split_rule(s.N, s.K, x.piece, {x.dh_tile, x.splits});
+  const g16::SplitRule rule = g16::split_rule(s.N, s.K, x.piece, {x.dh_tile, x.splits}, x.chosen);
   for (int v0 = 0, first = 1; v0 < s.V; v0 += x.piece, first = 0) {
     const int nv = std::min(x.piece, s.V - v0);
     const u16* wp = w + (int64_t)v0 * ldw;
@@ -554,7 +554,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
     const int db_blocks = db ? g16::cdiv(nv, 256) : 0;
     void* dbv = db ? static_cast<char*>(db) + (int64_t)v0 * (bias_kind == 1 ? 4 : 2) : nullptr;
     if (dh_blocks + db_blocks)
-      lce_grads<<<dh_blocks + db_blocks, 256, 0, st>>>(dh_blocks, x.slab, rule, s.K8, rw.inv, s.N, s.K, dh, x.dbp, x.ldz,
+      lce_grads<<<dh_blocks + db_blocks, 256, 0, st>>>(dh_blocks, x.slab, x.chosen, s.K8, rw.inv, s.N, s.K, dh, x.dbp, x.ldz,
                                                        x.dz_tile, nv, dbv, bias_kind, rw.cnt, g);
   }
 }

@@ -43,6 +43,7 @@ struct LceScratch {
   int splits, dz_tile, dh_tile, dw_tile;
   int64_t slab_rows;  // that the splits of dh need at any count of labelled rows
   float* slab;        // [slab_rows][K8]
+  int* chosen;        // the splits that the device chose
 };
 
 // How the products of a shape run (tiles, k splits of the hidden gradient); x.piece is set.

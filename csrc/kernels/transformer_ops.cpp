@@ -63,7 +63,7 @@ Mat mat(const at::Tensor& t, bool force = false) {
 void check16(const at::Tensor& t, const char* op, const char* name, const at::Tensor& like, int64_t dim) {
   TORCH_CHECK_VALUE(t.dim() == dim, op, ": ", name, " must have ", dim, " dimensions (got ", t.dim(), ")");
   TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": ", name,
-                   " must be bfloat16 or float16 (got ", t.scalar_type(), ")");
+                   " must be bfloat16 or float16 outside autocast (got ", t.scalar_type(), ")");
   TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), op, ": ", name, " must have the type of the first argument");
   TORCH_CHECK_VALUE(t.device() == like.device() && t.is_cuda(), op, ": ", name, " must be on the same GPU");
 }
@@ -209,8 +209,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
     x.dbp = dbp.data_ptr<float>();
   }
   if (need_h) {
-    slab = at::empty({x.slab_rows, K8}, f32);
+    slab = at::empty({x.slab_rows * K8 + 1}, f32);
     x.slab = slab.data_ptr<float>();
+    x.chosen = reinterpret_cast<int*>(x.slab + x.slab_rows * K8);
   }
   auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
   run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias), lse.data_ptr<float>(), x, m16(dh),

@@ -17,22 +17,31 @@ import torch
 from .. import _native
 
 ACTIVATIONS = ("silu", "gelu", "gelu_tanh", "relu", "sigmoid")
-_REDUCTIONS = ("none", "mean", "sum")
+_ACTIVATION = {name: i for i, name in enumerate(ACTIVATIONS)}
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _prepare(op, *tensors):
-    """Check the device and apply autocast's cast to the floating matrices of a call."""
-    first = tensors[0]
+_ops = {}
+
+
+def _op(name):
+    op = _ops.get(name)
+    if op is None:
+        _native.require_kernels()
+        op = _ops[name] = getattr(torch.ops.mihvd, name).default
+    return op
+
+
+def _on_gpu(op, *tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError("%s: every tensor must be on the GPU (got one on %s)" % (op, t.device))
-    _native.require_kernels()
-    if torch.is_autocast_enabled("cuda"):
-        dt = torch.get_autocast_dtype("cuda")
-        return [t if t is None or t.dtype == dt or not t.is_floating_point() else t.to(dt) for t in tensors]
-    if first.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError("%s: bfloat16 or float16 inputs are needed outside autocast (got %s)" % (op, first.dtype))
-    return list(tensors)
+
+
+def _autocast(*tensors):
+    """Autocast's cast of the floating matrices of a call."""
+    dt = torch.get_autocast_dtype("cuda")
+    return [t if t is None or t.dtype == dt or not t.is_floating_point() else t.to(dt) for t in tensors]
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
@@ -52,7 +61,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     captured in a HIP graph; results repeat bit for bit.
     """
     if reduction not in _REDUCTIONS:
-        raise ValueError("linear_cross_entropy: reduction must be one of %s (got %r)" % (_REDUCTIONS, reduction))
+        raise ValueError("linear_cross_entropy: reduction must be one of %s (got %r)" % (tuple(_REDUCTIONS), reduction))
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError("linear_cross_entropy: hidden [..., K] and weight [V, K] are needed (got %s and %s)"
                          % (tuple(hidden.shape), tuple(weight.shape)))
@@ -61,16 +70,16 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
                          % (tuple(hidden.shape[:-1]), tuple(labels.shape)))
     if labels.dtype != torch.int64:
         raise TypeError("linear_cross_entropy: labels must be int64 (got %s)" % labels.dtype)
-    if bias is not None and bias.dtype == torch.float32:
-        h, w, y = _prepare("linear_cross_entropy", hidden, weight, labels)
-        b = bias
-        if not b.is_cuda:
-            raise ValueError("linear_cross_entropy: every tensor must be on the GPU (got one on %s)" % b.device)
-    else:
-        h, w, y, b = _prepare("linear_cross_entropy", hidden, weight, labels, bias)
-    if h.dim() != 2:
-        h, y = h.reshape(-1, h.shape[-1]), y.reshape(-1)
-    loss = torch.ops.mihvd.linear_cross_entropy(h, w, y, b, ignore_index, _REDUCTIONS.index(reduction))
+    _on_gpu("linear_cross_entropy", hidden, weight, labels, bias)
+    if torch.is_autocast_enabled("cuda"):
+        if bias is None or bias.dtype == torch.float32:
+            hidden, weight = _autocast(hidden, weight)
+        else:
+            hidden, weight, bias = _autocast(hidden, weight, bias)
+    if hidden.dim() != 2:
+        hidden = hidden.reshape(-1, hidden.shape[-1])
+    flat = labels if labels.dim() == 1 else labels.reshape(-1)
+    loss = _op("linear_cross_entropy")(hidden, weight, flat, bias, ignore_index, _REDUCTIONS[reduction])
     return loss.view(labels.shape) if reduction == "none" and labels.dim() != 1 else loss
 
 
@@ -84,13 +93,16 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     without gradients only the product is written. From one row up; results repeat bit for bit and
     the call can be captured in a HIP graph.
     """
-    if activation not in ACTIVATIONS:
+    if activation not in _ACTIVATION:
         raise ValueError("gated_ffn: activation must be one of %s (got %r)" % (ACTIVATIONS, activation))
-    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[1] != x.shape[-1] or w_up.shape != w_gate.shape or \
-            w_down.shape != (w_gate.shape[1], w_gate.shape[0]) or 0 in w_gate.shape:
+    k = x.shape[-1] if x.dim() else 0
+    if w_gate.dim() != 2 or w_gate.shape[1] != k or w_up.shape != w_gate.shape or w_down.shape != (k, w_gate.shape[0]) or \
+            0 in w_gate.shape:
         raise ValueError("gated_ffn: x [..., K], w_gate and w_up [F, K] and w_down [K, F] are needed (got %s, %s, %s, %s)"
                          % tuple(tuple(t.shape) for t in (x, w_gate, w_up, w_down)))
-    x, w_gate, w_up, w_down = _prepare("gated_ffn", x, w_gate, w_up, w_down)
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    y = torch.ops.mihvd.gated_ffn(flat, w_gate, w_up, w_down, ACTIVATIONS.index(activation))
-    return y if x.dim() == 2 else y.view(x.shape)
+    _on_gpu("gated_ffn", x, w_gate, w_up, w_down)
+    if torch.is_autocast_enabled("cuda"):
+        x, w_gate, w_up, w_down = _autocast(x, w_gate, w_up, w_down)
+    if x.dim() == 2:
+        return _op("gated_ffn")(x, w_gate, w_up, w_down, _ACTIVATION[activation])
+    return _op("gated_ffn")(x.reshape(-1, k), w_gate, w_up, w_down, _ACTIVATION[activation]).view(x.shape)
