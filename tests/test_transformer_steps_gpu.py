@@ -1,6 +1,10 @@
 """linear_cross_entropy, gated_ffn and Muon used together on the GPU, and the calls around them: captured and
 replayed steps, streams, inference mode, two calls at once, many rows, differences, refusals."""
+import json
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -288,7 +292,7 @@ def test_bert_step_with_all_three(ffn):
         with torch.autocast("cuda", torch.bfloat16):
             loss = model(ids, labels)
         loss.backward()
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
         grads.append([p.grad.detach().clone() for p in model.parameters()])
         del loss
     # a logit rounded to bf16 is off by 2^-8 of it; a row's loss is the difference of two such means
@@ -305,3 +309,17 @@ def test_bert_step_with_all_three(ffn):
         o.step()
     moved = [not torch.equal(p, q) for p, q in zip(model.parameters(), before)]
     assert all(m or not g.any() for m, g in zip(moved, grads[0]))
+
+
+def test_stress_benchmark_with_all_three():
+    """The stress benchmark's BERT step with the gated block, the fused loss and Muon, replayed from a graph."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=root)
+    for k in ("RANK", "WORLD_SIZE", "MASTER_PORT"):
+        env.pop(k, None)
+    p = subprocess.run([sys.executable, os.path.join(root, "benchmarks", "stress_models.py"), "--model", "bert-base",
+                        "--steps", "3", "--warmup", "3", "--batch-size", "2", "--graph", "--bert-ffn", "swiglu", "--bert-loss",
+                        "fused", "--optimizer", "muon"], env=env, capture_output=True, text=True, timeout=110)
+    assert p.returncode == 0, p.stdout[-2000:] + p.stderr[-2000:]
+    rec = json.loads(p.stdout.strip().splitlines()[-1])
+    assert rec["config"]["optimizer"] == "muon" and math.isfinite(rec["config"]["final_loss"])
