@@ -25,9 +25,9 @@ MIHVD_OPNS_BEGIN
 
 namespace {
 #ifdef MIHVD_F16
-constexpr float DZ_SCALE = 16384.f;
+constexpr float DZ_SCALE = 16384.f, DZ_LOG2 = 14.f;
 #else
-constexpr float DZ_SCALE = 1.f;
+constexpr float DZ_SCALE = 1.f, DZ_LOG2 = 0.f;
 #endif
 
 // Sum of n over a block of 1024, for every thread.
@@ -144,6 +144,21 @@ __device__ __forceinline__ bool mine(const g16::Ctx& c, int lab, int& d) {
   return d >= 0 && d < NI * 16 && (d & 15) < 4;
 }
 
+// A value with lane ^ 16's and lane ^ 32's joined to it, without a trip through LDS: a swap of two copies
+// of v gives every lane the even and the odd rows' (the lower and the upper half's) values.
+template <class F>
+__device__ __forceinline__ float join_rows(float v, const F& f) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// exp(z - ref) with c = ref log2(e): one fma and one exponential to the base 2. The rounding of c, 2^-24 of it, is as
+// small as the rounding of lse itself, which c belongs to.
+constexpr float LOG2E = 1.44269504f;
+__device__ __forceinline__ float exp_from(float z, float c) { return __builtin_amdgcn_exp2f(fmaf(z, LOG2E, -c)); }
+
 // Statistics of one wave's columns: part[row][piece] = (max, sum of exp(z - max)), and the label's logit.
 // About nine vector instructions a logit, the exponential four of their time: with one wave a SIMD
 // that is a third of the products' time at K = 768.
@@ -188,17 +203,15 @@ struct EpiStats {
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) mx = fmaxf(mx, z[i][k]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float ref = mx == -INFINITY ? 0.f : mx;  // a row of -inf adds nothing, without inf - inf
+      mx = join_rows(mx, [](float a, float b) { return fmaxf(a, b); });
+      const float ref = (mx == -INFINITY ? 0.f : mx) * LOG2E;  // a row of -inf adds nothing, without inf - inf
       f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s4[k] += __expf(z[i][k] - ref);
+        for (int k = 0; k < 4; ++k) s4[k] += exp_from(z[i][k], ref);
       float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      s += __shfl_xor(s, 16);
-      s += __shfl_xor(s, 32);
+      s = join_rows(s, [](float a, float b) { return a + b; });
       if (c.lane < 16 && m < c.M) part[(int64_t)m * npart + slot] = make_float2(mx, s);
     });
   }
@@ -336,13 +349,13 @@ struct EpiDz {
       constexpr int j = J.value;
       g16::pin(acc, j);
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      const float ls = DZ_SCALE == 1.f ? p.ls[j] : p.ls[j] - __logf(DZ_SCALE);
+      const float ls = p.ls[j] * LOG2E - DZ_LOG2;
       f32x4 z[NI];
       logits(c, p.b, acc, j, z);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) z[i][k] = __expf(z[i][k] - ls);
+        for (int k = 0; k < 4; ++k) z[i][k] = exp_from(z[i][k], ls);
       int d;
       if (mine<NI>(c, p.lab[j] - v0, d)) {
 #pragma unroll
