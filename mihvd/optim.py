@@ -258,6 +258,16 @@ class FusedSGD(torch.optim.Optimizer):
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
+def _ns_coefficients(op, coefficients):
+    """The three as floats. A step's matrix a I + b A + c A A is held in fp16 scaled by 2^12, which ends at 16."""
+    if len(coefficients) != 3:
+        raise ValueError("%s: three coefficients are needed" % op)
+    abc = tuple(float(v) for v in coefficients)
+    if not sum(map(abs, abc)) <= 15:
+        raise ValueError("%s: the coefficients' magnitudes must not add up to more than 15 (got %s)" % (op, abc))
+    return abc
+
+
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
                   precision: str | None = None) -> torch.Tensor:
     """The matrix (or each matrix of a batch, [..., rows, cols]) with its singular values driven towards
@@ -277,11 +287,11 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
         raise TypeError("orthogonalize: float32, bfloat16 or float16 is needed (got %s)" % x.dtype)
     if precision not in (None, "fp32", "fp16"):
         raise ValueError("orthogonalize: precision must be 'fp32' or 'fp16' (got %r)" % (precision,))
-    if len(coefficients) != 3:
-        raise ValueError("orthogonalize: three coefficients are needed")
     if not 0 <= int(steps) <= 100:
         raise ValueError("orthogonalize: steps must be within 0..100 (got %r)" % (steps,))
-    a, b, c = (float(v) for v in coefficients)
+    a, b, c = _ns_coefficients("orthogonalize", coefficients)
+    if not x.numel():
+        return x.detach().clone()
     if x.is_cuda:
         from . import _native
 
@@ -311,9 +321,10 @@ class Muon(torch.optim.Optimizer):
     than two dimensions count as [first, rest]. Vectors, embeddings and heads belong to another
     optimizer (``FusedAdam``); parameters of fewer than two dimensions are refused.
 
-    fp32 contiguous GPU parameters take one fused path (``torch.ops.mihvd.muon_step``: matrices of one
-    shape run together, momentum, products and weight update in the kernels, no host
-    synchronisation, capturable); others use torch operations around :func:`orthogonalize`.
+    fp32 contiguous GPU parameters take one fused path (``torch.ops.mihvd.muon_step``: matrices of like
+    smaller sides run together, momentum, products and weight update in the kernels, no host
+    synchronisation, capturable from the second step on, with the learning rate it then has); others use
+    torch operations around :func:`orthogonalize`.
     ``precision`` is that of the products (see there).
     """
 
@@ -327,10 +338,9 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("Muon: scale must be 'spectral' or 'rms'")
         if precision not in ("fp32", "fp16"):
             raise ValueError("Muon: precision must be 'fp32' or 'fp16'")
-        if len(ns_coefficients) != 3:
-            raise ValueError("Muon: three ns_coefficients are needed")
+        ns_coefficients = _ns_coefficients("Muon", ns_coefficients)
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
-                                      ns_steps=int(ns_steps), ns_coefficients=tuple(ns_coefficients), eps=eps,
+                                      ns_steps=int(ns_steps), ns_coefficients=ns_coefficients, eps=eps,
                                       scale=scale, precision=precision))
 
     def add_param_group(self, group):
@@ -340,6 +350,9 @@ class Muon(torch.optim.Optimizer):
                 self.param_groups.pop()
                 raise ValueError("Muon: parameters must have at least two dimensions (got shape %s); give vectors to "
                                  "another optimizer" % (tuple(p.shape),))
+            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                self.param_groups.pop()
+                raise TypeError("Muon: parameters must be float32, bfloat16 or float16 (got %s)" % p.dtype)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -353,6 +366,9 @@ class Muon(torch.optim.Optimizer):
             for p in params:
                 st = self.state[p]
                 if "momentum_buffer" not in st:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: the first step of a parameter makes its momentum, which every replay "
+                                           "would clear; run one step before capturing")
                     st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 m = st["momentum_buffer"]
                 if p.grad.is_sparse:

@@ -53,8 +53,10 @@ def test_orthogonalize_refusals():
         orthogonalize(x, precision="bf16")
     with pytest.raises(ValueError, match="steps"):
         orthogonalize(x, steps=-1)
-    with pytest.raises(ValueError, match="coefficients"):
-        orthogonalize(x, coefficients=(1.0, 2.0))
+    for bad in ((1.0, 2.0), (9.0, -5.0, 2.0), (1.0, float("nan"), 0.0)):
+        with pytest.raises(ValueError, match="coefficients"):
+            orthogonalize(x, coefficients=bad)
+    assert orthogonalize(torch.zeros(0, 4)).shape == (0, 4) and orthogonalize(torch.zeros(2, 3, 0)).shape == (2, 3, 0)
 
 
 def test_muon_refusals_and_cpu_steps():
@@ -68,6 +70,8 @@ def test_muon_refusals_and_cpu_steps():
             Muon([w], **kw)
     with pytest.raises(ValueError, match="two dimensions"):
         Muon([w, torch.nn.Parameter(torch.zeros(4))])
+    with pytest.raises(TypeError, match="float64"):
+        Muon([torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float64))])
     opt = Muon([w], lr=0.05, momentum=0.9, weight_decay=0.1, scale="rms")
     ref, mom = w.detach().double().clone(), torch.zeros(6, 4, dtype=torch.float64)
     for k in range(3):

@@ -84,6 +84,19 @@ def test_step_captured_and_replayed():
             assert torch.equal(p, q)
 
 
+def test_first_muon_step_is_not_captured():
+    s = Stack()
+    for p in s.params():
+        p.grad = torch.ones_like(p)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(graph):
+            s.opt.step()
+    torch.cuda.synchronize()
+    s.opt.step()
+    assert all(torch.isfinite(p).all() for p in s.params())
+
+
 def test_two_graphs_share_nothing():
     """Two captured calls replayed in turn, each over its own inputs, keep their results."""
     from mihvd.ops import gated_ffn, linear_cross_entropy
@@ -309,6 +322,49 @@ def test_bert_step_with_all_three(ffn):
         o.step()
     moved = [not torch.equal(p, q) for p, q in zip(model.parameters(), before)]
     assert all(m or not g.any() for m, g in zip(moved, grads[0]))
+
+
+def test_offsets_past_32_bits():
+    """A block whose inner activations pass 2^31 elements (their gradients 2^32), and a vocabulary whose weight does:
+    the last rows come out as a small call's formula says."""
+    from mihvd.ops import gated_ffn, linear_cross_entropy
+
+    n, k, f, tail = (1 << 20) + 77, 16, 2056, 40
+    _, wg, wu, wd, _ = ffn_case(1, k, f, BF, 21)
+    x = torch.randn(n, k, device="cuda").to(BF)
+    dy = torch.randn(n, k, device="cuda").to(BF)
+    xl = x.requires_grad_()
+    y = gated_ffn(xl, wg.cuda(), wu.cuda(), wd.cuda())
+    dx, = torch.autograd.grad(y, xl, dy)
+    ref = ffn_ref(x[-tail:].detach().cpu(), wg, wu, wd, dy[-tail:].cpu(), "silu", BF)
+    close(y[-tail:], *ref[0], "y")
+    close(dx[-tail:], *ref[1], "dx")
+    del y, dx, x, xl, dy
+
+    v, k, n = (1 << 21) + 4099, 1032, 5
+    w = torch.randn(v, k, device="cuda", dtype=torch.float32).mul_(k ** -0.5).to(BF)
+    h = torch.randn(n, k, device="cuda").to(BF)
+    labels = torch.tensor([v - 1, 0, v - 3, -100, 1 << 21], device="cuda")
+    hl, wl = h.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(hl, wl, labels, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, [hl, wl])
+    assert float(dh[3].abs().max()) == 0
+    with torch.no_grad():
+        z = torch.cat([h.double() @ w[i:i + (1 << 18)].double().t() for i in range(0, v, 1 << 18)], 1)
+        p = torch.softmax(z, 1)
+        keep = labels != -100
+        zabs = 1032 * E32 * float((h.double().abs().sum(1) * w[-1000:].double().abs().max()).max())
+        lse = torch.logsumexp(z, 1)
+        want = (lse - z.gather(1, labels.clamp_min(0)[:, None]).squeeze(1))[keep]
+        rel = 2 * zabs + 2 * 2.0 ** -18 + float(lse.abs().max()) * 2.0 ** -22
+        assert abs(float(loss.double()) - float(want.sum())) <= 4 * rel + 16 * E32 * float(want.sum())
+        dz = p.scatter_add(1, labels.clamp_min(0)[:, None], torch.full((n, 1), -1.0, device="cuda", dtype=torch.float64))
+        dz *= keep[:, None]
+        for part in (slice(v - 64, v), slice(1 << 21, (1 << 21) + 64), slice(0, 64)):
+            d = dz[:, part]
+            ref = d.t() @ h.double()
+            err = (d.abs() * (2.0 ** -8 + 2.0 ** -21) + p[:, part] * keep[:, None] * rel + 2.0 ** -38).t() @ h.double().abs()
+            close(dw[part], ref.cpu(), (err * 1.01 + ref.abs() * 2.0 ** -8).cpu(), "dw")
 
 
 def test_stress_benchmark_with_all_three():
