@@ -13,12 +13,20 @@
 // are four consecutive n of one m (v_mfma_f32_16x16x32: C[4*(l>>4)+i][l&15]): packed 8-byte stores
 // along the output rows, and a reduction over n stays in the lane but for two exchanges.
 //
-// Staging is global_load_lds_dwordx4 into double-buffered swizzled LDS images. Out-of-range rows are clamped to the last row (their products only reach outputs
-// that are never stored); k positions past K are read from a page of zeros on both sides.
+// Staging is global_load_lds_dwordx4 into swizzled LDS images (two buffers; four at 64x64). Out-of-range rows
+// are clamped to the last row (their products only reach outputs that are never stored); k positions
+// past K are read from a page of zeros on both sides.
 //
-// What a caller guarantees (checked on the host by G16Side makers): 16-byte aligned bases, leading
+// What a caller guarantees (transformer_ops.cpp packs what does not fit): 16-byte aligned bases, leading
 // dimensions and KS extents that are multiples of 8 elements, KC rows that hold zeros (or any
 // finite values against zeros) from K to the next multiple of 8.
+//
+// Bound by the matrix pipe and by what a tile's end costs: plain bf16 products at 256x256 run at 1.02,
+// 1.31 and 1.45 PFLOP/s for K = 768, 2048 and 8192 (16384 square on this card's library: 1.65). A wave's
+// 128x128 part reads 32 KB of LDS for 128 MFMAs, which is half the LDS's rate; at 64x64 a wave the LDS
+// reads and the copies into it together take as long as the MFMAs, hence 256x256 wherever there are tiles
+// enough. Giving every block an equal run of k tiles across output tiles was slower at every shape tried
+// (2048 x 5632 x 16384: 427 us against 357): blocks at different k share nothing in L2.
 #pragma once
 
 #include <ATen/ATen.h>

