@@ -758,12 +758,12 @@ void launch_small(int tile, const Args& a, const Epi& e, hipStream_t stream, con
   else launch_tile<LM, LN, 128, 2, false, RAG>(a, g, e, stream);
 }
 
-// Split values (PL 2): one block a CU at either tile. A k tile, with its three products, takes about 0.85 us
-// at 128x128 and 0.42 at 64x64.
+// Split values (PL 2): one block a CU at either tile. A k tile, with its three products, takes 1.27 us at
+// 128x128 and 0.42 at 64x64, a tile's end 5.7 and 3 (K = 512 to 2048).
 inline int plan_split(int64_t tiles128, int64_t tiles64, int64_t K) {
   const int cus = device_cu_count();
   const double kt = cdiv(K, BK);
-  const double t128 = cdiv(tiles128, cus) * (kt * 0.85 + 7.0), t64 = cdiv(tiles64, cus) * (kt * 0.42 + 3.0);
+  const double t128 = cdiv(tiles128, cus) * (kt * 1.27 + 5.7), t64 = cdiv(tiles64, cus) * (kt * 0.42 + 3.0);
   return t64 < t128 ? T64 : T128;
 }
 template <int LM, int LN, int RAG = 0, class Epi>

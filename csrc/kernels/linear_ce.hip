@@ -162,7 +162,8 @@ __device__ __forceinline__ float exp_from(float z, float c) { return __builtin_a
 // Statistics of one wave's columns: part[row][piece] = (max, sum of exp(z - max)), and the label's logit.
 // A logit costs a read, half a max, an fma, an exponential (as long as four others) and an add: about 4 us a
 // 256x256 tile behind 17 us of products at K = 768. 1229 x 30522 x 768: 80 us (0.72 PFLOP/s, 600 tiles in
-// three rounds on 256 CUs); 8192 x 65536 x 1024: 0.99 to 1.08 ms (1.0 to 1.1 PFLOP/s).
+// three rounds on 256 CUs; at 128x128 75 us by itself, the same in a training step); 8192 x 65536 x 1024:
+// 0.99 to 1.08 ms (1.0 to 1.1 PFLOP/s; at 128x128 1.2 to 1.26).
 template <bool BIAS>
 struct EpiStats {
   const void* bias;
