@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""Data-parallel stress benchmarks of BASELINE.json's stretch configurations:
+"""Data-parallel stress benchmarks:
 
   * ResNet-50 synthetic ImageNet, bf16 autocast (25.6 M params: allreduce bandwidth stress)
   * BERT-base MLM, synthetic seq=512, bf16 autocast, fp16 allreduce compression (110 M params:

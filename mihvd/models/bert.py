@@ -1,5 +1,5 @@
 """BERT-base encoder + masked-LM head for the "BERT-base synthetic seq=512 on 8×MI355X (large-grad
-fusion + fp16 allreduce compression)" stretch configuration of BASELINE.json: 110 M parameters,
+fusion + fp16 allreduce compression)" stress configuration: 110 M parameters,
 440 MB of fp32 gradients per step, one embedding matrix of 94 MB — a fusion-buffer and
 compression stress test of the DP engine.
 
