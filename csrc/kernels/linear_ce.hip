@@ -3,6 +3,10 @@
 //   z = h W^T + b;   L_r = lse_r - z[r][y_r],  lse_r = log sum_v exp(z[r][v])
 //   dz = g_r (exp(z - lse) - onehot);  dh = dz W;  dW = dz^T h;  db = sum_r dz
 //
+// lse is kept as two numbers, the row's maximum and log sum exp(z - max), and the maximum is subtracted before
+// anything is scaled or rounded: logits of any size (words masked by -1e30 or the type's lowest value, all words
+// of a row masked alike) keep exact differences.
+//
 // Forward: the logits exist only as MFMA accumulators; every wave reduces its columns of a row to a
 // running (max, sum of exp) pair in fp32 and writes that pair, and the row's own label logit where
 // it holds it. A second kernel joins the pairs of a row. Backward recomputes the logits piece by
@@ -154,13 +158,16 @@ __device__ __forceinline__ float join_rows(float v, const F& f) {
   return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// exp(z - ref) with c = ref log2(e): one fma and one exponential to the base 2. The rounding of c, 2^-24 of it, is as
-// small as the rounding of lse itself, which c belongs to.
+// exp(z - top) 2^c. The difference comes first: z log2(e) and top log2(e), rounded each for itself, would be
+// off by 2^-24 of z, which is any number of powers of two where z is a large mask.
 constexpr float LOG2E = 1.44269504f;
-__device__ __forceinline__ float exp_from(float z, float c) { return __builtin_amdgcn_exp2f(fmaf(z, LOG2E, -c)); }
+__device__ __forceinline__ float exp_from(float z, float top) { return __builtin_amdgcn_exp2f((z - top) * LOG2E); }
+__device__ __forceinline__ float exp_from(float z, float top, float c) {
+  return __builtin_amdgcn_exp2f(fmaf(z - top, LOG2E, c));
+}
 
 // Statistics of one wave's columns: part[row][piece] = (max, sum of exp(z - max)), and the label's logit.
-// A logit costs a read, half a max, an fma, an exponential (as long as four others) and an add: about 4 us a
+// A logit costs a read, half a max, two for the difference, an exponential (as long as four others) and an add: about 4 us a
 // 256x256 tile behind 17 us of products at K = 768. 1229 x 30522 x 768: 80 us (0.72 PFLOP/s, 600 tiles in
 // three rounds on 256 CUs; at 128x128 75 us by itself, the same in a training step); 8192 x 65536 x 1024:
 // 0.99 to 1.08 ms (1.0 to 1.1 PFLOP/s; at 128x128 1.2 to 1.26).
@@ -206,7 +213,7 @@ struct EpiStats {
 #pragma unroll
         for (int k = 0; k < 4; ++k) mx = fmaxf(mx, z[i][k]);
       mx = join_rows(mx, [](float a, float b) { return fmaxf(a, b); });
-      const float ref = (mx == -INFINITY ? 0.f : mx) * LOG2E;  // a row of -inf adds nothing, without inf - inf
+      const float ref = mx == -INFINITY ? 0.f : mx;  // a strip of -inf adds nothing, without inf - inf
       f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -220,13 +227,13 @@ struct EpiStats {
 };
 
 // Joins the pairs of every row: WPR waves a row, four where there are few rows, so that their loads are in
-// flight together. Writes lse (compact) and the row's loss (all rows), and into `out`, if given, their sum
+// flight together. Writes lse (compact: maximum, log of the sum) and the row's loss (all rows), and into `out`, if given, their sum
 // or mean: every block adds up its rows, and the block that ends last adds up the blocks, both in a fixed
 // order.
 template <int WPR>
 __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ part, int npart,
                                                   const float* __restrict__ zlab, const int* __restrict__ label,
-                                                  const int* __restrict__ inv, int N, int V, float* __restrict__ lse,
+                                                  const int* __restrict__ inv, int N, int V, float2* __restrict__ lse,
                                                   float* __restrict__ rows, float* __restrict__ blocks,
                                                   int* __restrict__ done, const int* __restrict__ cnt, int mean,
                                                   float* __restrict__ out) {
@@ -277,9 +284,9 @@ __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ par
         const int y = label[c];
         // a label outside the vocabulary has no loss: NaN, and NaN gradients through lse
         const bool in = y >= 0 && y < V;
-        const float l = in ? logf(s) + mx : NAN;
+        const float2 l = in ? make_float2(mx, logf(s)) : make_float2(NAN, NAN);
         lse[c] = l;
-        v = l - (in ? zlab[c] : 0.f);
+        v = (l.x - (in ? zlab[c] : 0.f)) + l.y;
       }
       if (out) total += v;
       else rows[r] = v;
@@ -320,7 +327,7 @@ struct EpiDz {
   const void* bias;  // from v0 on
   int bias_kind;
   const int* label;
-  const float* lse;
+  const float2* lse;      // maximum, log of the sum
   const float* rowscale;  // g_r / G per compact row
   int v0;
   u16* dz;                // [rows][ld]
@@ -330,7 +337,8 @@ struct EpiDz {
   struct Pre {
     BiasRegs<BIAS, NI> b;
     int lab[MI];
-    float ls[MI], rs[ROWS ? MI : 1];
+    float2 ls[MI];
+    float rs[ROWS ? MI : 1];
   };
   template <int NI, int MI>
   __device__ __forceinline__ void load(const g16::Ctx& c, Pre<NI, MI>& p) const {
@@ -353,13 +361,13 @@ struct EpiDz {
       constexpr int j = J.value;
       g16::pin(acc, j);
       const int m = c.m0 + j * 16 + (c.lane & 15);
-      const float ls = p.ls[j] * LOG2E - DZ_LOG2;
+      const float top = p.ls[j].x, sub = DZ_LOG2 - p.ls[j].y * LOG2E;
       f32x4 z[NI];
       logits(c, p.b, acc, j, z);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) z[i][k] = exp_from(z[i][k], ls);
+        for (int k = 0; k < 4; ++k) z[i][k] = exp_from(z[i][k], top, sub);
       int d;
       if (mine<NI>(c, p.lab[j] - v0, d)) {
 #pragma unroll
@@ -476,7 +484,7 @@ void lce_plan_backward(LceShape& s, LceScratch& x, bool bias) {
 
 void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, const LceRowsOut& rw, const u16* h,
                     int64_t hs0, int64_t hs1, const u16* w, int64_t ldw, const void* bias, int bias_kind, u16* hc,
-                    float2* part, float* zlab, float* lse, float* rows, float* blocks, float* loss, int mean,
+                    float2* part, float* zlab, float2* lse, float* rows, float* blocks, float* loss, int mean,
                     hipStream_t st) {
   if (s.chunk) lce_count<<<g16::cdiv(s.N, s.chunk), 1024, 0, st>>>(labels, s.N, ignore, s.chunk, rw.counts);
   lce_gather<<<g16::cdiv(s.N, 16), 1024, 0, st>>>(labels, s.N, s.V, ignore, s.chunk ? rw.counts : nullptr, s.chunk, h, hs0,
@@ -503,7 +511,7 @@ void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, co
 }
 
 void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, const u16* hc, const u16* w, int64_t ldw,
-                     const void* bias, int bias_kind, const float* lse, const LceScratch& x, u16* dh, u16* dw, void* db,
+                     const void* bias, int bias_kind, const float2* lse, const LceScratch& x, u16* dh, u16* dw, void* db,
                      hipStream_t st) {
   // The slabs of all pieces add up, so one rule serves them all: as many splits as suit the labelled rows, which are
   // often few among all (with the head over 8192 positions, 1229 of them labelled, 138 us with the

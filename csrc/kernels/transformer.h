@@ -53,10 +53,10 @@ void lce_plan_backward(LceShape& s, LceScratch& x, bool bias);
 #define MIHVD_TRANSFORMER_DECLS                                                                                        \
   void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, const LceRowsOut& rw, const u16* h,      \
                       int64_t hs0, int64_t hs1, const u16* w, int64_t ldw, const void* bias, int bias_kind, u16* hc,   \
-                      float2* part, float* zlab, float* lse, float* rows, float* blocks, float* loss, int mean,        \
+                      float2* part, float* zlab, float2* lse, float* rows, float* blocks, float* loss, int mean,       \
                       hipStream_t st);                                                                                 \
   void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, const u16* hc, const u16* w,            \
-                       int64_t ldw, const void* bias, int bias_kind, const float* lse, const LceScratch& x, u16* dh,   \
+                       int64_t ldw, const void* bias, int bias_kind, const float2* lse, const LceScratch& x, u16* dh,  \
                        u16* dw, void* db, hipStream_t st);                                                             \
   void ffn_forward_16(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, int act, u16* g, u16* u,        \
                       u16* h, u16* y, c10::Device dev, hipStream_t st);                                                \

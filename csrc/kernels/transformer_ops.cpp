@@ -136,7 +136,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   if (N > 16384) s.chunk = (int)(cdiv(cdiv(N, 4096), 1024) * 1024);
   const int64_t nmeta = 3 * N + 2 + (s.chunk ? cdiv(N, s.chunk) : 0);
   at::Tensor loss = reduction ? at::empty({}, f32) : at::empty({N}, f32);
-  at::Tensor hc = at::empty({N, K8}, h.options()), lse = at::empty({N}, f32);
+  at::Tensor hc = at::empty({N, K8}, h.options()), lse = at::empty({N, 2}, f32);
   at::Tensor meta = at::empty({nmeta}, h.options().dtype(at::kInt));
   if (N == 0) {
     if (reduction) loss.fill_(reduction == 1 ? NAN : 0.f);
@@ -155,7 +155,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   auto run = h.scalar_type() == at::kHalf ? &f16::lce_forward_16 : &lce_forward_16;
   run(s, lab.data_ptr<int64_t>(), ignore_index, rw, p16(h), h.stride(0), h.stride(1), wm.p, wm.ld,
       bias ? bias->data_ptr() : nullptr, bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part), zlab,
-      lse.data_ptr<float>(), reduction ? nullptr : loss.data_ptr<float>(), blocks,
+      reinterpret_cast<float2*>(lse.data_ptr<float>()), reduction ? nullptr : loss.data_ptr<float>(), blocks,
       reduction ? loss.data_ptr<float>() : nullptr, reduction == 1, st);
   return {loss, hc, meta, lse};
 }
@@ -214,8 +214,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
     x.chosen = reinterpret_cast<int*>(x.slab + x.slab_rows * K8);
   }
   auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
-  run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias), lse.data_ptr<float>(), x, m16(dh),
-      m16(dw), need_b ? db.data_ptr() : nullptr, st);
+  run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias),
+      reinterpret_cast<const float2*>(lse.data_ptr<float>()), x, m16(dh), m16(dw), need_b ? db.data_ptr() : nullptr, st);
   return {dh, dw, db};
 }
 

@@ -1,0 +1,96 @@
+"""linear_cross_entropy, gated_ffn, orthogonalize and Muon at the ends of their ranges on the GPU: masks of any
+size over whole runs of words, sizes that every tile and piece serves, row counts past the launch limits, forward-mode
+derivatives, 16-bit parameters over many steps. Compared with the formulas in 64 bits (computed on the GPU in
+elementary operations where they are large)."""
+import math
+
+import pytest
+import torch
+
+from test_transformer_gpu import BF, E32, EXP, FP, close, floor_of, gen, half, lce_case, lce_ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _kernels():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from mihvd import _native
+
+    _native.require_kernels()
+
+
+def lce_ref_gpu(h, w, y, b, grow, dt):
+    """lce_ref with its sums on the GPU (sizes that take a CPU too long)."""
+    loss, ltol, *rest = lce_ref(h.cuda(), w.cuda(), y.cuda(), None if b is None else b.cuda(), grow.cuda(), dt)
+    return (loss.cpu(), ltol, *[tuple(t.cpu() if torch.is_tensor(t) else t for t in pair) for pair in rest])
+
+
+# Sizes whose logits run in 64, 128 and 256 wide tiles: strips of 32, 64 and 128 words to a wave.
+STRIPS = [(60, 64, 1111), (300, 100, 20000), (700, 136, 20011)]
+
+
+@pytest.mark.parametrize("low", [-1e10, -1e30, torch.finfo(BF).min, torch.finfo(torch.float32).min, -math.inf],
+                         ids=["1e10", "1e30", "bf16min", "fp32min", "inf"])
+@pytest.mark.parametrize("n,k,v", STRIPS)
+def test_lce_runs_of_masked_words(n, k, v, low):
+    """Runs of words masked by one large value, across whole strips and tiles and at the vocabulary's end: what
+    the formula gives over the words that are left; the masked words get exact zeros."""
+    from mihvd.ops import linear_cross_entropy
+
+    dt = BF if n != 300 else FP
+    h, w, y, b = lce_case(n, k, v, dt, torch.float32, seed=n)
+    off = torch.zeros(v, dtype=torch.bool)
+    off[v // 4:v // 4 + 600] = True
+    off[-300:] = True
+    left = (~off).nonzero().squeeze(1)
+    y = torch.where((y >= 0) & off[y.clamp(min=0)], left[y.clamp(min=0) % len(left)], y)
+    cnt = int((y != -100).sum())
+    scale = 64.0 if dt == FP else 1.0
+    place = torch.cumsum(~off, 0) - 1  # a word's place among those that are left
+    small = torch.where(y >= 0, place[y.clamp(min=0)], y)
+    grow = torch.full((n,), scale / cnt, dtype=torch.float64)
+    loss, ltol, dh, dw, db = lce_ref_gpu(h, w[left], small, b[left], grow, dt)
+    b[off] = low
+    bias = b.to(dt) if low == torch.finfo(BF).min and dt == BF else b
+    if bias.dtype == dt:
+        loss, ltol, dh, dw, db = lce_ref_gpu(h, w[left], small, bias[left], grow, dt)
+    leaves = [t.cuda().requires_grad_() for t in (h, w, bias)]
+    out = linear_cross_entropy(leaves[0], leaves[1], y.cuda(), leaves[2])
+    close(out, loss.sum() / cnt, ltol + n * E32 * float(loss.abs().max()), "loss")
+    gh, gw, gb = torch.autograd.grad(out, leaves, torch.tensor(scale, device="cuda"))
+    close(gh, *dh, "dh")
+    close(gw.cpu()[left], *dw, "dw")
+    close(gb.cpu()[left], *db, "db")
+    assert (gw.cpu()[off] == 0).all() and (gb.cpu()[off] == 0).all()
+
+
+@pytest.mark.parametrize("low", [-1e10, -1e30, torch.finfo(torch.float32).min, 1e30], ids=["m1e10", "m1e30", "fp32min", "p1e30"])
+@pytest.mark.parametrize("n,k,v", STRIPS)
+def test_lce_all_words_alike(n, k, v, low):
+    """Every word's bias is one value so large that the logits vanish beside it in 32 bits: the softmax is
+    uniform, the loss log v, and the gradients are those of a uniform softmax."""
+    from mihvd.ops import linear_cross_entropy
+
+    h, w, y, _ = lce_case(n, k, v, BF, None, seed=n + 1)
+    assert float((h.double() @ w.double().t()).abs().max()) < abs(low) * 2.0 ** -26
+    keep = y != -100
+    cnt = int(keep.sum())
+    leaves = [h.cuda().requires_grad_(), w.cuda().requires_grad_()]
+    b = torch.full((v,), low, device="cuda")
+    out = linear_cross_entropy(leaves[0], leaves[1], y.cuda(), b)
+    rel = 2 * EXP + math.log(v) * 2.0 ** -22
+    close(out, torch.tensor(math.log(v), dtype=torch.float64), rel + 2 * n * E32 * math.log(v), "loss")
+    gh, gw = torch.autograd.grad(out, leaves)
+    p = torch.full((n, v), 1.0 / v, dtype=torch.float64)
+    dz = p.clone()
+    dz[torch.arange(n)[keep], y[keep]] -= 1.0
+    g = (keep / cnt)[:, None]
+    err = g * (dz.abs() * (2.0 ** -8 + 2.0 ** -21) + p * rel)
+    dz = dz * g
+    acc = dz.abs() + err
+    want = dz @ w.double()
+    close(gh, want, (err + acc * v * E32) @ w.double().abs() + want.abs() * 2.0 ** -8, "dh")
+    want = dz.t() @ h.double()
+    close(gw, want, (err + acc * n * E32).t() @ h.double().abs() + want.abs() * 2.0 ** -8, "dw")
