@@ -60,46 +60,50 @@ __global__ void __launch_bounds__(1024) lce_count(const int64_t* __restrict__ la
 // Compacts the labelled rows: their row numbers, their labels in 32 bits (-1: outside the vocabulary),
 // every row's place among them, their count, and their hidden vectors. A block takes 16 rows, a wave
 // each, and counts the labels ahead of them by itself: of all rows (up to 16384 of them: 64 KB a block on
-// average, out of L2), or of its chunk on top of the chunks' counts.
+// average, out of L2), or of its chunk on top of the chunks' counts. (Blocks go round once more where there are
+// more rows than a launch of fewer than 2^32 threads has waves.)
+constexpr int64_t GATHER_BLOCKS = int64_t(1) << 21;
 __global__ void __launch_bounds__(1024) lce_gather(const int64_t* __restrict__ labels, int N, int V, int64_t ignore,
                                                    const int* __restrict__ counts, int chunk, const u16* __restrict__ h,
                                                    int64_t s0, int64_t s1, int K, int K8, const LceRowsOut rw,
                                                    u16* __restrict__ out) {
   __shared__ int sh[16], own[16];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int64_t first = (int64_t)blockIdx.x * 16;
-  int n = 0;
-  int64_t from = 0;
-  if (counts) {
-    const int c = (int)(first / chunk);
-    for (int i = t; i < c; i += 1024) n += counts[i];
-    from = (int64_t)c * chunk;
-  }
-  for (int64_t r = from + t; r < first; r += 1024) n += labels[r] != ignore;
-  const int64_t r = first + w;
-  const int64_t y = r < N ? labels[r] : ignore;
-  const bool on = y != ignore;
-  if (lane == 0) own[w] = on;
-  int pos = count_block(n, sh);  // its barriers publish own[] too
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (i < w) pos += own[i];
-  if (lane == 0 && r < N) {
-    rw.inv[r] = on ? pos : -1;
-    if (on) {
-      rw.idx[pos] = (int)r;
-      rw.label[pos] = y >= 0 && y < V ? (int)y : -1;
+  for (int64_t first = (int64_t)blockIdx.x * 16; first < N; first += (int64_t)gridDim.x * 16) {
+    int n = 0;
+    int64_t from = 0;
+    if (counts) {
+      const int c = (int)(first / chunk);
+      for (int i = t; i < c; i += 1024) n += counts[i];
+      from = (int64_t)c * chunk;
     }
-    if (r == N - 1) *rw.cnt = pos + (on ? 1 : 0);
-    if (r == 0) *rw.done = 0;
-  }
-  if (!on) return;
-  const u16* src = h + r * s0;
-  u16* dst = out + (int64_t)pos * K8;
-  if (s1 == 1 && (s0 & 7) == 0 && ((uintptr_t)h & 15) == 0 && K == K8) {
-    for (int k = lane * 8; k < K; k += 512) *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
-  } else {
-    for (int k = lane; k < K8; k += 64) dst[k] = k < K ? src[(int64_t)k * s1] : (u16)0;
+    for (int64_t r = from + t; r < first; r += 1024) n += labels[r] != ignore;
+    const int64_t r = first + w;
+    const int64_t y = r < N ? labels[r] : ignore;
+    const bool on = y != ignore;
+    if (first != (int64_t)blockIdx.x * 16) __syncthreads();  // own[] and sh[] have been read
+    if (lane == 0) own[w] = on;
+    int pos = count_block(n, sh);  // its barriers publish own[] too
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < w) pos += own[i];
+    if (lane == 0 && r < N) {
+      rw.inv[r] = on ? pos : -1;
+      if (on) {
+        rw.idx[pos] = (int)r;
+        rw.label[pos] = y >= 0 && y < V ? (int)y : -1;
+      }
+      if (r == N - 1) *rw.cnt = pos + (on ? 1 : 0);
+      if (r == 0) *rw.done = 0;
+    }
+    if (!on) continue;
+    const u16* src = h + r * s0;
+    u16* dst = out + (int64_t)pos * K8;
+    if (s1 == 1 && (s0 & 7) == 0 && ((uintptr_t)h & 15) == 0 && K == K8) {
+      for (int k = lane * 8; k < K; k += 512) *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
+    } else {
+      for (int k = lane; k < K8; k += 64) dst[k] = k < K ? src[(int64_t)k * s1] : (u16)0;
+    }
   }
 }
 
@@ -412,7 +416,9 @@ struct EpiDz {
 };
 
 // The ends of the two gradients that are summed up: blocks below `dh_blocks` write dh of every row, the sum of
-// its slabs or zeros where the label was ignored; the others db of a piece of the vocabulary.
+// its slabs or zeros where the label was ignored; the others db of a piece of the vocabulary. (Past GRAD_BLOCKS,
+// which with db's blocks stay below 2^32 threads, dh's blocks go round again.)
+constexpr int64_t GRAD_BLOCKS = int64_t(1) << 23;
 __global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __restrict__ slab,
                                                  const int* __restrict__ splits, int64_t ld, const int* __restrict__ inv, int N, int K,
                                                  u16* __restrict__ dh, const float* __restrict__ dbp, int64_t ldb, int tm,
@@ -422,28 +428,28 @@ __global__ void __launch_bounds__(256) lce_grads(int dh_blocks, const float* __r
   const int rows = *cnt;
   if ((int)blockIdx.x < dh_blocks) {
     const int nslab = *splits;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int k4 = (K + 3) / 4;
-    const int64_t r = i / k4;
-    const int k = (int)(i - r * k4) * 4;
-    if (r >= N) return;
-    const int c = inv[r];
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if (c >= 0) {
-      const int64_t stride = (int64_t)rows * ld;
-      const float* p = slab + (int64_t)c * ld + k;
-      int q = 0;
-      for (; q + 8 <= nslab; q += 8) {  // eight loads in flight
-        f32x4 v[8];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)N * k4; i += (int64_t)dh_blocks * 256) {
+      const int64_t r = i / k4;
+      const int k = (int)(i - r * k4) * 4;
+      const int c = inv[r];
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      if (c >= 0) {
+        const int64_t stride = (int64_t)rows * ld;
+        const float* p = slab + (int64_t)c * ld + k;
+        int q = 0;
+        for (; q + 8 <= nslab; q += 8) {  // eight loads in flight
+          f32x4 v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(p + (q + e) * stride);
+          for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(p + (q + e) * stride);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[e];
+          for (int e = 0; e < 8; ++e) s += v[e];
+        }
+        for (; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(p + q * stride);
+        s *= scale;
       }
-      for (; q < nslab; ++q) s += *reinterpret_cast<const f32x4*>(p + q * stride);
-      s *= scale;
+      g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
     }
-    g16::store4(dh + r * K, k, K, (K & 3) == 0, s[0], s[1], s[2], s[3]);
     return;
   }
   const int64_t v = (int64_t)(blockIdx.x - dh_blocks) * 256 + threadIdx.x;
@@ -487,7 +493,7 @@ void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, co
                     float2* part, float* zlab, float2* lse, float* rows, float* blocks, float* loss, int mean,
                     hipStream_t st) {
   if (s.chunk) lce_count<<<g16::cdiv(s.N, s.chunk), 1024, 0, st>>>(labels, s.N, ignore, s.chunk, rw.counts);
-  lce_gather<<<g16::cdiv(s.N, 16), 1024, 0, st>>>(labels, s.N, s.V, ignore, s.chunk ? rw.counts : nullptr, s.chunk, h, hs0,
+  lce_gather<<<(int)std::min<int64_t>(g16::cdiv(s.N, 16), GATHER_BLOCKS), 1024, 0, st>>>(labels, s.N, s.V, ignore, s.chunk ? rw.counts : nullptr, s.chunk, h, hs0,
                                                   hs1, s.K, s.K8, rw, hc);
   g16::Args a;
   a.m.p[0] = hc;
@@ -575,7 +581,7 @@ void lce_backward_16(const LceShape& s, const LceRows& rw, const LceGrad& g, con
       g16::launch<g16::KC, g16::KS>(x.dh_tile, a, e, st);
     }
     // the pieces' slabs add up: dh is whole behind the last one
-    const int dh_blocks = dh && v0 + nv == s.V ? g16::cdiv((int64_t)s.N * ((s.K + 3) / 4), 256) : 0;
+    const int dh_blocks = dh && v0 + nv == s.V ? (int)std::min<int64_t>(((int64_t)s.N * ((s.K + 3) / 4) + 255) / 256, GRAD_BLOCKS) : 0;
     const int db_blocks = db ? g16::cdiv(nv, 256) : 0;
     void* dbv = db ? static_cast<char*>(db) + (int64_t)v0 * (bias_kind == 1 ? 4 : 2) : nullptr;
     if (dh_blocks + db_blocks)

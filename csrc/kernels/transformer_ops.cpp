@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/library.h>
@@ -157,6 +158,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
       bias ? bias->data_ptr() : nullptr, bias_kind(bias), m16(hc), reinterpret_cast<float2*>(part), zlab,
       reinterpret_cast<float2*>(lse.data_ptr<float>()), reduction ? nullptr : loss.data_ptr<float>(), blocks,
       reduction ? loss.data_ptr<float>() : nullptr, reduction == 1, st);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return {loss, hc, meta, lse};
 }
 
@@ -216,6 +218,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   auto run = w.scalar_type() == at::kHalf ? &f16::lce_backward_16 : &lce_backward_16;
   run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias),
       reinterpret_cast<const float2*>(lse.data_ptr<float>()), x, m16(dh), m16(dw), need_b ? db.data_ptr() : nullptr, st);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return {dh, dw, db};
 }
 
@@ -265,6 +268,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_forward(const at:
     const FfnShape s{(int)N, (int)K, (int)up8(K), (int)F, (int)F8};
     auto run = x.scalar_type() == at::kHalf ? &f16::ffn_forward_16 : &ffn_forward_16;
     run(s, xm.p, xm.ld, wm.w, (int)act, m16(g), m16(u), m16(h), m16(y), x.device(), cur_stream());
+    C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   if (!save) h = at::Tensor();
   return {y, g, u, h};
@@ -301,6 +305,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
   auto run = x.scalar_type() == at::kHalf ? &f16::ffn_backward_16 : &ffn_backward_16;
   run(s, dym.p, dym.ld, xm.p, xm.ld, wm.w, (int)act, p16(g), p16(u), p16(h), m16(dgu), m16(dx), m16(dwg), m16(dwu),
       m16(dwd), x.device(), cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return {dx, dwg, dwu, dwd};
 }
 
@@ -457,6 +462,7 @@ void ns_launch(NsGroup& g, const NsParams& p, const at::TensorOptions& opt) {
   if (p.steps > 1) x1 = at::empty({all}, h);
   at::Tensor part = at::empty({g.count * NS_PART}, opt.dtype(at::kFloat));
   ns_run(g, p, NsScratch{m16(x0), m16(x1), m16(gram), m16(poly), part.data_ptr<float>()}, cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   g.count = 0;
 }
 

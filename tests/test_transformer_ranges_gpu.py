@@ -94,3 +94,50 @@ def test_lce_all_words_alike(n, k, v, low):
     close(gh, want, (err + acc * v * E32) @ w.double().abs() + want.abs() * 2.0 ** -8, "dh")
     want = dz.t() @ h.double()
     close(gw, want, (err + acc * n * E32).t() @ h.double().abs() + want.abs() * 2.0 ** -8, "dw")
+
+
+def test_lce_rows_past_a_launch():
+    """More rows than one launch has waves for (2^26 and some), in a pattern that repeats every 1024: every
+    row's loss and gradient is its pattern's."""
+    from mihvd.ops import linear_cross_entropy
+
+    k, v, n, per = 8, 24, (1 << 26) + 37, 1024
+    h, w, y, _ = lce_case(per, k, v, BF, None, seed=31)
+    grow = torch.rand(per, generator=gen(32), dtype=torch.float64).float().double()
+    loss, ltol, dh, _, _ = lce_ref(h, w, y, None, grow, BF)
+
+    def pattern(t):
+        return t.cuda().repeat(-(-n // per), *([1] * (t.dim() - 1)))[:n]
+
+    hl = pattern(h).requires_grad_()
+    rows = linear_cross_entropy(hl, w.cuda(), pattern(y), reduction="none")
+    gh, = torch.autograd.grad(rows, hl, pattern(grow.float()))
+    close(rows[:per], loss, ltol, "rows")
+    close(gh[:per], *dh, "dh")
+    for t in (rows.detach(), gh):
+        whole = t[:n // per * per].view(-1, *t[:per].shape)
+        assert (whole == whole[:1]).all() and torch.equal(t[n // per * per:], t[:n % per])
+    del hl, rows, gh, t, whole
+    torch.cuda.empty_cache()
+
+
+def test_lce_hidden_gradient_past_a_launch():
+    """A hidden gradient of more than 2^34 elements (one row's vector, expanded): rows of one label are alike to
+    the last, ignored ones zero."""
+    from mihvd.ops import linear_cross_entropy
+
+    k, v, n = 4104, 16, (1 << 22) + 5
+    h, w, _, _ = lce_case(1, k, v, BF, None, seed=33, drop=0.0)
+    y = torch.arange(n) % 5
+    y[y == 4] = -100
+    hl = h.cuda().expand(n, k).detach().requires_grad_()
+    loss = linear_cross_entropy(hl, w.cuda(), y.cuda(), reduction="sum")
+    gh, = torch.autograd.grad(loss, hl)
+    _, _, dh, _, _ = lce_ref(h.expand(5, k), w, y[:5], None, torch.ones(5, dtype=torch.float64), BF)
+    close(gh[:5], *dh, "dh")
+    for at in (n // 5 // 2 * 5, n - n % 5 - 50000):
+        part = gh[at:at + 50000].view(-1, 5, k)
+        assert (part == gh[:5]).all(), at
+    assert torch.equal(gh[-(n % 5):], gh[:n % 5])
+    del hl, loss, gh, part
+    torch.cuda.empty_cache()
