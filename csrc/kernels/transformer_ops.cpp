@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <map>
 #include <tuple>
 #include <unordered_set>
@@ -330,6 +331,13 @@ void once(const at::Tensor& gout, variable_list& grads) {
     if (t.defined()) t = Once::apply(t, any);
 }
 
+// A forward-mode derivative has no formula here, and would be taken for zero wherever a call passes the
+// autograd function by.
+void refuse_tangents(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), op, ": forward-mode derivatives are not implemented");
+}
+
 // Called by a backward pass before anything else runs. While a stream is captured, the engine would make a
 // leaf's gradient accumulator that an eager graph on the default stream still holds wait there for the
 // captured stream, which invalidates the capture inside the engine and ends the process: refused
@@ -391,6 +399,7 @@ at::Tensor linear_cross_entropy(const at::Tensor& h, const at::Tensor& w, const 
 }
 at::Tensor linear_cross_entropy_autograd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
                                          const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
+  refuse_tangents("linear_cross_entropy", {&h, &w, bias ? &*bias : &w});
   return LceFunction::apply(h, w, labels, bias, ignore_index, reduction);
 }
 
@@ -425,6 +434,7 @@ at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
 }
 at::Tensor gated_ffn_autograd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
                               int64_t act) {
+  refuse_tangents("gated_ffn", {&x, &wg, &wu, &wd});
   if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad()))
     return FfnFunction::apply(x, wg, wu, wd, act);
   at::AutoDispatchBelowADInplaceOrView below;

@@ -8,7 +8,8 @@ autograd formulas are registered beside them in csrc/kernels/transformer_ops.cpp
 
 Both run on bf16 or fp16 MFMA operands with fp32 accumulation. Under ``torch.autocast`` floating
 inputs are cast to the autocast type first, as ``torch.nn.functional.linear`` does; otherwise the
-inputs must be 16-bit themselves. There is no CPU or fp32 form: other inputs raise.
+inputs must be 16-bit themselves. There is no CPU or fp32 form: other inputs raise. Gradients are
+reverse-mode and of first order: forward-mode derivatives and gradients of gradients raise.
 """
 from __future__ import annotations
 

@@ -276,7 +276,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
         X = x / (|x|_F + eps);   A = X X^T;   X <- a X + (b A + c A A) X        (a, b, c = coefficients)
 
     (on the smaller side; the default coefficients leave the singular values near 1 within about 0.3).
-    The result has ``x``'s type and shape. ``precision``: ``"fp16"`` — one fp16 product with fp32
+    The result has ``x``'s type and shape, and takes no part in autograd (``x`` is detached). ``precision``: ``"fp16"`` — one fp16 product with fp32
     accumulation per step, the default for 16-bit inputs — or ``"fp32"`` — three products over split
     values (22 bits), the default for fp32. On the GPU it runs csrc/kernels/newton_schulz.hip; CPU
     tensors take the formula in fp32 torch operations.

@@ -141,3 +141,29 @@ def test_lce_hidden_gradient_past_a_launch():
     assert torch.equal(gh[-(n % 5):], gh[:n % 5])
     del hl, loss, gh, part
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", [True, False], ids=["grad", "no_grad"])
+def test_forward_mode_is_refused(which, grad):
+    """A tangent on any input raises, with reverse mode on or off: it is never dropped for a zero derivative."""
+    import torch.autograd.forward_ad as fwd
+
+    from mihvd.ops import gated_ffn, linear_cross_entropy
+    from test_transformer_gpu import ffn_case
+
+    block = [t.cuda() for t in ffn_case(5, 16, 24, BF, 1)[:4]]
+    h, w, y, b = (t.cuda() for t in lce_case(6, 16, 30, BF, torch.float32, 2))
+    head = [h, w, b]
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        args = [fwd.make_dual(t, torch.ones_like(t)) if i == which else t for i, t in enumerate(block)]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            gated_ffn(*args)
+        if which < 3:
+            args = [fwd.make_dual(t, torch.ones_like(t)) if i == which else t for i, t in enumerate(head)]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                linear_cross_entropy(args[0], args[1], y, args[2])
+    if which < 1:
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda t: gated_ffn(t, *block[1:]), (block[0],), (block[0],))
+    assert torch.isfinite(gated_ffn(*block)).all()
