@@ -65,7 +65,7 @@ Mat mat(const at::Tensor& t, bool force = false) {
 void check16(const at::Tensor& t, const char* op, const char* name, const at::Tensor& like, int64_t dim) {
   TORCH_CHECK_VALUE(t.dim() == dim, op, ": ", name, " must have ", dim, " dimensions (got ", t.dim(), ")");
   TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": ", name,
-                   " must be bfloat16 or float16 outside autocast (got ", t.scalar_type(), ")");
+                   " must be bfloat16 or float16 (float32 under autocast; got ", t.scalar_type(), ")");
   TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), op, ": ", name, " must have the type of the first argument");
   TORCH_CHECK_VALUE(t.device() == like.device() && t.is_cuda(), op, ": ", name, " must be on the same GPU");
 }

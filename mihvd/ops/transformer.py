@@ -6,9 +6,9 @@ autograd formulas are registered beside them in csrc/kernels/transformer_ops.cpp
 * ``gated_ffn(x, w_gate, w_up, w_down)`` — ``(act(x Wg^T) * (x Wu^T)) Wd^T`` with its backward pass
   (csrc/kernels/gated_ffn.hip).
 
-Both run on bf16 or fp16 MFMA operands with fp32 accumulation. Under ``torch.autocast`` floating
-inputs are cast to the autocast type first, as ``torch.nn.functional.linear`` does; otherwise the
-inputs must be 16-bit themselves. There is no CPU or fp32 form: other inputs raise. Gradients are
+Both run on bf16 or fp16 MFMA operands with fp32 accumulation. Under ``torch.autocast`` fp32, bf16 and
+fp16 inputs are cast to the autocast type first, as for ``torch.nn.functional.linear``; otherwise the
+inputs must be 16-bit themselves. There is no CPU, fp32 or fp64 form: other inputs raise. Gradients are
 reverse-mode and of first order: forward-mode derivatives and gradients of gradients raise.
 """
 from __future__ import annotations
@@ -40,9 +40,9 @@ def _on_gpu(op, *tensors):
 
 
 def _autocast(*tensors):
-    """Autocast's cast of the floating matrices of a call."""
+    """Autocast's cast of the floating matrices of a call. Like autocast it leaves float64 alone."""
     dt = torch.get_autocast_dtype("cuda")
-    return [t if t is None or t.dtype == dt or not t.is_floating_point() else t.to(dt) for t in tensors]
+    return [t if t is None or t.dtype in (dt, torch.float64) or not t.is_floating_point() else t.to(dt) for t in tensors]
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,

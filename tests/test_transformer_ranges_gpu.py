@@ -167,3 +167,21 @@ def test_forward_mode_is_refused(which, grad):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(lambda t: gated_ffn(t, *block[1:]), (block[0],), (block[0],))
     assert torch.isfinite(gated_ffn(*block)).all()
+
+
+def test_float64_is_not_cast_by_autocast():
+    """Autocast leaves doubles alone, and so do the operators: they refuse them as they do without it."""
+    from mihvd.ops import gated_ffn, linear_cross_entropy
+    from test_transformer_gpu import ffn_case
+
+    block = [t.cuda() for t in ffn_case(5, 16, 24, BF, 1)[:4]]
+    h, w, y, b = (t.cuda() for t in lce_case(6, 16, 30, BF, torch.float32, 2))
+    with torch.autocast("cuda", BF):
+        for i in range(4):
+            with pytest.raises(TypeError, match="bfloat16 or float16|type of the first"):
+                gated_ffn(*[t.double() if i == j else t.float() for j, t in enumerate(block)])
+        for i in range(2):
+            with pytest.raises(TypeError, match="bfloat16 or float16|type of the first"):
+                linear_cross_entropy(*[t.double() if i == j else t.float() for j, t in enumerate((h, w))], y)
+        with pytest.raises(TypeError, match="bias"):
+            linear_cross_entropy(h, w, y, b.double())
