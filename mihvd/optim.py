@@ -324,8 +324,9 @@ class Muon(torch.optim.Optimizer):
     fp32 contiguous GPU parameters take one fused path (``torch.ops.mihvd.muon_step``: matrices of like
     smaller sides run together, momentum, products and weight update in the kernels, no host
     synchronisation, capturable from the second step on, with the learning rate it then has); others use
-    torch operations around :func:`orthogonalize`.
-    ``precision`` is that of the products (see there).
+    torch operations around :func:`orthogonalize`. The momentum is fp32 for parameters of any type (a sum over
+    many steps loses in 16 bits what is small beside it), and so is the update; a 16-bit parameter is
+    rounded once a step. ``precision`` is that of the products (see there).
     """
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5,
@@ -354,6 +355,15 @@ class Muon(torch.optim.Optimizer):
                 self.param_groups.pop()
                 raise TypeError("Muon: parameters must be float32, bfloat16 or float16 (got %s)" % p.dtype)
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # torch has cast the state to its parameters' types: the momenta of 16-bit ones come back in fp32
+        loaded = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(loaded, [p for group in self.param_groups for p in group["params"]]):
+            m = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if m is not None and p.dtype != torch.float32:
+                self.state[p]["momentum_buffer"] = m.to(device=p.device, dtype=torch.float32)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -369,7 +379,7 @@ class Muon(torch.optim.Optimizer):
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("Muon: the first step of a parameter makes its momentum, which every replay "
                                            "would clear; run one step before capturing")
-                    st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
                 m = st["momentum_buffer"]
                 if p.grad.is_sparse:
                     raise RuntimeError("Muon: sparse gradients are not supported")
@@ -390,7 +400,7 @@ class Muon(torch.optim.Optimizer):
 
     @staticmethod
     def _plain(group, p, m):
-        g, mu, lr = p.grad, group["momentum"], group["lr"]
+        g, mu, lr = p.grad.float(), group["momentum"], group["lr"]
         m.mul_(mu).add_(g)
         u = g.add(m, alpha=mu) if group["nesterov"] else m
         rows, cols = p.shape[0], p.numel() // max(1, p.shape[0])
@@ -399,4 +409,7 @@ class Muon(torch.optim.Optimizer):
         s = math.sqrt(max(1.0, rows / cols)) if group["scale"] == "spectral" else 0.2 * math.sqrt(max(rows, cols))
         o = orthogonalize(u.reshape(rows, cols), group["ns_steps"], group["ns_coefficients"], group["eps"],
                           group["precision"])
-        p.mul_(1.0 - lr * group["weight_decay"]).add_(o.view(p.shape), alpha=-lr * s)
+        w = p.float()  # p itself where it is fp32
+        w.mul_(1.0 - lr * group["weight_decay"]).add_(o.view(p.shape), alpha=-lr * s)
+        if w is not p:
+            p.copy_(w)

@@ -1,0 +1,71 @@
+"""The optimizer side of the transformer-step operators at the ends of their ranges, without a GPU."""
+import copy
+import math
+
+import pytest
+import torch
+
+from test_transformer_cpu import ns64
+
+
+def muon_drift(dt, device, steps=40):
+    """A 16-bit parameter through many steps of one small gradient with noise, beside the 64-bit recurrence over
+    the same gradients: the largest error of the momentum, relative to its own size, and of the weight in
+    half steps of its type per step."""
+    from mihvd.optim import Muon
+
+    g = torch.Generator().manual_seed(5)
+    start = (torch.randn(24, 16, generator=g) * 0.5).to(dt)
+    drift = torch.randn(24, 16, generator=g) * 2e-3
+    w = torch.nn.Parameter(start.to(device))
+    opt = Muon([w], lr=0.02, momentum=0.99, weight_decay=0.01)
+    ref, mom = start.double(), torch.zeros(24, 16, dtype=torch.float64)
+    for k in range(steps):
+        d = ((torch.randn(24, 16, generator=g) * (0.3 if k == 0 else 1e-3)) + drift).to(dt)
+        w.grad = d.to(device)
+        opt.step()
+        mom = 0.99 * mom + d.double()
+        u = d.double() + 0.99 * mom
+        ref = ref * (1 - 0.02 * 0.01) - 0.02 * math.sqrt(24 / 16) * ns64(u.t()).t()
+    got = opt.state[w]["momentum_buffer"]
+    assert got.dtype == torch.float32
+    assert float((got.cpu().double() - mom).abs().max()) <= 2 * steps * 2.0 ** -24 * float(mom.abs().max())
+    # each step rounds the weight once; the updates' own errors (ns_tol: 64 * 2^-22 of their norm) are far below
+    half = torch.finfo(dt).eps / 2
+    tol = steps * (half * (float(ref.abs().max()) + 0.5) + 0.02 * 1.3 * 6 * 64 * 2.0 ** -22)
+    assert float((w.detach().cpu().double() - ref).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_muon_momentum_of_16_bit_parameters(dt):
+    muon_drift(dt, "cpu")
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
+def test_muon_checkpoint_keeps_the_momentum(dt):
+    """A momentum goes through state_dict and load_state_dict bit for bit, and the step behind it is the same."""
+    from mihvd.optim import Muon
+
+    g = torch.Generator().manual_seed(6)
+    a = [torch.nn.Parameter(torch.randn(6, 4, generator=g).to(dt)) for _ in range(3)]
+    opt = Muon([dict(params=a[:1]), dict(params=a[1:], lr=0.05)], lr=0.02)
+    for k in range(3):
+        for i, p in enumerate(a):
+            p.grad = None if i == 1 and k == 0 else (torch.randn(6, 4, generator=g) * 0.1).to(dt)
+        opt.step()
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    opt2 = Muon([dict(params=b[:1]), dict(params=b[1:])], lr=0.02)
+    opt2.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for p, q in zip(a, b):
+        m, n = opt.state[p]["momentum_buffer"], opt2.state[q]["momentum_buffer"]
+        assert m.dtype == n.dtype == torch.float32 and torch.equal(m, n)
+        q.grad = p.grad.clone()
+    opt.step()
+    opt2.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    # a checkpoint that holds the momentum in the parameter's type loads into fp32
+    old = copy.deepcopy(opt.state_dict())
+    for st in old["state"].values():
+        st["momentum_buffer"] = st["momentum_buffer"].to(dt)
+    opt2.load_state_dict(old)
+    assert all(opt2.state[q]["momentum_buffer"].dtype == torch.float32 for q in b)

@@ -185,3 +185,10 @@ def test_float64_is_not_cast_by_autocast():
                 linear_cross_entropy(*[t.double() if i == j else t.float() for j, t in enumerate((h, w))], y)
         with pytest.raises(TypeError, match="bias"):
             linear_cross_entropy(h, w, y, b.double())
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=["bf16", "fp16"])
+def test_muon_momentum_of_16_bit_parameters(dt):
+    from test_transformer_ranges_cpu import muon_drift
+
+    muon_drift(dt, "cuda")
