@@ -15,6 +15,7 @@ identical rule on the flat parameter buffer.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -259,13 +260,49 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 def _ns_coefficients(op, coefficients):
-    """The three as floats. A step's matrix a I + b A + c A A is held in fp16 scaled by 2^12, which ends at 16."""
+    """The three as floats."""
     if len(coefficients) != 3:
         raise ValueError("%s: three coefficients are needed" % op)
     abc = tuple(float(v) for v in coefficients)
     if not sum(map(abs, abc)) <= 15:
         raise ValueError("%s: the coefficients' magnitudes must not add up to more than 15 (got %s)" % (op, abc))
     return abc
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_reach(steps, a, b, c):
+    """The largest value that any of the matrices X, A = X X^T and a I + b A + c A A can hold before the last
+    step is done: their elements lie below their largest eigenvalues, and X's singular values start within one.
+    A step takes a singular value s to s q(s^2), q(t) = a + b t + c t^2; each maximum over [0, top] is at an
+    end or where the derivative vanishes."""
+
+    def most(f, top, roots):
+        return max(abs(f(t)) for t in (0.0, top, *[t for t in roots if 0.0 < t < top]))
+
+    def q(t):
+        return a + t * (b + t * c)
+
+    disc = 9 * b * b - 20 * a * c  # (s q(s^2))' = a + 3 b t + 5 c t^2
+    if c:
+        turns = [(-3 * b + sign * math.sqrt(disc)) / (10 * c) for sign in (1, -1)] if disc >= 0 else []
+        vertex = [-b / (2 * c)]
+    else:
+        turns, vertex = [-a / (3 * b)] if b else [], []
+    top, reach = 1.0, 1.0
+    for k in range(steps):
+        reach = max(reach, top, top * top, most(q, top * top, vertex))
+        if reach > 1e9:
+            break
+        top = most(lambda t: math.sqrt(t) * q(t), top * top, turns)
+    return reach
+
+
+def _ns_check_range(op, steps, coefficients):
+    """The kernels hold those matrices in fp16 scaled by 2^12, which ends at 16."""
+    reach = _ns_reach(steps, *coefficients)
+    if not reach <= 15:
+        raise ValueError("%s: %d steps with the coefficients %s can reach values of %.3g; the GPU's fp16 planes hold them "
+                         "up to 15" % (op, steps, tuple(coefficients), reach))
 
 
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
@@ -278,8 +315,9 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     (on the smaller side; the default coefficients leave the singular values near 1 within about 0.3).
     The result has ``x``'s type and shape, and takes no part in autograd (``x`` is detached). ``precision``: ``"fp16"`` — one fp16 product with fp32
     accumulation per step, the default for 16-bit inputs — or ``"fp32"`` — three products over split
-    values (22 bits), the default for fp32. On the GPU it runs csrc/kernels/newton_schulz.hip; CPU
-    tensors take the formula in fp32 torch operations.
+    values (22 bits), the default for fp32. On the GPU it runs csrc/kernels/newton_schulz.hip, and
+    coefficients whose steps can take singular values past 15 are refused (fp16 planes hold X, A and the
+    polynomial); CPU tensors take the formula in fp32 torch operations.
     """
     if x.dim() < 2:
         raise ValueError("orthogonalize: a matrix or a batch of matrices is needed (got shape %s)" % (tuple(x.shape),))
@@ -295,6 +333,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     if x.is_cuda:
         from . import _native
 
+        _ns_check_range("orthogonalize", int(steps), (a, b, c))
         _native.require_kernels()
         split = precision == "fp32" or (precision is None and x.dtype == torch.float32)
         out = torch.ops.mihvd.newton_schulz(x.detach().reshape(-1, *x.shape[-2:]), int(steps), a, b, c, float(eps), split)
@@ -372,6 +411,8 @@ class Muon(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
+            if any(p.is_cuda for p in params):
+                _ns_check_range("Muon", group["ns_steps"], group["ns_coefficients"])
             fused = ([], [], [])
             for p in params:
                 st = self.state[p]

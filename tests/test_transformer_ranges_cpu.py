@@ -69,3 +69,25 @@ def test_muon_checkpoint_keeps_the_momentum(dt):
         st["momentum_buffer"] = st["momentum_buffer"].to(dt)
     opt2.load_state_dict(old)
     assert all(opt2.state[q]["momentum_buffer"].dtype == torch.float32 for q in b)
+
+
+@pytest.mark.parametrize("steps,coef", [(1, (3.4445, -4.7750, 2.0315)), (5, (3.4445, -4.7750, 2.0315)),
+                                        (100, (3.4445, -4.7750, 2.0315)), (100, (1.5, -0.5, 0.0)), (7, (2.0, -1.5, 0.5)),
+                                        (3, (4.0, -2.0, 1.0)), (2, (-3.0, 0.0, 0.0)), (4, (3.0, 0.0, 0.0)), (3, (0.0, 4.0, -1.0)),
+                                        (3, (1.0, 2.0, -2.5)), (0, (9.0, 0.0, 0.0)), (3, (0.0, 0.0, 0.0))])
+def test_newton_schulz_reach(steps, coef):
+    """The bound on X, X X^T and the polynomial is what a fine grid of singular values attains."""
+    from mihvd.optim import _ns_reach
+
+    a, b, c = coef
+    lo, hi, want = 0.0, 1.0, 1.0
+    for _ in range(steps):
+        s = torch.linspace(lo, hi, 400001, dtype=torch.float64)
+        t = s * s
+        q = a + b * t + c * t * t
+        want = max(want, hi, hi * hi, float(q.abs().max()))
+        hi = float((s * q).abs().max())
+        if want > 1e9:
+            break
+    got = _ns_reach(steps, a, b, c)
+    assert want <= got * (1 + 1e-12) and (got <= want * (1 + 1e-6) or want > 1e9), (got, want)

@@ -192,3 +192,28 @@ def test_muon_momentum_of_16_bit_parameters(dt):
     from test_transformer_ranges_cpu import muon_drift
 
     muon_drift(dt, "cuda")
+
+
+def test_newton_schulz_coefficients_out_of_range():
+    """Coefficients whose steps can pass what fp16 planes hold are refused before anything is written; those
+    that stay within are computed, close to the bound too (a matrix of rank one starts at singular value one)."""
+    from mihvd.optim import Muon, orthogonalize
+    from test_transformer_gpu import ns64, ns_tol
+
+    x = (torch.randn(20, 1, generator=gen(41)) @ torch.randn(1, 30, generator=gen(42))).cuda()
+    for steps, coef in ((3, (4.0, -2.0, 1.0)), (3, (3.0, 0.0, 0.0)), (5, (2.0, 0.5, 0.0)), (2, (1.5, 1.0, 1.0))):
+        with pytest.raises(ValueError, match="coefficients"):
+            orthogonalize(x, steps=steps, coefficients=coef)
+        p = torch.nn.Parameter(x.clone())
+        p.grad = x.clone()
+        opt = Muon([p], ns_steps=steps, ns_coefficients=coef)
+        with pytest.raises(ValueError, match="coefficients"):
+            opt.step()
+        assert torch.equal(p, x)
+    for steps, coef in ((2, (3.5, 0.0, 0.0)), (1, (10.0, -1.0, 4.0)), (5, (1.5, -0.5, 0.0)), (2, (1.2, 0.5, 0.2))):
+        for dt in (torch.float32, FP):
+            got = orthogonalize(x.to(dt), steps=steps, coefficients=coef).double().cpu()
+            want = ns64(x.to(dt).cpu(), steps, coef)
+            # |f'(s)| s <= 5 |f(s)| at the one singular value; what rounding puts beside it grows by at most 12
+            tol = ns_tol(want, dt, dt == torch.float32)
+            assert torch.linalg.vector_norm(got - want) <= tol, (steps, coef)
