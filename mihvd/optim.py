@@ -370,31 +370,42 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5,
                  ns_coefficients=NS_COEFFICIENTS, eps=1e-7, scale="spectral", precision="fp32"):
-        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
+        super().__init__(params, self._checked(dict(
+            lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
+            ns_coefficients=ns_coefficients, eps=eps, scale=scale, precision=precision)))
+
+    @staticmethod
+    def _checked(group):
+        """A group's options (the constructor's or its own), checked."""
+        if group["lr"] < 0 or group["weight_decay"] < 0 or not 0 <= group["momentum"] < 1:
             raise ValueError("Muon: lr and weight_decay must not be negative, momentum must be within [0, 1)")
-        if not 0 <= int(ns_steps) <= 100:
+        if not 0 <= int(group["ns_steps"]) <= 100:
             raise ValueError("Muon: ns_steps must be within 0..100")
-        if scale not in ("spectral", "rms"):
+        if group["scale"] not in ("spectral", "rms"):
             raise ValueError("Muon: scale must be 'spectral' or 'rms'")
-        if precision not in ("fp32", "fp16"):
+        if group["precision"] not in ("fp32", "fp16"):
             raise ValueError("Muon: precision must be 'fp32' or 'fp16'")
-        ns_coefficients = _ns_coefficients("Muon", ns_coefficients)
-        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
-                                      ns_steps=int(ns_steps), ns_coefficients=ns_coefficients, eps=eps,
-                                      scale=scale, precision=precision))
+        group["ns_steps"] = int(group["ns_steps"])
+        group["ns_coefficients"] = _ns_coefficients("Muon", group["ns_coefficients"])
+        return group
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                self.param_groups.pop()
-                raise ValueError("Muon: parameters must have at least two dimensions (got shape %s); give vectors to "
-                                 "another optimizer" % (tuple(p.shape),))
-            if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-                self.param_groups.pop()
-                raise TypeError("Muon: parameters must be float32, bfloat16 or float16 (got %s)" % p.dtype)
+        try:
+            self._checked(self.param_groups[-1])
+            for p in self.param_groups[-1]["params"]:
+                if p.dim() < 2:
+                    raise ValueError("Muon: parameters must have at least two dimensions (got shape %s); give vectors to "
+                                     "another optimizer" % (tuple(p.shape),))
+                if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                    raise TypeError("Muon: parameters must be float32, bfloat16 or float16 (got %s)" % p.dtype)
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
+        for group in state_dict["param_groups"]:
+            self._checked(dict(self.defaults, **group))
         super().load_state_dict(state_dict)
         # torch has cast the state to its parameters' types: the momenta of 16-bit ones come back in fp32
         loaded = [i for group in state_dict["param_groups"] for i in group["params"]]
@@ -405,14 +416,16 @@ class Muon(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        for group in self.param_groups:  # before anything is written
+            self._checked(group)
+            if any(p.is_cuda for p in group["params"]):
+                _ns_check_range("Muon", group["ns_steps"], group["ns_coefficients"])
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
-            if any(p.is_cuda for p in params):
-                _ns_check_range("Muon", group["ns_steps"], group["ns_coefficients"])
             fused = ([], [], [])
             for p in params:
                 st = self.state[p]

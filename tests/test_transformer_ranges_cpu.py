@@ -91,3 +91,35 @@ def test_newton_schulz_reach(steps, coef):
             break
     got = _ns_reach(steps, a, b, c)
     assert want <= got * (1 + 1e-12) and (got <= want * (1 + 1e-6) or want > 1e9), (got, want)
+
+
+def test_muon_group_options():
+    """A group's own options are checked as the constructor's are, when it is added, loaded, or has been edited."""
+    from mihvd.optim import Muon
+
+    def par():
+        return torch.nn.Parameter(torch.ones(4, 3))
+
+    bad = (dict(lr=-1.0), dict(momentum=1.5), dict(weight_decay=-1.0), dict(ns_steps=101), dict(ns_steps=-1), dict(scale="adam"),
+           dict(precision="bf16"), dict(ns_coefficients=(1.0, 2.0)), dict(ns_coefficients=(16.0, 0.0, 0.0)))
+    opt = Muon([par()])
+    for kw in bad:
+        with pytest.raises(ValueError, match="Muon"):
+            Muon([dict(params=[par()], **kw)])
+        with pytest.raises(ValueError, match="Muon"):
+            opt.add_param_group(dict(params=[par()], **kw))
+        assert len(opt.param_groups) == 1
+        state = copy.deepcopy(opt.state_dict())
+        state["param_groups"][0].update(kw)
+        with pytest.raises(ValueError, match="Muon"):
+            opt.load_state_dict(state)
+        assert opt.param_groups[0]["scale"] == "spectral" and opt.param_groups[0]["ns_steps"] == 5
+        other = Muon([par(), par()])
+        other.param_groups[0].update(kw)
+        p = other.param_groups[0]["params"][0]
+        p.grad = torch.ones(4, 3)
+        with pytest.raises(ValueError, match="Muon"):
+            other.step()
+        assert (p == 1).all() and not other.state
+    opt.add_param_group(dict(params=[par()], ns_steps=3, scale="rms", precision="fp16", ns_coefficients=[1.5, -0.5, 0]))
+    assert opt.param_groups[1]["ns_coefficients"] == (1.5, -0.5, 0.0)
