@@ -6,6 +6,7 @@
 #include <c10/hip/HIPException.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <initializer_list>
@@ -558,6 +559,18 @@ void muon_step(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vect
   }
 }
 
+// The weights and momenta count as changed in place: a backward pass that saved a weight before the step raises.
+void muon_step_in_place(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vector<at::Tensor> ms, double lr,
+                        double momentum, bool nesterov, double weight_decay, int64_t steps, double a, double b, double c,
+                        double eps, int64_t scale_mode, bool split) {
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    muon_step(ps, std::move(gs), ms, lr, momentum, nesterov, weight_decay, steps, a, b, c, eps, scale_mode, split);
+  }
+  for (const auto* list : {&ps, &ms})
+    for (const at::Tensor& t : *list) torch::autograd::impl::bump_version(t);
+}
+
 }  // namespace
 }  // namespace mihvd
 
@@ -576,6 +589,8 @@ TORCH_LIBRARY_IMPL(mihvd, CUDA, m) {
   m.impl("newton_schulz", &mihvd::newton_schulz);
   m.impl("muon_step", &mihvd::muon_step);
 }
+
+TORCH_LIBRARY_IMPL(mihvd, ADInplaceOrView, m) { m.impl("muon_step", &mihvd::muon_step_in_place); }
 
 TORCH_LIBRARY_IMPL(mihvd, AutogradCUDA, m) {
   m.impl("linear_cross_entropy", &mihvd::linear_cross_entropy_autograd);

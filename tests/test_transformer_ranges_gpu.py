@@ -217,3 +217,29 @@ def test_newton_schulz_coefficients_out_of_range():
             # |f'(s)| s <= 5 |f(s)| at the one singular value; what rounding puts beside it grows by at most 12
             tol = ns_tol(want, dt, dt == torch.float32)
             assert torch.linalg.vector_norm(got - want) <= tol, (steps, coef)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, BF], ids=["fp32", "bf16"])
+def test_muon_step_counts_as_a_change(dt):
+    """A graph that saved a weight before the step cannot be run backward with the weight after it, on the fused
+    path and the other."""
+    from mihvd.optim import Muon
+
+    w = torch.nn.Parameter(torch.randn(16, 24, generator=gen(51)).cuda().to(dt))
+    x = torch.randn(5, 24, generator=gen(52)).cuda().to(dt).requires_grad_()
+    w.grad = torch.ones_like(w)
+    opt = Muon([w], lr=0.1)
+    y = (x @ w.t()).sum()
+    before = w._version
+    opt.step()
+    m = opt.state[w]["momentum_buffer"]
+    assert w._version > before and m._version > 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    (x @ w.t()).sum().backward()
+    wd = w.detach().double()
+    # a sum of 16 weights, in fp32 (and rounded to bf16)
+    tol = (16 * E32 + (half(dt) if dt == BF else 0)) * wd.abs().sum(0)
+    close(x.grad, wd.sum(0).expand(5, 24).cpu(), tol.expand(5, 24).cpu(), "x.grad")
+    with torch.inference_mode():
+        opt.step()
