@@ -53,15 +53,22 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
   }
 }
 
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
 // Sum of squares of each matrix, NS_PART partial sums; for Muon the momentum is updated on the way:
-// m = mu m + g, u = g + mu m (nesterov) or m. Bound by memory: one read of each input, one write of m.
+// m = mu m + g, u = g + mu m (nesterov) or m. Bound by memory: one read of each input, one write of m. In 64
+// bits: the squares of fp32 values above 2^64 or below 2^-75 leave fp32's range.
 template <int KIND>
-__global__ void __launch_bounds__(256) ns_norm(const NsGroup t, int muon, float mu, int nesterov, float* __restrict__ partial) {
-  __shared__ float sh[4];
+__global__ void __launch_bounds__(256) ns_norm(const NsGroup t, int muon, float mu, int nesterov, double* __restrict__ partial) {
+  __shared__ double sh[4];
   const NsMat& q = t.m[blockIdx.y];
   const int64_t n = (int64_t)q.rows * q.cols, stride = (int64_t)gridDim.x * 1024;
   const bool vec = n % 4 == 0 && ((uintptr_t)q.src & (KIND ? 7 : 15)) == 0 && (!muon || ((uintptr_t)q.mom & 15) == 0);
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
   if (vec) {
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += stride) {
       f32x4 v = load4<KIND>(q.src, i);
@@ -75,7 +82,7 @@ __global__ void __launch_bounds__(256) ns_norm(const NsGroup t, int muon, float 
         *reinterpret_cast<f32x4*>(q.mom + i) = m;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] = fmaf(v[k], v[k], s[k]);
+      for (int k = 0; k < 4; ++k) s[k] = fma((double)v[k], (double)v[k], s[k]);
     }
   } else {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride / 4) {
@@ -85,10 +92,10 @@ __global__ void __launch_bounds__(256) ns_norm(const NsGroup t, int muon, float 
         q.mom[i] = m;
         v = nesterov ? fmaf(mu, m, v) : m;
       }
-      s[0] = fmaf(v, v, s[0]);
+      s[0] = fma((double)v, (double)v, s[0]);
     }
   }
-  const float w = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  const double w = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = w;
   __syncthreads();
   if (threadIdx.x == 0) partial[blockIdx.y * NS_PART + blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
@@ -98,11 +105,11 @@ __global__ void __launch_bounds__(256) ns_norm(const NsGroup t, int muon, float 
 // where the matrix is tall; zeros in the padding.
 template <int KIND>
 __global__ void __launch_bounds__(256) ns_scale(const NsGroup t, int muon, float mu, int nesterov, float eps,
-                                                const float* __restrict__ partial, u16* __restrict__ x) {
+                                                const double* __restrict__ partial, u16* __restrict__ x) {
   __shared__ float sh[64][65];
   const NsMat& q = t.m[blockIdx.y];
   const int tl = q.len / 64, tiles = t.side / 64 * tl;
-  const float inv = S / (sqrtf(wave_sum(partial[blockIdx.y * NS_PART + (threadIdx.x & 63)])) + eps);
+  const double inv = S / (sqrt(wave_sum64(partial[blockIdx.y * NS_PART + (threadIdx.x & 63)])) + eps);
   const bool tall = q.rows > q.cols;
   const int64_t plane = (int64_t)t.side * q.len;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(256) ns_scale(const NsGroup t, int muon, float
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sh[r][c + k] = v[k] * inv;
+      for (int k = 0; k < 4; ++k) sh[r][c + k] = (float)(v[k] * inv);
     }
     __syncthreads();
 #pragma unroll

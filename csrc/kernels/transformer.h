@@ -106,7 +106,7 @@ struct NsParams {
 struct NsScratch {
   u16 *x0, *x1;       // X before and after a step
   u16 *gram, *poly;   // [count][planes][side][side]
-  float* partial;              // [count][NS_PART]
+  double* partial;    // [count][NS_PART]
 };
 constexpr int NS_PART = 64;
 void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& s, hipStream_t st);

@@ -471,8 +471,8 @@ void ns_launch(NsGroup& g, const NsParams& p, const at::TensorOptions& opt) {
     poly = at::empty({sq}, h);
   }
   if (p.steps > 1) x1 = at::empty({all}, h);
-  at::Tensor part = at::empty({g.count * NS_PART}, opt.dtype(at::kFloat));
-  ns_run(g, p, NsScratch{m16(x0), m16(x1), m16(gram), m16(poly), part.data_ptr<float>()}, cur_stream());
+  at::Tensor part = at::empty({g.count * NS_PART}, opt.dtype(at::kDouble));
+  ns_run(g, p, NsScratch{m16(x0), m16(x1), m16(gram), m16(poly), part.data_ptr<double>()}, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
   g.count = 0;
 }

@@ -338,8 +338,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
         split = precision == "fp32" or (precision is None and x.dtype == torch.float32)
         out = torch.ops.mihvd.newton_schulz(x.detach().reshape(-1, *x.shape[-2:]), int(steps), a, b, c, float(eps), split)
         return out.view(x.shape)
-    z = x.detach().float()
-    z = z / (torch.linalg.vector_norm(z, dim=(-2, -1), keepdim=True) + eps)
+    z = x.detach().double()  # the norm's squares may leave fp32's range
+    z = (z / (torch.linalg.vector_norm(z, dim=(-2, -1), keepdim=True) + eps)).float()
     tall = z.shape[-2] > z.shape[-1]
     if tall:
         z = z.transpose(-2, -1)

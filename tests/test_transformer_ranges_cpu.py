@@ -123,3 +123,14 @@ def test_muon_group_options():
         assert (p == 1).all() and not other.state
     opt.add_param_group(dict(params=[par()], ns_steps=3, scale="rms", precision="fp16", ns_coefficients=[1.5, -0.5, 0]))
     assert opt.param_groups[1]["ns_coefficients"] == (1.5, -0.5, 0.0)
+
+
+@pytest.mark.parametrize("by,eps", [(2.0 ** 100, 1e-7), (2.0 ** 120, 1e-7), (2.0 ** -90, 0.0)])
+def test_orthogonalize_far_norms_cpu(by, eps):
+    """Values whose squares leave fp32's range have the result of their moderate multiple."""
+    from mihvd.optim import orthogonalize
+
+    x = torch.randn(12, 7, generator=torch.Generator().manual_seed(8))
+    want = ns64(x, eps=0.0)
+    got = orthogonalize(x * by, eps=eps)
+    assert float((got.double() - want).norm()) <= 64 * 5 * 2.0 ** -24 * float(want.norm())

@@ -243,3 +243,24 @@ def test_muon_step_counts_as_a_change(dt):
     close(x.grad, wd.sum(0).expand(5, 24).cpu(), tol.expand(5, 24).cpu(), "x.grad")
     with torch.inference_mode():
         opt.step()
+
+
+@pytest.mark.parametrize("by,eps", [(2.0 ** 100, 1e-7), (2.0 ** 120, 1e-7), (2.0 ** -90, 0.0)])
+@pytest.mark.parametrize("dt", [torch.float32, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("m,n", [(70, 33), (20, 300)])
+def test_orthogonalize_far_norms(m, n, dt, by, eps):
+    """Values whose squares leave fp32's range have the result of their moderate multiple; a Muon step takes
+    such gradients."""
+    from mihvd.optim import Muon, orthogonalize
+    from test_transformer_gpu import ns64, ns_tol
+
+    x = torch.randn(2, m, n, generator=gen(61)).to(dt)
+    got = orthogonalize((x * by).cuda(), eps=eps).double().cpu()
+    for i in range(2):
+        want = ns64(x[i], eps=0.0)
+        assert torch.linalg.vector_norm(got[i] - want) <= ns_tol(want, dt, dt == torch.float32), i
+    w = torch.nn.Parameter(torch.zeros(m, n, device="cuda", dtype=dt))
+    w.grad = (x[0] * by).cuda()
+    Muon([w], lr=1.0, momentum=0.5, eps=eps).step()
+    want = ns64(x[0], eps=0.0) * math.sqrt(max(1.0, m / n))
+    assert torch.linalg.vector_norm(w.detach().double().cpu() + want) <= 1.01 * ns_tol(want, dt, True)
