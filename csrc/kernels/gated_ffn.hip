@@ -201,6 +201,7 @@ struct EpiGateGrad {
 // by splits with a third launch, 20 us), of 2048 through 5632 22 us (3.1 TB/s). The rows are read again
 // by every block: at 32 rows 13 and 40 us (core: 22 and 48), at 64 rows 18 and 58, so up to 32 come here.
 // MB: groups of 16 rows.
+constexpr int FEW = 32;
 template <int MB, bool DUAL, class Out>
 __device__ __forceinline__ void few_rows(const u16* __restrict__ x, int64_t ldx, int N, const u16* __restrict__ w0,
                                          const u16* __restrict__ w1, int64_t ldw, int F, int K, const Out& out) {
@@ -307,6 +308,8 @@ g16::Side side(const u16* p, int64_t ld, int ext) {
   return s;
 }
 
+int gate_tile(const FfnShape& s) { return g16::plan(s.N, 2 * (int64_t)s.F, s.K, 1, 1, false, false, 1.5, g16::T_DUAL).tile; }
+
 template <int ACT>
 void up_gate(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, u16* g, u16* u, u16* h, hipStream_t st) {
   g16::Args a;
@@ -316,7 +319,7 @@ void up_gate(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, 
   a.M = s.N;
   a.N = s.F;
   a.K = s.K;
-  g16::launch<g16::KC, g16::KC, true>(g16::plan(s.N, 2 * (int64_t)s.F, s.K, 1, 1, false, false, 1.5).tile, a, EpiGate<ACT>{g, u, h, s.F8}, st);
+  g16::launch<g16::KC, g16::KC, true>(gate_tile(s), a, EpiGate<ACT>{g, u, h, s.F8}, st);
 }
 
 template <int ACT>
@@ -333,10 +336,20 @@ void grad_gate(const FfnShape& s, const u16* dy, int64_t lddy, const FfnWeights&
 
 }  // namespace
 
+#ifndef MIHVD_F16
+FfnPlan ffn_plan(const FfnShape& s) {
+  const g16::Plan p[4] = {g16::product_plan(s.N, s.K, s.F), g16::product_plan(s.K, s.F, s.N),
+                          g16::product_plan(s.F, s.K, s.N, 1, 2), g16::product_plan(s.N, s.K, s.F, 2)};
+  FfnPlan r{s.N <= FEW ? 0 : gate_tile(s), {}, {}};
+  for (int i = 0; i < 4; ++i) r.tile[i] = p[i].tile, r.splits[i] = p[i].splits;
+  return r;
+}
+#endif
+
 void ffn_forward_16(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeights& w, int act, u16* g, u16* u, u16* h,
                     u16* y, c10::Device dev, hipStream_t st) {
   if (s.N <= 16) return forward_few<1>(s, x, ldx, w, act, g, u, h, y, st);
-  if (s.N <= 32) return forward_few<2>(s, x, ldx, w, act, g, u, h, y, st);
+  if (s.N <= FEW) return forward_few<2>(s, x, ldx, w, act, g, u, h, y, st);
   switch (act) {
     case ACT_SILU: up_gate<ACT_SILU>(s, x, ldx, w, g, u, h, st); break;
     case ACT_GELU: up_gate<ACT_GELU>(s, x, ldx, w, g, u, h, st); break;

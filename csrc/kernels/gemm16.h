@@ -721,7 +721,9 @@ inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 // Output tiles; every shape runs four waves, two along each side. T256 and T128 double buffer (one and
 // two blocks a CU); T64 keeps four buffers (two blocks a CU): for products with few tiles, whose time is
 // the copies' latency.
-enum { T64 = 64, T128 = 128, T256 = 256 };
+enum { T64 = 64, T128 = 128, T256 = 256, T_ALL = T64 | T128 | T256 };
+// DUAL has no 64 (its columns come in blocks of 64 of each matrix); launch_small no 256.
+enum { T_DUAL = T128 | T256, T_SMALL = T64 | T128 };
 
 template <int LM, int LN, int T, int S, bool DUAL, int RAG, int PL = 1, class Epi>
 void launch_tile(Args a, Ragged g, const Epi& e, hipStream_t stream) {
@@ -776,16 +778,19 @@ void launch_split(int tile, const Args& a, const Epi& e, hipStream_t stream, con
 // MI355X (16-bit operands, K = 768 and more): a 64-wide k tile takes 1.45 at 256x256; at 128x128 0.67 with
 // one block on a CU and 0.93 with two; at 64x64 0.3 and 0.57. A tile's end costs about 7, 4 and 1.5
 // more (`epi` scales it for epilogues that compute), a launch 4; splits pay a second launch and their
-// slabs' way through memory at 4 TB/s.
+// slabs' way through memory at 4 TB/s. `allowed`: the tiles that
+// the launch has.
 struct Plan {
   int tile, splits;
 };
-inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym, bool may_split, double epi = 1.0) {
+inline Plan plan(int64_t M, int64_t N, int64_t K, int nseg, int batch, bool sym, bool may_split, double epi = 1.0,
+                 int allowed = T_ALL) {
   Plan best{T128, 1};
   double best_t = 1e30;
   const int64_t kt = (int64_t)cdiv(K, BK) * nseg;
   const int cus = device_cu_count();
   for (int tile : {T256, T128, T64}) {
+    if (!(allowed & tile)) continue;
     const int64_t tm = cdiv(M, tile), tn = cdiv(N, tile);
     const int64_t tiles = (sym ? tm * (tm + 1) / 2 : tm * tn) * batch;
     for (int s = 1; s <= 64 && (s == 1 || (may_split && kt / s >= 4)); ++s) {
@@ -942,10 +947,13 @@ static __global__ void __launch_bounds__(256) slab_sum(const float* __restrict__
 
 // A product rounded once into 16-bit outputs (one or two batch entries), split along k when its
 // tiles alone leave CUs idle.
+inline Plan product_plan(int64_t M, int64_t N, int64_t K, int nseg = 1, int batch = 1) {
+  return plan(M, N, K, nseg, batch, false, true);
+}
 template <int LM, int LN>
 void product(Args a, u16* out0, u16* out1, int64_t ldo, float alpha, const float* dev_alpha, c10::Device dev,
              hipStream_t stream) {
-  const Plan p = plan(a.M, a.N, a.K, a.nseg, a.batch, false, true);
+  const Plan p = product_plan(a.M, a.N, a.K, a.nseg, a.batch);
   a.splits = p.splits;
   if (p.splits == 1) {
     launch<LM, LN>(p.tile, a, EpiStore{{out0, out1}, ldo, alpha, dev_alpha}, stream);

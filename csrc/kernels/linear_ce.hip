@@ -478,8 +478,7 @@ void lce_plan(LceShape& s) {
 void lce_plan_backward(LceShape& s, LceScratch& x, bool bias) {
   // the bias gradient's sums on top of the accumulators spill at 256x256 (135 us a piece against 84
   // without them, at 1229 x 30522 x 768); at 128x128 they fit
-  x.dz_tile = g16::plan(s.N, std::min(x.piece, s.V), s.K, 1, 1, false, false, 1.5).tile;
-  if (bias && x.dz_tile == g16::T256) x.dz_tile = g16::T128;
+  x.dz_tile = g16::plan(s.N, std::min(x.piece, s.V), s.K, 1, 1, false, false, 1.5, bias ? g16::T_SMALL : g16::T_ALL).tile;
   const g16::Plan p = g16::plan(s.N, s.K, x.piece, 1, 1, false, true);
   x.dh_tile = p.tile;
   x.splits = p.splits;

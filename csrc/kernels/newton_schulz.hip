@@ -415,13 +415,33 @@ void with_kind(const NsParams& p, F&& f) {
 
 }  // namespace
 
+// Tiles of the three products of a step; the last one of all has its own epilogue, hence a fourth.
+NsPlan ns_plan(const NsGroup& g) {
+  using namespace g16;
+  const int64_t sp = g.side;
+  int64_t total = 0;
+  for (int i = 0; i < g.count; ++i) total += g.m[i].len;
+  auto half = [&](int t) { return (int64_t)cdiv(sp, t) * (cdiv(sp, t) + 1) / 2 * g.count; };  // tiles of a symmetric product
+  auto full = [&](int t) {
+    int64_t n = 0;
+    for (int i = 0; i < g.count; ++i) n += (int64_t)cdiv(sp, t) * cdiv(g.m[i].len, t);
+    return n;
+  };
+  if (g.planes == 2) {
+    const int upd = plan_split(full(128), full(64), sp);
+    return {plan_split(half(128), half(64), total / g.count), plan_split(half(128), half(64), sp), upd, upd};
+  }
+  return {plan(sp, sp, total / g.count, 1, g.count, true, false).tile, plan(sp, sp, sp, 1, g.count, true, false, 1.0, T_SMALL).tile,
+          plan(sp, total, sp, 1, 1, false, false).tile, plan(sp, total, sp, 1, 1, false, false, 1.0, T_SMALL).tile};
+}
+
 void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_t st) {
   using namespace g16;
   NsOut out{};
   Ragged rg;
   rg.rows = g.side;
   rg.count = g.count;
-  int64_t most = 0, total = 0;
+  int64_t most = 0;
   for (int i = 0; i < g.count; ++i) {
     out.dst[i] = g.m[i].dst;
     out.rows[i] = g.m[i].rows;
@@ -430,7 +450,6 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     rg.len[i] = g.m[i].len;
     rg.off[i] = g.m[i].off;
     most = std::max<int64_t>(most, g.m[i].len);
-    total += g.m[i].len;
   }
   const int grid = (int)std::min<int64_t>(2048, g.side / 64 * (most / 64));
   with_kind(p, [&](auto K) {
@@ -444,22 +463,7 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
   // The sides are padded to 64 with zeros, which the products keep: a zero row or column of X gives zero
   // rows and columns of A, B and the next X.
   const int64_t sp = g.side, pa = sp * sp;
-  auto half = [&](int t) { return (int64_t)cdiv(sp, t) * (cdiv(sp, t) + 1) / 2 * g.count; };  // tiles of a symmetric product
-  auto full = [&](int t) {
-    int64_t n = 0;
-    for (int i = 0; i < g.count; ++i) n += (int64_t)cdiv(sp, t) * cdiv(g.m[i].len, t);
-    return n;
-  };
-  int t_gram, t_poly, t_upd;
-  if (g.planes == 2) {
-    t_gram = plan_split(half(128), half(64), total / g.count);
-    t_poly = plan_split(half(128), half(64), sp);
-    t_upd = plan_split(full(128), full(64), sp);
-  } else {
-    t_gram = plan(sp, sp, total / g.count, 1, g.count, true, false).tile;
-    t_poly = plan(sp, sp, sp, 1, g.count, true, false).tile;
-    t_upd = plan(sp, total, sp, 1, 1, false, false).tile;
-  }
+  const NsPlan tile = ns_plan(g);
   u16 *x = sc.x0, *y = sc.x1;
   for (int it = 0; it < p.steps; ++it) {
     Args a;
@@ -467,20 +471,20 @@ void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& sc, hipStream_
     a.sym = 1;
     a.M = a.N = g.side;
     a.m = a.n = ragged_side(x, g.side);
-    run_product<KC, KC, 1, false>(g.planes, t_gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f, 0.f},
+    run_product<KC, KC, 1, false>(g.planes, tile.gram, a, EpiPlanes<false>{sc.gram, nullptr, sp, pa, g.planes, 1, INV_S, 0.f, 0.f},
                                   st, rg);
     a.K = g.side;
     a.m = a.n = square_side(sc.gram, sp, g.planes);
-    run_product<KC, KC, 0, true>(g.planes, t_poly, a,
+    run_product<KC, KC, 0, true>(g.planes, tile.poly, a,
                                  EpiPlanes<true>{sc.poly, sc.gram, sp, pa, g.planes, 1, p.c * INV_S, p.b, p.a * S}, st, rg);
     a.sym = 0;
     a.m = square_side(sc.poly, sp, g.planes);
     a.n = ragged_side(x, 0);
     if (it + 1 < p.steps) {
-      run_product<KC, KS, 2, false>(g.planes, t_upd, a, EpiPlanes<false>{y, nullptr, 0, 0, g.planes, 0, INV_S, 0.f, 0.f}, st, rg);
+      run_product<KC, KS, 2, false>(g.planes, tile.update, a, EpiPlanes<false>{y, nullptr, 0, 0, g.planes, 0, INV_S, 0.f, 0.f}, st, rg);
     } else {
       auto fin = [&](auto K) {
-        run_product<KC, KS, 2, true>(g.planes, t_upd, a, EpiFinal<K.value>{out, INV_S * INV_S, p.decay}, st, rg);
+        run_product<KC, KS, 2, true>(g.planes, tile.last, a, EpiFinal<K.value>{out, INV_S * INV_S, p.decay}, st, rg);
       };
       if (p.muon) fin(std::integral_constant<int, 3>{});
       else with_kind(p, fin);

@@ -74,6 +74,12 @@ struct FfnWeights {
 };
 enum { ACT_SILU = 0, ACT_GELU, ACT_GELU_TANH, ACT_RELU, ACT_SIGMOID, ACT_COUNT };
 
+// Tiles and k splits: the gate product (0: the kernels for few rows); y, dWd, the batch of dWg and dWu, dx.
+struct FfnPlan {
+  int gate, tile[4], splits[4];
+};
+FfnPlan ffn_plan(const FfnShape& s);
+
 MIHVD_TRANSFORMER_DECLS
 namespace f16 {
 MIHVD_TRANSFORMER_DECLS
@@ -109,6 +115,10 @@ struct NsScratch {
   double* partial;    // [count][NS_PART]
 };
 constexpr int NS_PART = 64;
+struct NsPlan {
+  int gram, poly, update, last;
+};
+NsPlan ns_plan(const NsGroup& g);
 void ns_run(const NsGroup& g, const NsParams& p, const NsScratch& s, hipStream_t st);
 
 }  // namespace mihvd

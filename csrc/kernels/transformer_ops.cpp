@@ -164,6 +164,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   return {loss, hc, meta, lse};
 }
 
+void lce_pieces(const LceShape& s, LceScratch& x) {
+  const int64_t N = s.N;
+  x.piece = (int)std::min<int64_t>(up8(s.V), std::max<int64_t>(256, DZ_BYTES / (2 * N) / 256 * 256));
+  x.ldz = up8(x.piece);
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& gout, const at::Tensor& hc,
                                                             const at::Tensor& w, const c10::optional<at::Tensor>& bias_in,
                                                             const at::Tensor& meta, const at::Tensor& lse,
@@ -202,9 +208,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   }
   const Mat wm = mat(w);
   LceScratch x{};
-  x.piece = (int)std::min<int64_t>(up8(V), std::max<int64_t>(256, DZ_BYTES / (2 * N) / 256 * 256));
-  x.ldz = up8(x.piece);
   LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0, 0};
+  lce_pieces(s, x);
   lce_plan_backward(s, x, bias.has_value());
   at::Tensor dz = at::empty({N, x.ldz}, w.options()), dbp, slab;
   x.dz = m16(dz);
@@ -571,10 +576,39 @@ void muon_step_in_place(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, 
     for (const at::Tensor& t : *list) torch::autograd::impl::bump_version(t);
 }
 
+// How a call of these sizes runs, for tests that have to reach every kernel and for reading profiles:
+//   linear_cross_entropy [rows, hidden, vocabulary, bias]: tiles of the logits, dz, dh, dW; dh's splits at most; pieces
+//   gated_ffn [rows, hidden, inner]: the gate product's tile (0: few rows); tile, splits of y, dWd, dWg and dWu, dx
+//   orthogonalize [batch, rows, cols, planes]: tiles of X X^T, the polynomial, X's update, the last update
+std::vector<int64_t> transformer_plan(c10::string_view op, std::vector<int64_t> z) {
+  if (op == "linear_cross_entropy" && z.size() == 4) {
+    LceShape s{(int)z[0], (int)z[1], (int)up8(z[1]), (int)z[2], 0, 0, 0};
+    LceScratch x{};
+    lce_plan(s);
+    lce_pieces(s, x);
+    lce_plan_backward(s, x, z[3] != 0);
+    return {s.tile, x.dz_tile, x.dh_tile, x.dw_tile, x.splits, cdiv(s.V, x.piece)};
+  }
+  if (op == "gated_ffn" && z.size() == 3) {
+    const FfnPlan p = ffn_plan({(int)z[0], (int)z[1], (int)up8(z[1]), (int)z[2], (int)up8(z[2])});
+    std::vector<int64_t> r{p.gate};
+    for (int i = 0; i < 4; ++i) r.insert(r.end(), {p.tile[i], p.splits[i]});
+    return r;
+  }
+  TORCH_CHECK_VALUE(op == "orthogonalize" && z.size() == 4, "transformer_plan: linear_cross_entropy, gated_ffn or orthogonalize "
+                    "and its sizes");
+  NsGroup g{};
+  g.planes = (int)z[3];
+  for (int64_t i = 0; i < z[0]; ++i) ns_add(g, z[1], z[2], nullptr, nullptr, nullptr, 0.f);
+  const NsPlan p = ns_plan(g);
+  return {p.gram, p.poly, p.update, p.last};
+}
+
 }  // namespace
 }  // namespace mihvd
 
 TORCH_LIBRARY_FRAGMENT(mihvd, m) {
+  m.def("transformer_plan(str op, int[] sizes) -> int[]", &mihvd::transformer_plan);
   m.def("linear_cross_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, int ignore_index, int reduction) "
         "-> Tensor");
   m.def("gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor");

@@ -134,3 +134,37 @@ def test_orthogonalize_far_norms_cpu(by, eps):
     want = ns64(x, eps=0.0)
     got = orthogonalize(x * by, eps=eps)
     assert float((got.double() - want).norm()) <= 64 * 5 * 2.0 ** -24 * float(want.norm())
+
+
+def _plan(op, *sizes):
+    from mihvd import _native
+
+    if not _native.load_kernels():
+        pytest.skip("no kernel library")
+    return list(torch.ops.mihvd.transformer_plan(op, list(sizes)))
+
+
+def _estimate(tile, m, n, k, epi=1.0, batch=1, cus=256):
+    """us of an unsplit product, by the measured terms that the plan names."""
+    tiles = -(-m // tile) * -(-n // tile) * batch
+    two = tile < 256 and tiles > cus
+    unit = {256: 1.45, 128: 0.93 if two else 0.67, 64: 0.57 if two else 0.3}[tile]
+    return 4.0 + -(-tiles // (2 * cus if two else cus)) * (-(-k // 64) * unit + epi * {256: 7.0, 128: 4.0, 64: 1.5}[tile])
+
+
+@pytest.mark.parametrize("what,sizes", [("gate", (391, 32, 9208)), ("gate", (43318, 21, 94)), ("gate", (100, 512, 1000)),
+                                        ("dz", (37170, 138, 146)), ("dz", (1086, 283, 7189)), ("dz", (1229, 768, 30522)),
+                                        ("last", (7, 192, 4864)), ("last", (11, 192, 3584)), ("last", (1, 4100, 2100))])
+def test_plans_price_the_tiles_that_run(what, sizes):
+    """Products whose kernels have two of the three tiles take the cheaper of those two."""
+    if what == "gate":
+        n, k, f = sizes
+        got, tiles, args = _plan("gated_ffn", n, k, f)[0], (128, 256), (n, 2 * f, k, 1.5)
+    elif what == "dz":
+        n, k, v = sizes
+        got, tiles, args = _plan("linear_cross_entropy", n, k, v, 1)[1], (64, 128), (n, v, k, 1.5)
+    else:
+        b, r, c = sizes
+        side, length = (-(-min(r, c) // 64) * 64, -(-max(r, c) // 64) * 64)
+        got, tiles, args = _plan("orthogonalize", b, r, c, 1)[3], (64, 128), (side, length * b, side)
+    assert got == min(tiles, key=lambda t: _estimate(t, *args))
