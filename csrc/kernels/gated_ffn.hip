@@ -363,7 +363,7 @@ void ffn_forward_16(const FfnShape& s, const u16* x, int64_t ldx, const FfnWeigh
   a.M = s.N;
   a.N = s.K;
   a.K = s.F;
-  g16::product<g16::KC, g16::KC>(a, y, nullptr, s.K, 1.f, nullptr, dev, st);
+  g16::product<g16::KC, g16::KC>(a, y, nullptr, s.K, dev, st);
 }
 
 void ffn_backward_16(const FfnShape& s, const u16* dy, int64_t lddy, const u16* x, int64_t ldx, const FfnWeights& w,
@@ -385,7 +385,7 @@ void ffn_backward_16(const FfnShape& s, const u16* dy, int64_t lddy, const u16* 
     a.M = s.K;
     a.N = s.F;
     a.K = s.N;
-    g16::product<g16::KS, g16::KS>(a, dwd, nullptr, s.F, 1.f, nullptr, dev, st);
+    g16::product<g16::KS, g16::KS>(a, dwd, nullptr, s.F, dev, st);
   }
   if (dwg || dwu) {
     g16::Args a;
@@ -396,7 +396,7 @@ void ffn_backward_16(const FfnShape& s, const u16* dy, int64_t lddy, const u16* 
     a.N = s.K;
     a.K = s.N;
     a.batch = dwg && dwu ? 2 : 1;
-    g16::product<g16::KS, g16::KS>(a, dwg ? dwg : dwu, dwg ? dwu : nullptr, s.K, 1.f, nullptr, dev, st);
+    g16::product<g16::KS, g16::KS>(a, dwg ? dwg : dwu, dwg ? dwu : nullptr, s.K, dev, st);
   }
   if (dx) {
     g16::Args a;
@@ -408,7 +408,7 @@ void ffn_backward_16(const FfnShape& s, const u16* dy, int64_t lddy, const u16* 
     a.M = s.N;
     a.N = s.K;
     a.K = s.F;
-    g16::product<g16::KC, g16::KS>(a, dx, nullptr, s.K, 1.f, nullptr, dev, st);
+    g16::product<g16::KC, g16::KS>(a, dx, nullptr, s.K, dev, st);
   }
 }
 

@@ -928,21 +928,19 @@ struct EpiSlab {
   }
 };
 
-// out[batch][m][n] = alpha * sum of the slabs, in split order
+// out[batch][m][n] = sum of the slabs, in split order
 static __global__ void __launch_bounds__(256) slab_sum(const float* __restrict__ slab, int splits, int64_t stride,
                                                        int64_t ld, int M, int N, u16* __restrict__ out0,
-                                                       u16* __restrict__ out1, int64_t ldo, float alpha,
-                                                       const float* __restrict__ dev_alpha) {
+                                                       u16* __restrict__ out1, int64_t ldo) {
   const int n4 = (N + 3) >> 2;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t m = i / n4;
   const int n = (int)(i - m * n4) * 4;
   if (m >= M) return;
-  const float al = dev_alpha ? alpha * *dev_alpha : alpha;
   const float* p = slab + (int64_t)blockIdx.y * splits * stride + m * ld + n;
   f32x4 s = *reinterpret_cast<const f32x4*>(p);
   for (int q = 1; q < splits; ++q) s += *reinterpret_cast<const f32x4*>(p + q * stride);
-  store4((blockIdx.y ? out1 : out0) + m * ldo, n, N, (ldo & 3) == 0, s[0] * al, s[1] * al, s[2] * al, s[3] * al);
+  store4((blockIdx.y ? out1 : out0) + m * ldo, n, N, (ldo & 3) == 0, s[0], s[1], s[2], s[3]);
 }
 
 // A product rounded once into 16-bit outputs (one or two batch entries), split along k when its
@@ -951,19 +949,18 @@ inline Plan product_plan(int64_t M, int64_t N, int64_t K, int nseg = 1, int batc
   return plan(M, N, K, nseg, batch, false, true);
 }
 template <int LM, int LN>
-void product(Args a, u16* out0, u16* out1, int64_t ldo, float alpha, const float* dev_alpha, c10::Device dev,
-             hipStream_t stream) {
+void product(Args a, u16* out0, u16* out1, int64_t ldo, c10::Device dev, hipStream_t stream) {
   const Plan p = product_plan(a.M, a.N, a.K, a.nseg, a.batch);
   a.splits = p.splits;
   if (p.splits == 1) {
-    launch<LM, LN>(p.tile, a, EpiStore{{out0, out1}, ldo, alpha, dev_alpha}, stream);
+    launch<LM, LN>(p.tile, a, EpiStore{{out0, out1}, ldo, 1.f, nullptr, nullptr}, stream);
     return;
   }
   const int64_t ld = up8(a.N), stride = (int64_t)a.M * ld;
   at::Tensor slab = at::empty({a.batch * a.splits * stride}, at::TensorOptions().device(dev).dtype(at::kFloat));
   launch<LM, LN>(p.tile, a, EpiSlab{slab.data_ptr<float>(), ld, stride, a.splits, 0}, stream);
   slab_sum<<<dim3(cdiv((int64_t)a.M * ((a.N + 3) / 4), 256), a.batch), 256, 0, stream>>>(
-      slab.data_ptr<float>(), a.splits, stride, ld, a.M, a.N, out0, out1, ldo, alpha, dev_alpha);
+      slab.data_ptr<float>(), a.splits, stride, ld, a.M, a.N, out0, out1, ldo);
 }
 
 }  // namespace g16
