@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/library.h>
 
 #include <initializer_list>
@@ -22,6 +23,7 @@ namespace mihvd {
 namespace {
 
 constexpr int64_t MAX_ROWS = int64_t(1) << 30, MAX_LD = int64_t(1) << 22;
+constexpr int64_t LCE_CHUNKS = 4096;
 constexpr int64_t DZ_BYTES = int64_t(512) << 20;  // bound on the gradient piece that backward holds
 
 inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
@@ -135,12 +137,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward(const at:
   if (bias_in) bias = bias_in->contiguous();
   LceShape s{(int)N, (int)K, (int)K8, (int)V, 0, 0, 0};
   // Blocks that count all labels ahead of their rows for themselves read 64 KB on average at 16384 rows; past that
-  // the chunks (at most 4096) are counted ahead, which costs a launch.
-  if (N > 16384) s.chunk = (int)(cdiv(cdiv(N, 4096), 1024) * 1024);
-  const int64_t nmeta = 3 * N + 2 + (s.chunk ? cdiv(N, s.chunk) : 0);
+  // the chunks (at most LCE_CHUNKS) are counted ahead, which costs a launch.
+  if (N > 16384) s.chunk = (int)(cdiv(cdiv(N, LCE_CHUNKS), 1024) * 1024);
   at::Tensor loss = reduction ? at::empty({}, f32) : at::empty({N}, f32);
   at::Tensor hc = at::empty({N, K8}, h.options()), lse = at::empty({N, 2}, f32);
-  at::Tensor meta = at::empty({nmeta}, h.options().dtype(at::kInt));
+  at::Tensor meta = at::empty({3 * N + 2 + LCE_CHUNKS}, h.options().dtype(at::kInt));
   if (N == 0) {
     if (reduction) loss.fill_(reduction == 1 ? NAN : 0.f);
     meta.zero_();
@@ -170,10 +171,16 @@ void lce_pieces(const LceShape& s, LceScratch& x) {
   x.ldz = up8(x.piece);
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& gout, const at::Tensor& hc,
-                                                            const at::Tensor& w, const c10::optional<at::Tensor>& bias_in,
-                                                            const at::Tensor& meta, const at::Tensor& lse,
-                                                            int64_t reduction, bool need_h, bool need_w, bool need_b) {
+// The gradients that are asked for, in the order hidden, weight, bias.
+std::vector<at::Tensor> wanted(std::initializer_list<at::Tensor> ts) {
+  std::vector<at::Tensor> r;
+  for (const at::Tensor& t : ts)
+    if (t.defined()) r.push_back(t);
+  return r;
+}
+std::vector<at::Tensor> lce_backward(const at::Tensor& gout, const at::Tensor& hc, const at::Tensor& w,
+                                     const c10::optional<at::Tensor>& bias_in, const at::Tensor& meta, const at::Tensor& lse,
+                                     int64_t reduction, bool need_h, bool need_w, bool need_b) {
   const int64_t N = lse.size(0), V = w.size(0), K = w.size(1), K8 = up8(K);
   TORCH_CHECK_VALUE(hc.dim() == 2 && hc.size(0) == N && hc.size(1) == K8 && hc.is_contiguous() &&
                         meta.numel() >= 3 * N + 2 && hc.scalar_type() == w.scalar_type(),
@@ -195,7 +202,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   if (N == 0) {
     if (need_w) dw.zero_();
     if (need_b) db.zero_();
-    return {dh, dw, db};
+    return wanted({dh, dw, db});
   }
   const LceRows rw = rows_of(meta, N);
   LceGrad g{gout.data_ptr<float>(), reduction == 1 ? rw.cnt : nullptr, nullptr};
@@ -226,7 +233,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> lce_backward(const at::Tensor& go
   run(s, rw, g, p16(hc), wm.p, wm.ld, bias ? bias->data_ptr() : nullptr, bias_kind(bias),
       reinterpret_cast<const float2*>(lse.data_ptr<float>()), x, m16(dh), m16(dw), need_b ? db.data_ptr() : nullptr, st);
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  return {dh, dw, db};
+  return wanted({dh, dw, db});
 }
 
 // ------------------------------------------------------------------------------------------ //
@@ -277,11 +284,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_forward(const at:
     run(s, xm.p, xm.ld, wm.w, (int)act, m16(g), m16(u), m16(h), m16(y), x.device(), cur_stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
-  if (!save) h = at::Tensor();
   return {y, g, u, h};
 }
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_train(const at::Tensor& x, const at::Tensor& wg,
+                                                                     const at::Tensor& wu, const at::Tensor& wd, int64_t act) {
+  return ffn_forward(x, wg, wu, wd, act, true);
+}
+at::Tensor ffn_infer(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t act) {
+  return std::get<0>(ffn_forward(x, wg, wu, wd, act, false));
+}
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
+std::vector<at::Tensor> ffn_backward(
     const at::Tensor& dy, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
     const at::Tensor& g, const at::Tensor& u, const at::Tensor& h, int64_t act, bool need_x, bool need_g, bool need_u,
     bool need_d) {
@@ -302,7 +315,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
   if (N == 0) {
     for (at::Tensor* t : {&dwg, &dwu, &dwd})
       if (t->defined()) t->zero_();
-    return {dx, dwg, dwu, dwd};
+    return wanted({dx, dwg, dwu, dwd});
   }
   at::Tensor dgu;
   if (need_x || need_g || need_u) dgu = at::empty({N, 2 * F8}, x.options());
@@ -313,7 +326,71 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_backward(
   run(s, dym.p, dym.ld, xm.p, xm.ld, wm.w, (int)act, p16(g), p16(u), p16(h), m16(dgu), m16(dx), m16(dwg), m16(dwu),
       m16(dwd), x.device(), cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  return {dx, dwg, dwu, dwd};
+  return wanted({dx, dwg, dwu, dwd});
+}
+
+// ------------------------------------------------------------------------------------------ //
+// Shapes and types alone, for tensors without data (tracing): the checks are the kernels' own.
+
+c10::SymInt sym8(const c10::SymInt& n) { return (n + 7) / 8 * 8; }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> lce_forward_meta(const at::Tensor& h, const at::Tensor&,
+                                                                            const at::Tensor&, const c10::optional<at::Tensor>&,
+                                                                            int64_t, int64_t reduction) {
+  const c10::SymInt N = h.sym_size(0);
+  const auto f32 = h.options().dtype(at::kFloat);
+  return {reduction ? at::empty({}, f32) : at::empty_symint({N}, f32), at::empty_symint({N, sym8(h.sym_size(1))}, h.options()),
+          at::empty_symint({N * 3 + (2 + LCE_CHUNKS)}, h.options().dtype(at::kInt)), at::empty_symint({N, 2}, f32)};
+}
+std::vector<at::Tensor> lce_backward_meta(const at::Tensor&, const at::Tensor& hc, const at::Tensor& w,
+                                          const c10::optional<at::Tensor>& bias, const at::Tensor&, const at::Tensor&, int64_t,
+                                          bool need_h, bool need_w, bool need_b) {
+  at::Tensor dh, dw, db;
+  if (need_h) dh = at::empty_symint({hc.sym_size(0), w.sym_size(1)}, w.options());
+  if (need_w) dw = at::empty_symint(w.sym_sizes(), w.options());
+  if (need_b && bias) db = at::empty_symint(bias->sym_sizes(), bias->options());
+  return wanted({dh, dw, db});
+}
+at::Tensor ffn_infer_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t) {
+  return at::empty_symint(x.sym_sizes(), x.options());
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> ffn_train_meta(const at::Tensor& x, const at::Tensor& wg,
+                                                                          const at::Tensor&, const at::Tensor&, int64_t) {
+  const std::vector<c10::SymInt> inner{x.sym_size(0), sym8(wg.sym_size(0))};
+  auto mid = [&] { return at::empty_symint(inner, x.options()); };
+  return {at::empty_symint(x.sym_sizes(), x.options()), mid(), mid(), mid()};
+}
+std::vector<at::Tensor> ffn_backward_meta(const at::Tensor&, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                                          const at::Tensor& wd, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
+                                          bool need_x, bool need_g, bool need_u, bool need_d) {
+  auto like = [&](bool need, const at::Tensor& t) { return need ? at::empty_symint(t.sym_sizes(), x.options()) : at::Tensor(); };
+  return wanted({like(need_x, x), like(need_g, wg), like(need_u, wu), like(need_d, wd)});
+}
+
+// The operators that have kernels, reached through the dispatcher, so that tracing sees them.
+template <class F>
+c10::TypedOperatorHandle<F> op_of(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+const auto& lce_forward_op() {
+  static const auto op = op_of("mihvd::_linear_cross_entropy", &lce_forward);
+  return op;
+}
+const auto& lce_backward_op() {
+  static const auto op = op_of("mihvd::_linear_cross_entropy_backward", &lce_backward);
+  return op;
+}
+const auto& ffn_infer_op() {
+  static const auto op = op_of("mihvd::_gated_ffn", &ffn_infer);
+  return op;
+}
+const auto& ffn_train_op() {
+  static const auto op = op_of("mihvd::_gated_ffn_train", &ffn_train);
+  return op;
+}
+const auto& ffn_backward_op() {
+  static const auto op = op_of("mihvd::_gated_ffn_backward", &ffn_backward);
+  return op;
 }
 
 // ------------------------------------------------------------------------------------------ //
@@ -373,11 +450,21 @@ void refuse_eager_leaves(const char* op) {
   }
 }
 
+// The wanted gradients back in their places.
+template <size_t N>
+variable_list spread(std::vector<at::Tensor> got, const bool (&need)[N]) {
+  variable_list r(N);
+  size_t k = 0;
+  for (size_t i = 0; i < N; ++i)
+    if (need[i]) r[i] = std::move(got[k++]);
+  return r;
+}
+
 struct LceFunction : torch::autograd::Function<LceFunction> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
                             const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, hc, meta, lse] = lce_forward(h, w, labels, bias, ignore_index, reduction);
+    auto [loss, hc, meta, lse] = lce_forward_op().call(h, w, labels, bias, ignore_index, reduction);
     ctx->save_for_backward({hc, w, meta, lse, bias ? *bias : at::Tensor()});
     ctx->saved_data["reduction"] = reduction;
     return loss;
@@ -387,12 +474,13 @@ struct LceFunction : torch::autograd::Function<LceFunction> {
     const variable_list t = ctx->get_saved_variables();
     c10::optional<at::Tensor> bias;
     if (t[4].defined()) bias = t[4];
-    variable_list grads(3);
+    const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), bias && ctx->needs_input_grad(3)};
+    variable_list grads;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      std::tie(grads[0], grads[1], grads[2]) =
-          lce_backward(gout[0], t[0], t[1], bias, t[2], t[3], ctx->saved_data["reduction"].toInt(),
-                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), bias && ctx->needs_input_grad(3));
+      grads = spread(lce_backward_op().call(gout[0], t[0], t[1], bias, t[2], t[3], ctx->saved_data["reduction"].toInt(), need[0],
+                                            need[1], need[2]),
+                     need);
     }
     once(gout[0], grads);
     return {grads[0], grads[1], at::Tensor(), grads[2], at::Tensor(), at::Tensor()};
@@ -401,19 +489,18 @@ struct LceFunction : torch::autograd::Function<LceFunction> {
 
 at::Tensor linear_cross_entropy(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
                                 const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
-  return std::get<0>(lce_forward(h, w, labels, bias, ignore_index, reduction));
-}
-at::Tensor linear_cross_entropy_autograd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& labels,
-                                         const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction) {
   refuse_tangents("linear_cross_entropy", {&h, &w, bias ? &*bias : &w});
-  return LceFunction::apply(h, w, labels, bias, ignore_index, reduction);
+  if (at::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad() || (bias && bias->requires_grad())))
+    return LceFunction::apply(h, w, labels, bias, ignore_index, reduction);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(lce_forward_op().call(h, w, labels, bias, ignore_index, reduction));
 }
 
 struct FfnFunction : torch::autograd::Function<FfnFunction> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                             const at::Tensor& wd, int64_t act) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, g, u, h] = ffn_forward(x, wg, wu, wd, act, true);
+    auto [y, g, u, h] = ffn_train_op().call(x, wg, wu, wd, act);
     ctx->save_for_backward({x, wg, wu, wd, g, u, h});
     ctx->saved_data["act"] = act;
     return y;
@@ -421,13 +508,13 @@ struct FfnFunction : torch::autograd::Function<FfnFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
     refuse_eager_leaves("gated_ffn");
     const variable_list t = ctx->get_saved_variables();
-    variable_list grads(4);
+    const bool need[4] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)};
+    variable_list grads;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      std::tie(grads[0], grads[1], grads[2], grads[3]) =
-          ffn_backward(dy[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], ctx->saved_data["act"].toInt(),
-                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2),
-                       ctx->needs_input_grad(3));
+      grads = spread(ffn_backward_op().call(dy[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], ctx->saved_data["act"].toInt(),
+                                            need[0], need[1], need[2], need[3]),
+                     need);
     }
     once(dy[0], grads);
     grads.emplace_back();
@@ -436,15 +523,11 @@ struct FfnFunction : torch::autograd::Function<FfnFunction> {
 };
 
 at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t act) {
-  return std::get<0>(ffn_forward(x, wg, wu, wd, act, false));
-}
-at::Tensor gated_ffn_autograd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
-                              int64_t act) {
   refuse_tangents("gated_ffn", {&x, &wg, &wu, &wd});
   if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad()))
     return FfnFunction::apply(x, wg, wu, wd, act);
   at::AutoDispatchBelowADInplaceOrView below;
-  return gated_ffn(x, wg, wu, wd, act);
+  return ffn_infer_op().call(x, wg, wu, wd, act);
 }
 
 // ------------------------------------------------------------------------------------------ //
@@ -564,6 +647,12 @@ void muon_step(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vect
   }
 }
 
+at::Tensor newton_schulz_meta(const at::Tensor& x, int64_t, double, double, double, double, bool) {
+  return at::empty_symint(x.sym_sizes(), x.options());
+}
+void muon_step_meta(std::vector<at::Tensor>, std::vector<at::Tensor>, std::vector<at::Tensor>, double, double, bool, double, int64_t,
+                    double, double, double, double, int64_t, bool) {}
+
 // The weights and momenta count as changed in place: a backward pass that saved a weight before the step raises.
 void muon_step_in_place(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, std::vector<at::Tensor> ms, double lr,
                         double momentum, bool nesterov, double weight_decay, int64_t steps, double a, double b, double c,
@@ -610,23 +699,40 @@ std::vector<int64_t> transformer_plan(c10::string_view op, std::vector<int64_t> 
 TORCH_LIBRARY_FRAGMENT(mihvd, m) {
   m.def("transformer_plan(str op, int[] sizes) -> int[]", &mihvd::transformer_plan);
   m.def("linear_cross_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, int ignore_index, int reduction) "
-        "-> Tensor");
-  m.def("gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor");
+        "-> Tensor", &mihvd::linear_cross_entropy);
+  m.def("gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor", &mihvd::gated_ffn);
+  // what those two are made of: loss, packed rows, row numbers and labels, (maximum, log of the sum); y, g, u, h
+  m.def("_linear_cross_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, int ignore_index, int reduction) "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_linear_cross_entropy_backward(Tensor grad, Tensor rows, Tensor weight, Tensor? bias, Tensor meta, Tensor lse, "
+        "int reduction, bool need_hidden, bool need_weight, bool need_bias) -> Tensor[]");
+  m.def("_gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor");
+  m.def("_gated_ffn_train(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_gated_ffn_backward(Tensor grad, Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, Tensor g, Tensor u, Tensor h, "
+        "int act, bool need_x, bool need_gate, bool need_up, bool need_down) -> Tensor[]");
   m.def("newton_schulz(Tensor x, int steps, float a, float b, float c, float eps, bool split) -> Tensor");
   m.def("muon_step(Tensor(a!)[] p, Tensor[] g, Tensor(b!)[] m, float lr, float momentum, bool nesterov, "
         "float weight_decay, int steps, float a, float b, float c, float eps, int scale_mode, bool split) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(mihvd, CUDA, m) {
-  m.impl("linear_cross_entropy", &mihvd::linear_cross_entropy);
-  m.impl("gated_ffn", &mihvd::gated_ffn);
+  m.impl("_linear_cross_entropy", &mihvd::lce_forward);
+  m.impl("_linear_cross_entropy_backward", &mihvd::lce_backward);
+  m.impl("_gated_ffn", &mihvd::ffn_infer);
+  m.impl("_gated_ffn_train", &mihvd::ffn_train);
+  m.impl("_gated_ffn_backward", &mihvd::ffn_backward);
   m.impl("newton_schulz", &mihvd::newton_schulz);
   m.impl("muon_step", &mihvd::muon_step);
 }
 
-TORCH_LIBRARY_IMPL(mihvd, ADInplaceOrView, m) { m.impl("muon_step", &mihvd::muon_step_in_place); }
-
-TORCH_LIBRARY_IMPL(mihvd, AutogradCUDA, m) {
-  m.impl("linear_cross_entropy", &mihvd::linear_cross_entropy_autograd);
-  m.impl("gated_ffn", &mihvd::gated_ffn_autograd);
+TORCH_LIBRARY_IMPL(mihvd, Meta, m) {
+  m.impl("_linear_cross_entropy", &mihvd::lce_forward_meta);
+  m.impl("_linear_cross_entropy_backward", &mihvd::lce_backward_meta);
+  m.impl("_gated_ffn", &mihvd::ffn_infer_meta);
+  m.impl("_gated_ffn_train", &mihvd::ffn_train_meta);
+  m.impl("_gated_ffn_backward", &mihvd::ffn_backward_meta);
+  m.impl("newton_schulz", &mihvd::newton_schulz_meta);
+  m.impl("muon_step", &mihvd::muon_step_meta);
 }
+
+TORCH_LIBRARY_IMPL(mihvd, ADInplaceOrView, m) { m.impl("muon_step", &mihvd::muon_step_in_place); }

@@ -168,3 +168,28 @@ def test_plans_price_the_tiles_that_run(what, sizes):
         side, length = (-(-min(r, c) // 64) * 64, -(-max(r, c) // 64) * 64)
         got, tiles, args = _plan("orthogonalize", b, r, c, 1)[3], (64, 128), (side, length * b, side)
     assert got == min(tiles, key=lambda t: _estimate(t, *args))
+
+
+def test_fake_tensors_have_shapes():
+    """Tensors without data go through the operators' checks to the shapes and types of their results."""
+    from mihvd import _native
+    from mihvd.ops import gated_ffn, linear_cross_entropy
+    from mihvd.optim import orthogonalize
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    if not _native.load_kernels():
+        pytest.skip("no kernel library")
+    with FakeTensorMode():
+        def t(*s, dt=torch.bfloat16, **kw):
+            return torch.empty(*s, dtype=dt, device="cuda:0", **kw)
+
+        y = t(2, 5, dt=torch.long)
+        for grad in (True, False):
+            h, w, b = t(2, 5, 17, requires_grad=grad), t(33, 17, requires_grad=grad), t(33, dt=torch.float32)
+            for red, shape in (("mean", ()), ("sum", ()), ("none", (2, 5))):
+                out = linear_cross_entropy(h, w, y, b, reduction=red)
+                assert out.shape == shape and out.dtype == torch.float32 and out.requires_grad == grad
+            z = gated_ffn(h, t(12, 17), t(12, 17), t(17, 12), activation="gelu")
+            assert z.shape == h.shape and z.dtype == h.dtype and z.requires_grad == grad
+        x = t(3, 12, 17, dt=torch.float16)
+        assert orthogonalize(x).shape == x.shape and orthogonalize(x).dtype == x.dtype
