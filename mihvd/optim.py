@@ -392,8 +392,10 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         try:
-            self._checked(self.param_groups[-1])
-            for p in self.param_groups[-1]["params"]:
+            params = self._checked(self.param_groups[-1])["params"]
+            if len({id(p) for p in params}) != len(params):
+                raise ValueError("Muon: a parameter is listed twice (matrices run together: both updates would run at once)")
+            for p in params:
                 if p.dim() < 2:
                     raise ValueError("Muon: parameters must have at least two dimensions (got shape %s); give vectors to "
                                      "another optimizer" % (tuple(p.shape),))

@@ -193,3 +193,16 @@ def test_fake_tensors_have_shapes():
             assert z.shape == h.shape and z.dtype == h.dtype and z.requires_grad == grad
         x = t(3, 12, 17, dt=torch.float16)
         assert orthogonalize(x).shape == x.shape and orthogonalize(x).dtype == x.dtype
+
+
+def test_muon_refuses_a_parameter_twice():
+    from mihvd.optim import Muon
+
+    p, q = torch.nn.Parameter(torch.ones(4, 3)), torch.nn.Parameter(torch.ones(4, 3))
+    with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning, match="duplicate"):
+        Muon([p, q, p])
+    opt = Muon([q])
+    with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning, match="duplicate"):
+        opt.add_param_group(dict(params=[p, p]))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[p]))
