@@ -60,9 +60,10 @@ __global__ void __launch_bounds__(1024) lce_count(const int64_t* __restrict__ la
 // Compacts the labelled rows: their row numbers, their labels in 32 bits (-1: outside the vocabulary),
 // every row's place among them, their count, and their hidden vectors. A block takes 16 rows, a wave
 // each, and counts the labels ahead of them by itself: of all rows (up to 16384 of them: 64 KB a block on
-// average, out of L2), or of its chunk on top of the chunks' counts. (Blocks go round once more where there are
-// more rows than a launch of fewer than 2^32 threads has waves.)
+// average, out of L2), or of its chunk on top of the chunks' counts. AGAIN: blocks go round, where there are more
+// rows than a launch of fewer than 2^32 threads has waves (the loop costs 3 of 7 us at 8192 rows).
 constexpr int64_t GATHER_BLOCKS = int64_t(1) << 21;
+template <bool AGAIN>
 __global__ void __launch_bounds__(1024) lce_gather(const int64_t* __restrict__ labels, int N, int V, int64_t ignore,
                                                    const int* __restrict__ counts, int chunk, const u16* __restrict__ h,
                                                    int64_t s0, int64_t s1, int K, int K8, const LceRowsOut rw,
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(1024) lce_gather(const int64_t* __restrict__ l
     const int64_t r = first + w;
     const int64_t y = r < N ? labels[r] : ignore;
     const bool on = y != ignore;
-    if (first != (int64_t)blockIdx.x * 16) __syncthreads();  // own[] and sh[] have been read
+    if (AGAIN && first != (int64_t)blockIdx.x * 16) __syncthreads();  // own[] and sh[] have been read
     if (lane == 0) own[w] = on;
     int pos = count_block(n, sh);  // its barriers publish own[] too
 #pragma unroll
@@ -96,14 +97,16 @@ __global__ void __launch_bounds__(1024) lce_gather(const int64_t* __restrict__ l
       if (r == N - 1) *rw.cnt = pos + (on ? 1 : 0);
       if (r == 0) *rw.done = 0;
     }
-    if (!on) continue;
-    const u16* src = h + r * s0;
-    u16* dst = out + (int64_t)pos * K8;
-    if (s1 == 1 && (s0 & 7) == 0 && ((uintptr_t)h & 15) == 0 && K == K8) {
-      for (int k = lane * 8; k < K; k += 512) *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
-    } else {
-      for (int k = lane; k < K8; k += 64) dst[k] = k < K ? src[(int64_t)k * s1] : (u16)0;
+    if (on) {
+      const u16* src = h + r * s0;
+      u16* dst = out + (int64_t)pos * K8;
+      if (s1 == 1 && (s0 & 7) == 0 && ((uintptr_t)h & 15) == 0 && K == K8) {
+        for (int k = lane * 8; k < K; k += 512) *reinterpret_cast<uint4*>(dst + k) = *reinterpret_cast<const uint4*>(src + k);
+      } else {
+        for (int k = lane; k < K8; k += 64) dst[k] = k < K ? src[(int64_t)k * s1] : (u16)0;
+      }
     }
+    if (!AGAIN) return;
   }
 }
 
@@ -492,8 +495,13 @@ void lce_forward_16(const LceShape& s, const int64_t* labels, int64_t ignore, co
                     float2* part, float* zlab, float2* lse, float* rows, float* blocks, float* loss, int mean,
                     hipStream_t st) {
   if (s.chunk) lce_count<<<g16::cdiv(s.N, s.chunk), 1024, 0, st>>>(labels, s.N, ignore, s.chunk, rw.counts);
-  lce_gather<<<(int)std::min<int64_t>(g16::cdiv(s.N, 16), GATHER_BLOCKS), 1024, 0, st>>>(labels, s.N, s.V, ignore, s.chunk ? rw.counts : nullptr, s.chunk, h, hs0,
-                                                  hs1, s.K, s.K8, rw, hc);
+  const int64_t blocks16 = g16::cdiv(s.N, 16);
+  auto gather = [&](auto kernel) {
+    kernel<<<(int)std::min(blocks16, GATHER_BLOCKS), 1024, 0, st>>>(labels, s.N, s.V, ignore, s.chunk ? rw.counts : nullptr,
+                                                                   s.chunk, h, hs0, hs1, s.K, s.K8, rw, hc);
+  };
+  if (blocks16 <= GATHER_BLOCKS) gather(lce_gather<false>);
+  else gather(lce_gather<true>);
   g16::Args a;
   a.m.p[0] = hc;
   a.m.ld = s.K8;
