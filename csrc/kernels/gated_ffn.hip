@@ -54,8 +54,8 @@ __device__ __forceinline__ void act_both(float x, float& a, float& d) {
 }
 
 // Three outputs a tile (h, and g and u for training), so its end moves 192 KB: 8192 rows of 768 through
-// 2 x 2048 take 80 us (0.64 PFLOP/s; at 128x128 73 by itself, but the whole step 352 against 344:
-// power), 16384 of 2048 through 2 x 5632 680 to 730 us (1.04 to 1.11 PFLOP/s).
+// 2 x 2048 take 80 us (0.64 PFLOP/s; at 128x128 73 by itself, but the whole step 352 against 344),
+// 16384 of 2048 through 2 x 5632 680 to 730 us (1.04 to 1.11 PFLOP/s).
 template <int ACT>
 struct EpiGate {
   u16 *g, *u, *h;  // [N][F8]; g and u null without gradients

@@ -21,8 +21,8 @@
 // dimensions and KS extents that are multiples of 8 elements, KC rows that hold zeros (or any
 // finite values against zeros) from K to the next multiple of 8.
 //
-// Bound by the matrix pipe and by what a tile's end costs: plain bf16 products at 256x256 run at 1.02,
-// 1.31 and 1.45 PFLOP/s for K = 768, 2048 and 8192 (16384 square on this card's library: 1.65). A wave's
+// Bound by the matrix pipe and by what a tile's end costs: plain bf16 products of 8192 x 8192 at 256x256 run at
+// 0.97, 1.20 and 1.45 PFLOP/s for K = 768, 2048 and 8192 (the card's library: 1.10, 1.40 and 1.40). A wave's
 // 128x128 part reads 32 KB of LDS for 128 MFMAs, which is half the LDS's rate; at 64x64 a wave the LDS
 // reads and the copies into it together take as long as the MFMAs, hence 256x256 wherever there are tiles
 // enough. Giving every block an equal run of k tiles across output tiles was slower at every shape tried

@@ -20,7 +20,9 @@
 //
 // dz is held as (exp(z - lse) - onehot) * (g_r / G) * 2^shift with G = max |g_r|; G and 2^-shift come
 // back in the epilogues. bf16 needs no shift; fp16 takes 2^14, so that probabilities down to 4e-9
-// stay normal numbers (fp16's smallest is 6e-5) and 1.0 stays far from 65504.
+// stay normal numbers (fp16's smallest is 6e-5) and 1.0 stays far from 65504. With row weights that is a
+// probability times g_r / G: dW needs the weights inside its sum over rows, and one 16-bit dz serves both
+// products, so in fp16 rows far below the largest weight lose digits of their small probabilities.
 #include "gemm16.h"
 
 #include "transformer.h"
@@ -174,10 +176,10 @@ __device__ __forceinline__ float exp_from(float z, float top, float c) {
 }
 
 // Statistics of one wave's columns: part[row][piece] = (max, sum of exp(z - max)), and the label's logit.
-// A logit costs a read, half a max, two for the difference, an exponential (as long as four others) and an add: about 4 us a
-// 256x256 tile behind 17 us of products at K = 768. 1229 x 30522 x 768: 80 us (0.72 PFLOP/s, 600 tiles in
-// three rounds on 256 CUs; at 128x128 75 us by itself, the same in a training step); 8192 x 65536 x 1024:
-// 0.99 to 1.08 ms (1.0 to 1.1 PFLOP/s; at 128x128 1.2 to 1.26).
+// A logit costs a read, half a max, a subtraction, a product, an exponential (as long as four others) and an add:
+// about 4 us a
+// 256x256 tile behind 17 us of products at K = 768. 1229 x 30522 x 768: 84 us (0.69 PFLOP/s, 600 tiles in
+// three rounds on 256 CUs); 8192 x 65536 x 1024: 0.98 to 1.08 ms (1.0 to 1.1 PFLOP/s; at 128x128 1.2 to 1.26).
 template <bool BIAS>
 struct EpiStats {
   const void* bias;
@@ -234,7 +236,8 @@ struct EpiStats {
 };
 
 // Joins the pairs of every row: WPR waves a row, four where there are few rows, so that their loads are in
-// flight together. Writes lse (compact: maximum, log of the sum) and the row's loss (all rows), and into `out`, if given, their sum
+// flight together. Writes lse (compact: maximum, log of the sum) and the row's loss (all rows), and into `out`, if
+// given, their sum
 // or mean: every block adds up its rows, and the block that ends last adds up the blocks, both in a fixed
 // order.
 template <int WPR>
@@ -324,8 +327,8 @@ __global__ void __launch_bounds__(256) lce_finish(const float2* __restrict__ par
   }
 }
 
-// (1229 x 30522 x 768 with a bias at 128x128: 84 us; a piece of 32768 of 8192 x 65536 x 1024 at 256x256:
-// 560 to 590 us, 0.93 to 0.98 PFLOP/s, 0.54 GB of it written.)
+// (1229 x 30522 x 768 with a bias at 128x128: 86 us; a piece of 32768 of 8192 x 65536 x 1024 at 256x256:
+// 560 to 600 us, 0.92 to 0.98 PFLOP/s, 0.54 GB of it written.)
 // dz of one piece of the vocabulary (its columns start at v0), times DZ_SCALE, and with BIAS its sums over
 // the wave's rows (the bias gradient's terms). ROWS: rows have weights of their own. The scale is
 // folded into the exponent; the label's column is put right afterwards, by the one lane that has it.

@@ -9,8 +9,9 @@ autograd formulas are registered beside them in csrc/kernels/transformer_ops.cpp
 Both run on bf16 or fp16 MFMA operands with fp32 accumulation. Under ``torch.autocast`` fp32, bf16 and
 fp16 inputs are cast to the autocast type first, as for ``torch.nn.functional.linear``; otherwise the
 inputs must be 16-bit themselves. There is no CPU, fp32 or fp64 form: other inputs raise. Gradients are
-reverse-mode and of first order: forward-mode derivatives and gradients of gradients raise. Traced
-(fake tensors, ``torch.compile``), each is one node forward and one backward.
+reverse-mode and of first order: forward-mode derivatives, gradients of gradients and ``torch.func``'s
+gradient transforms raise. Traced (fake tensors, ``torch.compile``), each is one node forward and one
+backward.
 """
 from __future__ import annotations
 

@@ -256,6 +256,9 @@ class FusedSGD(torch.optim.Optimizer):
         return loss
 
 
+# Published with the update rule (K. Jordan et al., "Muon: an optimizer for hidden layers in neural networks", 2024), as
+# is the scale sqrt(max(1, rows / cols)); 0.2 sqrt(max(rows, cols)) is from J. Liu et al., "Muon is scalable for
+# LLM training", 2025.
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
@@ -313,11 +316,11 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
         X = x / (|x|_F + eps);   A = X X^T;   X <- a X + (b A + c A A) X        (a, b, c = coefficients)
 
     (on the smaller side; the default coefficients leave the singular values near 1 within about 0.3).
-    The result has ``x``'s type and shape, and takes no part in autograd (``x`` is detached). ``precision``: ``"fp16"`` — one fp16 product with fp32
-    accumulation per step, the default for 16-bit inputs — or ``"fp32"`` — three products over split
-    values (22 bits), the default for fp32. On the GPU it runs csrc/kernels/newton_schulz.hip, and
-    coefficients whose steps can take singular values past 15 are refused (fp16 planes hold X, A and the
-    polynomial); CPU tensors take the formula in fp32 torch operations.
+    The result has ``x``'s type and shape, and takes no part in autograd (``x`` is detached). ``precision``:
+    ``"fp16"`` — one fp16 product with fp32 accumulation per step, the default for 16-bit inputs, off by about
+    0.0016 of the result's norm — or ``"fp32"`` — three products over split values (22 bits), the default for
+    fp32. On the GPU it runs csrc/kernels/newton_schulz.hip, and coefficients whose steps can pass what fp16
+    planes hold of X, A and the polynomial are refused; CPU tensors take the formula in fp32 torch operations.
     """
     if x.dim() < 2:
         raise ValueError("orthogonalize: a matrix or a batch of matrices is needed (got shape %s)" % (tuple(x.shape),))
