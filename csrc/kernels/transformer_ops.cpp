@@ -670,6 +670,9 @@ void muon_step_in_place(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs, 
 //   gated_ffn [rows, hidden, inner]: the gate product's tile (0: few rows); tile, splits of y, dWd, dWg and dWu, dx
 //   orthogonalize [batch, rows, cols, planes]: tiles of X X^T, the polynomial, X's update, the last update
 std::vector<int64_t> transformer_plan(c10::string_view op, std::vector<int64_t> z) {
+  for (size_t i = 0; i < z.size(); ++i)
+    TORCH_CHECK_VALUE(z[i] >= (op == "linear_cross_entropy" && i == 3 ? 0 : 1) && z[i] <= MAX_LD, "transformer_plan: sizes within 1..",
+                      MAX_LD);
   if (op == "linear_cross_entropy" && z.size() == 4) {
     LceShape s{(int)z[0], (int)z[1], (int)up8(z[1]), (int)z[2], 0, 0, 0};
     LceScratch x{};
@@ -684,8 +687,8 @@ std::vector<int64_t> transformer_plan(c10::string_view op, std::vector<int64_t> 
     for (int i = 0; i < 4; ++i) r.insert(r.end(), {p.tile[i], p.splits[i]});
     return r;
   }
-  TORCH_CHECK_VALUE(op == "orthogonalize" && z.size() == 4, "transformer_plan: linear_cross_entropy, gated_ffn or orthogonalize "
-                    "and its sizes");
+  TORCH_CHECK_VALUE(op == "orthogonalize" && z.size() == 4 && z[0] <= NS_MAX && z[3] <= 2,
+                    "transformer_plan: linear_cross_entropy, gated_ffn or orthogonalize and its sizes");
   NsGroup g{};
   g.planes = (int)z[3];
   for (int64_t i = 0; i < z[0]; ++i) ns_add(g, z[1], z[2], nullptr, nullptr, nullptr, 0.f);

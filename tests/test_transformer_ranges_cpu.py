@@ -206,3 +206,15 @@ def test_muon_refuses_a_parameter_twice():
         opt.add_param_group(dict(params=[p, p]))
     assert len(opt.param_groups) == 1
     opt.add_param_group(dict(params=[p]))
+
+
+def test_plan_refusals():
+    from mihvd import _native
+
+    if not _native.load_kernels():
+        pytest.skip("no kernel library")
+    for op, sizes in (("linear_cross_entropy", [0, 8, 8, 1]), ("linear_cross_entropy", [8, 8, 8]), ("gated_ffn", [8, 0, 8]),
+                      ("gated_ffn", [8, 8, 8, 8]), ("orthogonalize", [0, 8, 8, 1]), ("orthogonalize", [1, 8, 8, 3]),
+                      ("orthogonalize", [33, 8, 8, 1]), ("gated_ffn", [1 << 40, 8, 8]), ("softmax", [1, 2, 3])):
+        with pytest.raises(ValueError, match="transformer_plan"):
+            torch.ops.mihvd.transformer_plan(op, sizes)
