@@ -264,3 +264,143 @@ def test_orthogonalize_far_norms(m, n, dt, by, eps):
     Muon([w], lr=1.0, momentum=0.5, eps=eps).step()
     want = ns64(x[0], eps=0.0) * math.sqrt(max(1.0, m / n))
     assert torch.linalg.vector_norm(w.detach().double().cpu() + want) <= 1.01 * ns_tol(want, dt, True)
+
+
+def test_row_weights_and_masks_captured():
+    """Per-row losses with weighted gradients and a masked vocabulary, captured once and replayed over new labels,
+    weights and masks in the same tensors."""
+    from mihvd.ops import linear_cross_entropy
+
+    n, k, v = 90, 72, 700
+    h, w, y, b = (t.cuda() for t in lce_case(n, k, v, BF, torch.float32, 71))
+    gr = torch.rand(n, generator=gen(72)).cuda()
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (h, w, b)]
+        rows = linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="none")
+        return (rows.detach(), *torch.autograd.grad(rows, leaves, gr))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in range(4):
+        g = gen(80 + seed)
+        off = torch.zeros(v, dtype=torch.bool)
+        off[100 * seed:100 * seed + 300] = True
+        new = torch.randint(0, v, (n,), generator=g)
+        new[off[new]] = -100
+        if seed == 3:
+            new.fill_(-100)  # nothing labelled
+        y.copy_(new)
+        gr.copy_(torch.randn(n, generator=g))
+        b.copy_(torch.where(off, torch.tensor(-1e30), torch.randn(v, generator=g)))
+        want = run()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), seed
+        assert all(torch.isfinite(p).all() for p in want)
+
+
+@pytest.mark.parametrize("dt", [BF, torch.float32], ids=["bf16", "fp32"])
+def test_muon_captured(dt):
+    """Steps of 16-bit parameters and of fp32 ones, channels_last among them, replayed from a graph."""
+    from mihvd.optim import Muon
+
+    def make():
+        g = gen(91)
+        ps = [torch.nn.Parameter(torch.randn(*s, generator=g).cuda().to(dt)) for s in ((24, 40), (40, 24), (16, 8, 3, 3))]
+        ps[2].data = ps[2].data.to(memory_format=torch.channels_last)
+        for p in ps:
+            p.grad = torch.empty_like(p)
+        return ps, Muon(ps, lr=0.05, weight_decay=0.1)
+
+    (a, oa), (c, oc) = make(), make()
+
+    def grads(seed):
+        g = gen(seed)
+        for p, q in zip(a, c):
+            d = torch.randn(*p.shape, generator=g).cuda()
+            p.grad.copy_(d)
+            q.grad.copy_(d)
+
+    grads(1)
+    oa.step()
+    oc.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oc.step()
+    for seed in range(2, 6):
+        grads(seed)
+        oa.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(a, c):
+            assert torch.equal(p, q) and torch.equal(oa.state[p]["momentum_buffer"], oc.state[q]["momentum_buffer"])
+
+
+def test_threads_on_their_own_streams():
+    """Two threads call the operators at once, each on a stream of its own."""
+    import threading
+
+    from mihvd.ops import gated_ffn, linear_cross_entropy
+    from mihvd.optim import orthogonalize
+    from test_transformer_gpu import ffn_case
+
+    def work(seed):
+        h, w, y, b = (t.cuda() for t in lce_case(150, 64, 900, BF, torch.float32, seed))
+        x, wg, wu, wd, dy = (t.cuda() for t in ffn_case(40 + seed, 64, 200, BF, seed))
+        lh, lx = h.requires_grad_(), x.requires_grad_()
+        loss, z = linear_cross_entropy(lh, w, y, b), gated_ffn(lx, wg, wu, wd)
+        return (loss.detach(), z.detach(), *torch.autograd.grad(loss, lh), *torch.autograd.grad(z, lx, dy),
+                orthogonalize(w.float()[:100]))
+
+    want = [work(s) for s in (1, 2)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def loop(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(5):
+                got = work(i + 1)
+                st.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_capture_beside_an_eager_graph_of_a_side_stream():
+    """The way out that the refusal names: an eager step run on a side stream may stay alive (as its loss does after
+    a warm-up loop) while the next one is captured."""
+    from test_transformer_steps_gpu import Stack
+
+    s = Stack()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = s.loss()
+        alive.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    want = [p.grad.clone() for p in s.params()]
+    for p in s.params():
+        p.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = s.loss()
+        loss.backward()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, alive) and all(torch.equal(p.grad, q) for p, q in zip(s.params(), want))
